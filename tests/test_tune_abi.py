@@ -1,0 +1,73 @@
+"""The second part of the C ABI (include/flux_hip_tune.h): every function is exported and bound, the ctypes structures have the
+layout of the header's, and bad arguments are refused before anything is launched (no GPU needed)."""
+import ctypes
+import os
+import re
+import subprocess
+
+import pytest
+
+from triton_kernels import _native as nv
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "flux_hip_tune.h")
+STRUCTS = {"flux_layer_norm_fwd_args": nv.LayerNormFwdArgs, "flux_layer_norm_bwd_args": nv.LayerNormBwdArgs}
+
+
+def text():
+    return re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+
+
+def test_every_declared_function_is_exported_and_bound():
+    names = set(re.findall(r"\b(flux_[a-z0-9_]+)\s*\(", text()))
+    assert names == set(nv.TUNE_SIGNATURES)
+    assert not names & set(nv.SIGNATURES)
+    version = int(re.search(r"#define FLUX_TUNE_ABI_VERSION (\d+)", text()).group(1))
+    assert nv.lib().flux_tune_abi_version() == nv.TUNE_ABI_VERSION == version
+
+
+def test_struct_layouts_match_the_header(tmp_path):
+    assert set(re.findall(r"typedef struct (\w+)", text())) == set(STRUCTS)
+    lines, want = [], []
+    for name, struct in STRUCTS.items():
+        lines.append(f'printf("%zu ", sizeof({name}));')
+        want.append(ctypes.sizeof(struct))
+        for field, _ in struct._fields_:
+            lines.append(f'printf("%zu ", offsetof({name}, {field}));')
+            want.append(getattr(struct, field).offset)
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "flux_hip_tune.h"\nint main(void){' + "\n".join(lines) + "return 0;}\n")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "sizes")], check=True)
+    assert [int(t) for t in subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.split()] == want
+
+
+BUF = ctypes.create_string_buffer(256)
+P = ctypes.addressof(BUF)
+
+
+def layer_norm_args(**kw):
+    return nv.LayerNormFwdArgs(**{**dict(x=P, w=P, b=P, y=P, batch=2, seq=3, x_sb=24, x_sl=8, groups=1, n=8, x_dtype=0, w_dtype=0, eps=1e-5), **kw})
+
+
+@pytest.mark.parametrize("change,rc", [(dict(x=None), -1), (dict(y=None), -1), (dict(mean=P), -1), (dict(batch=-1), -2), (dict(seq=-1), -2), (dict(n=0), -2), (dict(groups=3), -2),
+                                       (dict(n=65537), -5), (dict(batch=2**20, seq=2**20), -2), (dict(x_dtype=2), -3), (dict(x_dtype=1), -3), (dict(batch=0, x=None), 0)])
+def test_layer_norm_refusals(change, rc):
+    assert nv.lib().flux_layer_norm(ctypes.byref(layer_norm_args(**change)), None) == rc
+    assert nv.lib().flux_layer_norm(None, None) == -1
+
+
+@pytest.mark.parametrize("change,ws,rc", [(dict(dy=None), 1 << 20, -1), (dict(mean=None), 1 << 20, -1), (dict(groups=3), 1 << 20, -2), (dict(), 0, -1), (dict(n=70000), 1 << 20, -5),
+                                          (dict(x_dtype=1), 1 << 20, -3), (dict(dx=None, dw=None, db=None), 0, 0), (dict(batch=0), 1 << 20, -2), (dict(batch=0, dw=None, db=None), 0, 0)])
+def test_layer_norm_bwd_refusals(change, ws, rc):
+    a = nv.LayerNormBwdArgs(**{**dict(dy=P, x=P, w=P, mean=P, rstd=P, dx=P, dw=P, db=P, batch=2, seq=3, dy_sb=24, dy_sl=8, x_sb=24, x_sl=8, groups=1, n=8, x_dtype=0, w_dtype=0), **change})
+    assert nv.lib().flux_layer_norm_bwd(ctypes.byref(a), P if ws else None, ws, None) == rc
+
+
+def test_layer_norm_bwd_workspace():
+    a = nv.LayerNormBwdArgs(dy=P, x=P, w=P, mean=P, rstd=P, dx=P, dw=P, db=P, batch=4, seq=1000, dy_sb=8000, dy_sl=8, x_sb=8000, x_sl=8, groups=4, n=8, x_dtype=0, w_dtype=0)
+    need = nv.lib().flux_layer_norm_bwd_workspace_bytes(ctypes.byref(a))
+    assert need > 0 and need % (2 * 4 * 8 * 4) == 0
+    assert nv.lib().flux_layer_norm_bwd(ctypes.byref(a), P, need - 1, None) == -2      # too small
+    assert nv.lib().flux_layer_norm_bwd(ctypes.byref(a), P + 2, need, None) == -1      # not aligned
+    a.dw = a.db = None
+    assert nv.lib().flux_layer_norm_bwd_workspace_bytes(ctypes.byref(a)) == 0

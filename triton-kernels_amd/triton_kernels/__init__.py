@@ -6,12 +6,14 @@ from triton_kernels.functional import (
     apply_rope_torch_compile,
     layer_norm_modulation_torch,
     layer_norm_modulation_torch_compile,
+    layer_norm_torch,
     rms_norm_torch,
     rms_norm_torch_compile,
 )
 from triton_kernels.kernels import (
     apply_rope,
     attention_into,
+    layer_norm,
     layer_norm_modulation,
     linear,
     linear_into,
@@ -19,12 +21,12 @@ from triton_kernels.kernels import (
     rms_norm,
     scaled_dot_product_attention,
 )
-from triton_kernels.modules import DoubleStreamBlock, QKNorm, RMSNorm, SingleStreamBlock
+from triton_kernels.modules import DoubleStreamBlock, LayerNorm, QKNorm, RMSNorm, SingleStreamBlock
 
 __all__ = [
     "apply_rope_torch", "apply_rope_torch_compile", "layer_norm_modulation_torch",
-    "layer_norm_modulation_torch_compile", "rms_norm_torch", "rms_norm_torch_compile",
-    "apply_rope", "layer_norm_modulation", "linear", "rms_norm", "scaled_dot_product_attention",
+    "layer_norm_modulation_torch_compile", "layer_norm_torch", "rms_norm_torch", "rms_norm_torch_compile",
+    "apply_rope", "layer_norm", "layer_norm_modulation", "linear", "rms_norm", "scaled_dot_product_attention",
     "attention_into", "linear_into", "qkv_prep",
-    "DoubleStreamBlock", "QKNorm", "RMSNorm", "SingleStreamBlock",
+    "DoubleStreamBlock", "LayerNorm", "QKNorm", "RMSNorm", "SingleStreamBlock",
 ]

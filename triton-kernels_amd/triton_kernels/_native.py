@@ -100,6 +100,23 @@ class AttnArgs(Structure):
     ]
 
 
+class LayerNormFwdArgs(Structure):
+    _fields_ = [
+        ("x", c_void_p), ("w", c_void_p), ("b", c_void_p), ("y", c_void_p), ("mean", c_void_p), ("rstd", c_void_p),
+        ("batch", c_int64), ("seq", c_int64), ("x_sb", c_int64), ("x_sl", c_int64), ("groups", c_int64), ("w_sb", c_int64), ("b_sb", c_int64),
+        ("n", c_int32), ("x_dtype", c_int32), ("w_dtype", c_int32), ("plus_one", c_int32), ("eps", c_float),
+    ]
+
+
+class LayerNormBwdArgs(Structure):
+    _fields_ = [
+        ("dy", c_void_p), ("x", c_void_p), ("w", c_void_p), ("mean", c_void_p), ("rstd", c_void_p),
+        ("dx", c_void_p), ("dw", c_void_p), ("db", c_void_p),
+        ("batch", c_int64), ("seq", c_int64), ("dy_sb", c_int64), ("dy_sl", c_int64), ("x_sb", c_int64), ("x_sl", c_int64), ("groups", c_int64), ("w_sb", c_int64),
+        ("n", c_int32), ("x_dtype", c_int32), ("w_dtype", c_int32), ("plus_one", c_int32),
+    ]
+
+
 # name -> (restype, argtypes); also the list the symbol-export test walks.
 SIGNATURES = {
     "flux_abi_version": (c_int32, []),
@@ -136,6 +153,15 @@ SIGNATURES = {
                                      c_int32, c_int32, c_void_p]),
 }
 
+# The same for include/flux_hip_tune.h.
+TUNE_ABI_VERSION = 1
+TUNE_SIGNATURES = {
+    "flux_tune_abi_version": (c_int32, []),
+    "flux_layer_norm": (c_int32, [POINTER(LayerNormFwdArgs), c_void_p]),
+    "flux_layer_norm_bwd_workspace_bytes": (c_int64, [POINTER(LayerNormBwdArgs)]),
+    "flux_layer_norm_bwd": (c_int32, [POINTER(LayerNormBwdArgs), c_void_p, c_int64, c_void_p]),
+}
+
 
 def lib_path() -> str:
     return _LIB_PATH
@@ -153,11 +179,11 @@ def lib():
                 "(or `make -C triton-kernels_amd/csrc`). There is no fallback path."
             )
         handle = ctypes.CDLL(_LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **TUNE_SIGNATURES}.items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
-        if handle.flux_abi_version() != ABI_VERSION:
+        if handle.flux_abi_version() != ABI_VERSION or handle.flux_tune_abi_version() != TUNE_ABI_VERSION:
             raise RuntimeError("libfluxhip.so: ABI version mismatch")
         _lib = handle
     return _lib
@@ -269,6 +295,7 @@ def src4(t: torch.Tensor | None) -> Src4:
 
 __all__ = [
     "lib", "lib_path", "check", "last_error", "dtype_code", "require_gpu", "stream_ptr", "on_device", "ptr", "src4",
-    "Src4", "QkvPrepArgs", "LinearArgs", "LinearPairArgs", "LinearPlan", "RmsNormArgs", "LayerNormArgs", "AttnArgs", "SIGNATURES", "byref",
+    "Src4", "QkvPrepArgs", "LinearArgs", "LinearPairArgs", "LinearPlan", "RmsNormArgs", "LayerNormArgs", "AttnArgs", "LayerNormFwdArgs", "LayerNormBwdArgs",
+    "SIGNATURES", "TUNE_SIGNATURES", "byref",
     "FLUX_BF16", "FLUX_F32", "ACT_NONE", "ACT_GELU_TANH", "ACT_SILU", "LINEAR_SHARED_GPU", "MAX_ROW",
 ]

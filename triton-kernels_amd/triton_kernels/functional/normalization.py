@@ -16,6 +16,18 @@ def layer_norm_modulation_torch(x: Tensor, scale: Tensor, shift: Tensor) -> Tens
     return modulate(normed, scale=scale, shift=shift)
 
 
+def layer_norm_torch(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5, *, plus_one: bool = False) -> Tensor:
+    """Layer norm with weights of all rows ([N]) or of each batch element ([B, 1, N] beside an x of [B, L, N]) in float32, rounded once."""
+    xf = x.float()
+    d = xf - xf.mean(-1, keepdim=True)
+    y = d * torch.rsqrt(d.pow(2).mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * (weight.float() + 1 if plus_one else weight.float())
+    if bias is not None:
+        y = y + bias.float()
+    return y.to(x.dtype)
+
+
 def rms_norm_torch(x: Tensor, scale: Tensor) -> Tensor:
     xf = x.float()
     inv_rms = torch.rsqrt(xf.pow(2).mean(dim=-1, keepdim=True) + 1e-6)

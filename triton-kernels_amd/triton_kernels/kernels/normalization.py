@@ -1,8 +1,9 @@
-"""rms_norm and layer_norm_modulation: Python launchers over the HIP row-wise kernels.
+"""rms_norm, layer_norm_modulation and layer_norm: Python launchers over the HIP row-wise kernels.
 
 Same call signatures, defaults and assertion behaviour as kernels/normalization.py:47-77 and
 :142-193 of the reference; the device work is flux_rms_norm / flux_rms_norm_bwd /
-flux_layer_norm_modulation in libfluxhip.so.
+flux_layer_norm_modulation in libfluxhip.so. layer_norm, which the reference does not have, is the layer norm
+that can be trained (flux_layer_norm / flux_layer_norm_bwd).
 """
 from __future__ import annotations
 
@@ -199,3 +200,105 @@ def _layer_norm_args(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor):
     y = torch.empty_like(x)
     rows = x.numel() // n
     return (x.data_ptr(), weight.data_ptr(), bias.data_ptr(), y.data_ptr(), batch, rows // batch if batch else 0, mod_stride), y, (x, weight, bias)
+
+
+class _layer_norm(torch.autograd.Function):
+    """layer_norm of an x seen as [batch, seq, n], with weight and bias [groups, n] (or None)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, plus_one, grad_mode):
+        batch, seq, n = x.shape
+        dev = x.device
+        need_grad = grad_mode and any(ctx.needs_input_grad[:3])
+        y = torch.empty((batch, seq, n), dtype=x.dtype, device=dev)
+        stats = torch.empty((2, batch * seq), dtype=torch.float32, device=dev) if need_grad else (None, None)
+        a = nv.LayerNormFwdArgs(x.data_ptr(), nv.ptr(weight), nv.ptr(bias), y.data_ptr(), nv.ptr(stats[0]), nv.ptr(stats[1]),
+                                batch, seq, x.stride(0), x.stride(1), groups, weight.stride(0) if weight is not None else 0, bias.stride(0) if bias is not None else 0,
+                                n, nv.dtype_code(x), nv.dtype_code(x if weight is None and bias is None else weight if weight is not None else bias), plus_one, eps)
+        if batch * seq:
+            with nv.on_device(dev):
+                rc = nv.lib().flux_layer_norm(nv.byref(a), nv.stream_ptr(dev))
+            nv.check(rc, "flux_layer_norm")
+        if need_grad:
+            ctx.save_for_backward(x, weight, stats)
+            ctx.groups, ctx.plus_one, ctx.bias_dtype = groups, plus_one, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors   # (what saved-tensor hooks gave back)
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        dev = nv.require_gpu(dy, x, weight, stats)
+        batch, seq, n = dy.shape
+        groups = ctx.groups
+        if x.shape != dy.shape or stats.shape != (2, batch * seq) or (weight is not None and weight.shape != (groups, n)):
+            raise RuntimeError("layer_norm: saved tensors came back with other sizes")
+        x, dy = _unit_stride(x), _unit_stride(dy if dy.dtype == x.dtype else dy.to(x.dtype))
+        stats = stats.float().contiguous()
+        w_dtype = weight.dtype if weight is not None else ctx.bias_dtype or x.dtype
+        if weight is not None:
+            weight = _unit_stride(weight)
+        dx = torch.empty((batch, seq, n), dtype=x.dtype, device=dev) if want_x else None
+        sums = torch.empty if batch * seq else torch.zeros
+        dw = sums((groups, n), dtype=w_dtype, device=dev) if want_w else None
+        db = sums((groups, n), dtype=w_dtype, device=dev) if want_b else None
+        if batch * seq:
+            a = nv.LayerNormBwdArgs(dy.data_ptr(), x.data_ptr(), nv.ptr(weight), stats[0].data_ptr(), stats[1].data_ptr(), nv.ptr(dx), nv.ptr(dw), nv.ptr(db),
+                                    batch, seq, dy.stride(0), dy.stride(1), x.stride(0), x.stride(1), groups, weight.stride(0) if weight is not None else 0,
+                                    n, nv.dtype_code(x), nv._DTYPE_CODE[w_dtype], ctx.plus_one)
+            need = nv.lib().flux_layer_norm_bwd_workspace_bytes(nv.byref(a))
+            ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+            with nv.on_device(dev):
+                rc = nv.lib().flux_layer_norm_bwd(nv.byref(a), nv.ptr(ws), need, nv.stream_ptr(dev))
+            nv.check(rc, "flux_layer_norm_bwd")
+        return dx, dw, db, None, None, None, None
+
+
+def _unit_stride(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5, *, plus_one: bool = False) -> torch.Tensor:
+    """layer_norm(x) * weight + bias over the last dimension, with gradients for all three; rounded once.
+
+    weight, bias : [N], shared by all rows, or one for each element of x's first dimension, [B, N] or [B, 1, ..., N] (chunks of a wider modulation
+    tensor are read in place); either may be None. Their gradients are sums over the rows that share them, formed in fp32.
+    plus_one : the factor is 1 + weight, adaLN's scale. layer_norm_modulation is that operator for inference, in the rounding order of
+    PyTorch's bf16 operations and without gradients.
+    x is bf16 or fp32, [..., N] with N up to 65536; a bf16 x takes fp32 weights too.
+    """
+    nv.require_gpu(x, weight, bias)
+    assert x.dim() >= 1, "layer_norm needs at least one dimension"
+    nv.dtype_code(x)
+    n = x.shape[-1]
+    if n > nv.MAX_ROW:
+        calculate_settings(n)
+    batch = x.shape[0] if x.dim() > 1 else 1
+    per_batch = False
+    for t in (weight, bias):
+        if t is None:
+            continue
+        assert t.dim() >= 1 and t.shape[-1] == n, f"weight and bias are [{n}] or one such vector for each of {batch} batch elements, not {tuple(t.shape)}"
+        if t.numel() != n:
+            assert x.dim() > 1 and t.dim() > 1 and t.shape[0] == batch and t.numel() == batch * n, \
+                f"weight and bias are [{n}] or one such vector for each of {batch} batch elements, not {tuple(t.shape)}"
+            per_batch = True
+    groups = batch if per_batch else 1
+
+    def vectors(t, dtype):
+        if t is None:
+            return None
+        if t.dtype != dtype:
+            t = t.to(dtype)
+        t = t.reshape(-1, n)
+        return _unit_stride(t if t.shape[0] == groups else t.expand(groups, n))
+
+    w_dtype = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
+    if w_dtype != x.dtype and not (x.dtype == torch.bfloat16 and w_dtype == torch.float32):
+        w_dtype = x.dtype
+    if groups > 1 and any(t is not None and t.numel() == n for t in (weight, bias)):
+        w_dtype = torch.float32   # one of the two is shared: its gradient is the sum of the groups', which are not rounded before that
+    rows = _unit_stride(x.reshape(batch, -1, n)) if x.numel() else x.reshape(batch, x.numel() // max(1, batch * n), n)
+    y = _layer_norm.apply(rows, vectors(weight, w_dtype), vectors(bias, w_dtype), groups, float(eps), bool(plus_one), torch.is_grad_enabled())
+    return y.reshape(x.shape)

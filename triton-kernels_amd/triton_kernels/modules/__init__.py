@@ -9,9 +9,9 @@ from triton_kernels.modules.blocks import (
     SingleStreamBlock,
     attention,
 )
-from triton_kernels.modules.normalization import QKNorm, RMSNorm
+from triton_kernels.modules.normalization import LayerNorm, QKNorm, RMSNorm
 
 __all__ = [
     "MLP", "DoubleStreamBlock", "Linear", "LinearGELU", "Modulation", "ModulationOut", "SelfAttention",
-    "SingleStreamBlock", "attention", "QKNorm", "RMSNorm",
+    "SingleStreamBlock", "attention", "LayerNorm", "QKNorm", "RMSNorm",
 ]

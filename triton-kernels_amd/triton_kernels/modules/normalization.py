@@ -1,10 +1,10 @@
-"""RMSNorm / QKNorm modules on the HIP rms_norm (modules/normalization.py:8-26 of the reference).
-Parameter names (`scale`, `query_norm`, `key_norm`) are part of the state-dict contract."""
+"""RMSNorm / QKNorm modules on the HIP rms_norm (modules/normalization.py:8-26 of the reference) and LayerNorm on layer_norm.
+Parameter names (`scale`, `query_norm`, `key_norm`; torch.nn.LayerNorm's) are part of the state-dict contract."""
 import torch
 from torch import Tensor, nn
 from torch.nn.modules.module import _has_any_global_hook
 
-from triton_kernels.kernels.normalization import rms_norm, rms_norm_pair
+from triton_kernels.kernels.normalization import layer_norm, rms_norm, rms_norm_pair
 
 
 def plain(module: nn.Module, cls: type) -> bool:
@@ -33,3 +33,15 @@ class QKNorm(nn.Module):
             q, k = rms_norm_pair(q, self.query_norm.scale, k, self.key_norm.scale)
             return q.to(v), k.to(v)
         return self.query_norm(q).to(v), self.key_norm(k).to(v)
+
+
+class LayerNorm(nn.LayerNorm):
+    """torch.nn.LayerNorm over the last dimension on the HIP layer_norm, forward and backward."""
+
+    def __init__(self, normalized_shape: int, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True, device=None, dtype=None) -> None:
+        super().__init__(normalized_shape, eps, elementwise_affine, bias, device=device, dtype=dtype)
+        assert len(self.normalized_shape) == 1, "LayerNorm is over the last dimension"
+
+    def forward(self, input: Tensor) -> Tensor:
+        assert input.shape[-1:] == self.normalized_shape, f"expected rows of {self.normalized_shape[0]}, got {tuple(input.shape)}"
+        return layer_norm(input, self.weight, self.bias, self.eps)
