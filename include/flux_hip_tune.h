@@ -46,6 +46,36 @@ typedef struct flux_layer_norm_bwd_args {
 int64_t flux_layer_norm_bwd_workspace_bytes(const flux_layer_norm_bwd_args* args);
 int flux_layer_norm_bwd(const flux_layer_norm_bwd_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Rotary positions of several axes, straight from the tokens' ids.
+ * A row has P = sum(axes_dim) / 2 pairs (x[2i], x[2i+1]); the first axes_dim[0] / 2 of them belong to axis 0, and so on. Pair j of an axis of
+ * d values turns by the angle ids[b, l, axis] * theta^(-2j/d), formed in 64 bits.
+ * ids is [B, L, n_axes] with element strides (ids_sb, ids_sl, ids_sa), ids_sb = 0 for one list of positions for all batch elements.
+ * ------------------------------------------------------------------------------------------- */
+enum flux_ids_dtype { FLUX_IDS_F32 = 0, FLUX_IDS_F64 = 1, FLUX_IDS_I32 = 2, FLUX_IDS_I64 = 3 };
+enum { FLUX_ROPE_MOST_AXES = 8, FLUX_ROPE_MOST_DIM = 512 };
+typedef struct flux_rope_ids {
+    const void* ids; int64_t sb, sl, sa;
+    double theta;
+    int32_t dtype, n_axes, axes_dim[8];
+} flux_rope_ids;
+
+/* q_out = q and k_out = k with every pair turned by its angle ((x0 c - x1 s, x0 s + x1 c); inverse != 0: by the negative one, which is the
+ * backward pass). q is [B, Hq, L, D] and k [B, Hk, L, D] with strides as in flux_src4, D = 2 P; the outputs are contiguous. Either may be
+ * absent (null pointers and no heads). fp32 arithmetic, rounded once; sines and cosines are within 2^-23 of those of the 64-bit angle. */
+typedef struct flux_rope_nd_args {
+    flux_src4 q, k;
+    void* q_out; void* k_out;
+    flux_rope_ids at;
+    int64_t B, Hq, Hk, L;
+    int32_t D, dtype, inverse;
+} flux_rope_nd_args;
+int flux_rope_nd(const flux_rope_nd_args* args, void* stream);
+
+/* The rotation matrices themselves, as flux_qkv_prep and the q/k epilogue of flux_linear_bf16 take them:
+ * out[b, l, pair] = [[c, -s], [s, c]], fp32, contiguous [B, L, P, 2, 2]. */
+int flux_rope_table(const flux_rope_ids* at, float* out, int64_t B, int64_t L, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,7 +11,8 @@ from triton_kernels import _native as nv
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HEADER = os.path.join(ROOT, "include", "flux_hip_tune.h")
-STRUCTS = {"flux_layer_norm_fwd_args": nv.LayerNormFwdArgs, "flux_layer_norm_bwd_args": nv.LayerNormBwdArgs}
+STRUCTS = {"flux_layer_norm_fwd_args": nv.LayerNormFwdArgs, "flux_layer_norm_bwd_args": nv.LayerNormBwdArgs, "flux_rope_ids": nv.RopeIds,
+           "flux_rope_nd_args": nv.RopeNdArgs}
 
 
 def text():
@@ -71,3 +72,36 @@ def test_layer_norm_bwd_workspace():
     assert nv.lib().flux_layer_norm_bwd(ctypes.byref(a), P + 2, need, None) == -1      # not aligned
     a.dw = a.db = None
     assert nv.lib().flux_layer_norm_bwd_workspace_bytes(ctypes.byref(a)) == 0
+
+
+def rope_ids(**kw):
+    axes = kw.pop("axes", (16, 24, 24))
+    return nv.RopeIds(**{**dict(ids=P, sb=0, sl=3, sa=1, theta=10000.0, dtype=0, n_axes=len(axes), axes_dim=(ctypes.c_int32 * 8)(*axes[:8])), **kw})
+
+
+IDS_REFUSALS = [(dict(ids=None), -1), (dict(dtype=4), -3), (dict(dtype=-1), -3), (dict(n_axes=0), -2), (dict(n_axes=9), -2), (dict(axes=(16, 23, 25)), -2), (dict(axes=(64, 0)), -2),
+                (dict(axes=(-2, 66)), -2), (dict(axes=(256, 258)), -2), (dict(theta=0.0), -2), (dict(theta=float("inf")), -2), (dict(theta=float("nan")), -2)]
+
+
+@pytest.mark.parametrize("change,rc", IDS_REFUSALS)
+def test_rope_ids_refusals(change, rc):
+    at = rope_ids(**change)
+    src = nv.Src4(P, 0, 0, 0)
+    a = nv.RopeNdArgs(q=src, k=src, q_out=P, k_out=P, at=at, B=1, Hq=1, Hk=1, L=1, D=64)
+    assert nv.lib().flux_rope_nd(ctypes.byref(a), None) == rc
+    assert nv.lib().flux_rope_table(ctypes.byref(at), P, 1, 1, None) == rc
+
+
+@pytest.mark.parametrize("change,rc", [(dict(D=62), -2), (dict(B=-1), -2), (dict(L=-1), -2), (dict(Hq=-1), -2), (dict(L=2**31), -2), (dict(B=65536), -2), (dict(q_out=None), -1), (dict(k=nv.Src4()), -1),
+                                       (dict(dtype=2), -3), (dict(L=0), 0), (dict(B=0), 0), (dict(Hq=0, Hk=0), 0)])
+def test_rope_nd_refusals(change, rc):
+    src = nv.Src4(P, 0, 0, 0)
+    a = nv.RopeNdArgs(**{**dict(q=src, k=src, q_out=P, k_out=P, at=rope_ids(), B=1, Hq=1, Hk=1, L=1, D=64), **change})
+    assert nv.lib().flux_rope_nd(ctypes.byref(a), None) == rc
+    assert nv.lib().flux_rope_nd(None, None) == -1
+
+
+def test_rope_table_refusals():
+    at, call = ctypes.byref(rope_ids()), nv.lib().flux_rope_table
+    assert call(at, None, 1, 1, None) == -1 and call(None, P, 1, 1, None) == -1 and call(at, P, -1, 1, None) == -2 and call(at, P, 1, 2**31, None) == -2
+    assert call(at, P + 4, 1, 1, None) == -4 and call(at, P, 2**20, 2**20, None) == -2 and call(at, P, 0, 5, None) == 0

@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import sys
-from ctypes import POINTER, Structure, byref, c_char_p, c_float, c_int32, c_int64, c_void_p
+from ctypes import POINTER, Structure, byref, c_char_p, c_double, c_float, c_int32, c_int64, c_void_p
 
 import torch
 
@@ -117,6 +117,20 @@ class LayerNormBwdArgs(Structure):
     ]
 
 
+class RopeIds(Structure):
+    _fields_ = [
+        ("ids", c_void_p), ("sb", c_int64), ("sl", c_int64), ("sa", c_int64), ("theta", c_double),
+        ("dtype", c_int32), ("n_axes", c_int32), ("axes_dim", c_int32 * 8),
+    ]
+
+
+class RopeNdArgs(Structure):
+    _fields_ = [
+        ("q", Src4), ("k", Src4), ("q_out", c_void_p), ("k_out", c_void_p), ("at", RopeIds),
+        ("B", c_int64), ("Hq", c_int64), ("Hk", c_int64), ("L", c_int64), ("D", c_int32), ("dtype", c_int32), ("inverse", c_int32),
+    ]
+
+
 # name -> (restype, argtypes); also the list the symbol-export test walks.
 SIGNATURES = {
     "flux_abi_version": (c_int32, []),
@@ -160,6 +174,8 @@ TUNE_SIGNATURES = {
     "flux_layer_norm": (c_int32, [POINTER(LayerNormFwdArgs), c_void_p]),
     "flux_layer_norm_bwd_workspace_bytes": (c_int64, [POINTER(LayerNormBwdArgs)]),
     "flux_layer_norm_bwd": (c_int32, [POINTER(LayerNormBwdArgs), c_void_p, c_int64, c_void_p]),
+    "flux_rope_nd": (c_int32, [POINTER(RopeNdArgs), c_void_p]),
+    "flux_rope_table": (c_int32, [POINTER(RopeIds), c_void_p, c_int64, c_int64, c_void_p]),
 }
 
 
@@ -295,7 +311,7 @@ def src4(t: torch.Tensor | None) -> Src4:
 
 __all__ = [
     "lib", "lib_path", "check", "last_error", "dtype_code", "require_gpu", "stream_ptr", "on_device", "ptr", "src4",
-    "Src4", "QkvPrepArgs", "LinearArgs", "LinearPairArgs", "LinearPlan", "RmsNormArgs", "LayerNormArgs", "AttnArgs", "LayerNormFwdArgs", "LayerNormBwdArgs",
+    "Src4", "QkvPrepArgs", "LinearArgs", "LinearPairArgs", "LinearPlan", "RmsNormArgs", "LayerNormArgs", "AttnArgs", "LayerNormFwdArgs", "LayerNormBwdArgs", "RopeIds", "RopeNdArgs",
     "SIGNATURES", "TUNE_SIGNATURES", "byref",
     "FLUX_BF16", "FLUX_F32", "ACT_NONE", "ACT_GELU_TANH", "ACT_SILU", "LINEAR_SHARED_GPU", "MAX_ROW",
 ]

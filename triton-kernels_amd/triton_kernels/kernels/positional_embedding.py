@@ -1,6 +1,9 @@
 """apply_rope: rotate q and k by per-position 2x2 matrices (kernels/positional_embedding.py:55-82 of
-the reference), plus the fused gather flux_qkv_prep it is a special case of."""
+the reference), plus the fused gather flux_qkv_prep it is a special case of. apply_rope_nd, which the reference
+does not have, rotates by positions of several axes without such matrices, and rope_table makes them."""
 from __future__ import annotations
+
+import ctypes
 
 import torch
 from torch import Tensor
@@ -115,3 +118,121 @@ def apply_rope(xq: Tensor, xk: Tensor, freqs_cis: Tensor) -> tuple[Tensor, Tenso
     assert xq.dim() == 4 and xq.shape == xk.shape and xq.dtype == xk.dtype
     q, k, _ = qkv_prep(xq, xk, None, pe=freqs_cis)
     return q, k
+
+
+_IDS_DTYPE = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}
+
+
+def _not_differentiated(ids: Tensor) -> None:
+    if torch.is_grad_enabled() and ids.requires_grad:
+        raise NotImplementedError("positions are not differentiated")
+
+
+def _rope_ids(ids: Tensor, axes_dim, theta: float, B: int | None = None, L: int | None = None) -> tuple["nv.RopeIds", Tensor]:
+    """The positions as the library takes them, and what has to live until the launch."""
+    axes = [int(d) for d in axes_dim]
+    assert ids.dim() in (2, 3) and ids.shape[-1] == len(axes), f"ids must be [L, {len(axes)}] or [B, L, {len(axes)}], got {tuple(ids.shape)}"
+    assert 1 <= len(axes) <= 8 and all(d > 0 and d % 2 == 0 for d in axes), f"one to eight axes of an even number of values, got {axes}"
+    if L is not None:
+        assert ids.shape[-2] == L and (ids.dim() == 2 or ids.shape[0] in (1, B)), f"ids of shape {tuple(ids.shape)} for {B} sequences of {L}"
+    if ids.dtype not in _IDS_DTYPE:
+        if ids.dtype == torch.bool or ids.is_complex():
+            raise TypeError(f"unsupported dtype {ids.dtype} of ids")
+        ids = ids.float() if ids.is_floating_point() else ids.to(torch.int64)
+    sb = ids.stride(0) if ids.dim() == 3 and ids.shape[0] > 1 else 0
+    return nv.RopeIds(ids.data_ptr(), sb, ids.stride(-2), ids.stride(-1), float(theta), _IDS_DTYPE[ids.dtype], len(axes), (ctypes.c_int32 * 8)(*axes)), ids
+
+
+def _rotated(q: Tensor | None, k: Tensor | None, ids: Tensor, axes_dim, theta: float, inverse: bool) -> tuple[Tensor | None, Tensor | None]:
+    ref = q if q is not None else k
+    B, _, L, D = ref.shape
+    dev = nv.require_gpu(q, k, ids)
+    at, keep = _rope_ids(ids, axes_dim, theta, B, L)
+    outs = []
+    a = nv.RopeNdArgs(at=at, B=B, L=L, D=D, dtype=nv.dtype_code(ref), inverse=inverse)
+    for name, x in (("q", q), ("k", k)):
+        if x is None:
+            outs.append(None)
+            continue
+        if x.stride(3) != 1:
+            x = x.contiguous()
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        setattr(a, name, nv.src4(x))
+        setattr(a, f"{name}_out", out.data_ptr())
+        setattr(a, f"H{name}", x.shape[1])
+        keep = (keep, x)
+        outs.append(out)
+    with nv.on_device(dev):
+        rc = nv.lib().flux_rope_nd(nv.byref(a), nv.stream_ptr(dev))
+    nv.check(rc, "flux_rope_nd")
+    return tuple(outs)
+
+
+class _apply_rope_nd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, xq, xk, ids, axes_dim, theta):
+        ctx.save_for_backward(ids)
+        ctx.set_materialize_grads(False)
+        ctx.axes_dim, ctx.theta = axes_dim, theta
+        return _rotated(xq, xk, ids, axes_dim, theta, False)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        """A rotation's backward pass is the rotation by the negative angles."""
+        if dq is None and dk is None:
+            return None, None, None, None, None
+        ids, = ctx.saved_tensors
+        dq = dq if ctx.needs_input_grad[0] else None
+        dk = dk if ctx.needs_input_grad[1] else None
+        return (*_apply_rope_nd_inverse.apply(dq, dk, ids, ctx.axes_dim, ctx.theta), None, None, None)
+
+
+class _apply_rope_nd_inverse(torch.autograd.Function):
+    """The backward pass as a function of its own, so that it is differentiable in turn."""
+
+    @staticmethod
+    def forward(ctx, dq, dk, ids, axes_dim, theta):
+        ctx.save_for_backward(ids)
+        ctx.set_materialize_grads(False)
+        ctx.axes_dim, ctx.theta = axes_dim, theta
+        return _rotated(dq, dk, ids, axes_dim, theta, True)
+
+    @staticmethod
+    def backward(ctx, q, k):
+        if q is None and k is None:
+            return None, None, None, None, None
+        ids, = ctx.saved_tensors
+        return (*_apply_rope_nd.apply(q, k, ids, ctx.axes_dim, ctx.theta), None, None, None)
+
+
+def apply_rope_nd(xq: Tensor, xk: Tensor | None, ids: Tensor, axes_dim, theta: float = 10000.0) -> tuple[Tensor, Tensor | None]:
+    """q and k rotated by positions of several axes (time, height, width), with gradients for both.
+
+    xq, xk : [B, H, L, D] views with any strides; xk may have another number of heads or be None. bf16 or fp32.
+    ids : the tokens' positions, [B, L, n] or [L, n] for all batch elements: float32, float64, int32 or int64 (others are converted).
+    axes_dim : values of a row that belong to each of the n axes, in order; even, D in all, at most 512.
+    Pair j of an axis of d values turns by ids[b, l, axis] * theta^(-2j/d), formed in 64 bits: apply_rope with EmbedND's table, without the
+    table. The results are contiguous and rounded once.
+    """
+    for x in (xq, xk):
+        assert x is None or (x.dim() == 4 and x.dtype == xq.dtype), "q and k are [B, H, L, D] of one type"
+    B, _, L, D = xq.shape
+    assert xk is None or (xk.shape[0], *xk.shape[2:]) == (B, L, D), f"q {tuple(xq.shape)} and k {tuple(xk.shape)} differ in more than their heads"
+    axes = tuple(int(d) for d in axes_dim)
+    assert sum(axes) == D, f"axes of {sum(axes)} values in all for rows of {D}"
+    _not_differentiated(ids)
+    return _apply_rope_nd.apply(xq, xk, ids, axes, float(theta))
+
+
+def rope_table(ids: Tensor, axes_dim, theta: float = 10000.0) -> Tensor:
+    """The fp32 rotation matrices that the blocks and apply_rope take, [B, 1, L, D/2, 2, 2] for ids [B, L, n] ([1, 1, ...] for [L, n]):
+    one kernel for what EmbedND of the plain blocks computes; arguments as in apply_rope_nd."""
+    dev = nv.require_gpu(ids)
+    _not_differentiated(ids)
+    at, _keep = _rope_ids(ids, axes_dim, theta)
+    B, L = ids.shape[0] if ids.dim() == 3 else 1, ids.shape[-2]
+    out = torch.empty((B, 1, L, sum(at.axes_dim) // 2, 2, 2), dtype=torch.float32, device=dev)
+    with nv.on_device(dev):
+        rc = nv.lib().flux_rope_table(nv.byref(at), out.data_ptr(), B, L, nv.stream_ptr(dev))
+    nv.check(rc, "flux_rope_table")
+    return out
