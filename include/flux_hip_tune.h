@@ -76,6 +76,28 @@ int flux_rope_nd(const flux_rope_nd_args* args, void* stream);
  * out[b, l, pair] = [[c, -s], [s, c]], fp32, contiguous [B, L, P, 2, 2]. */
 int flux_rope_table(const flux_rope_ids* at, float* out, int64_t B, int64_t L, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * A projection shared by many requests, each with a low-rank adapter of its own:
+ *   y[m] = act(x[m] W^T + bias + s_i (x[m] a_i^T) b_i^T),  i = adapter[m / (M / requests)]
+ * x [M, K] (row stride ldx), w [N, K] (row stride ldw), bias [N] or null, y [M, N] (row stride ldy) as in flux_linear_bf16, bf16; act
+ * is FLUX_ACT_NONE or FLUX_ACT_GELU_TANH. lora_a is [adapters, rank, K], lora_b [adapters, N, rank], contiguous bf16, with rank up to
+ * FLUX_LORA_MOST_RANK; scaling is fp32 [adapters] or null (1). adapter holds one number for each of `requests` groups of M / requests rows that
+ * follow one another, int32 or (wide_ids) int64; a number outside [0, adapters) means no adapter, and nothing of lora_a and lora_b is read for it.
+ * fp32 sums; s_i x a_i^T is rounded to bf16 once, y once. What is not finite in an adapter reaches rows of its own requests only.
+ * The workspace (flux_linear_lora_workspace_bytes; 256-byte aligned, the launch's own until it has run) holds s_i x a_i^T and, where K is cut
+ * over workgroups, partial sums; flux_linear_lora_least_bytes is what the call cannot do without.
+ * ------------------------------------------------------------------------------------------- */
+#define FLUX_LORA_MOST_RANK 256
+typedef struct flux_linear_lora_args {
+    const void* x; const void* w; const void* bias; void* y;
+    const void* lora_a; const void* lora_b; const void* adapter; const float* scaling;
+    int64_t M, N, K, ldx, ldw, ldy, requests;
+    int32_t adapters, rank, wide_ids, act;
+} flux_linear_lora_args;
+int64_t flux_linear_lora_workspace_bytes(const flux_linear_lora_args* args);
+int64_t flux_linear_lora_least_bytes(const flux_linear_lora_args* args);
+int flux_linear_lora_bf16(const flux_linear_lora_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

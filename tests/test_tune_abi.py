@@ -12,7 +12,7 @@ from triton_kernels import _native as nv
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HEADER = os.path.join(ROOT, "include", "flux_hip_tune.h")
 STRUCTS = {"flux_layer_norm_fwd_args": nv.LayerNormFwdArgs, "flux_layer_norm_bwd_args": nv.LayerNormBwdArgs, "flux_rope_ids": nv.RopeIds,
-           "flux_rope_nd_args": nv.RopeNdArgs}
+           "flux_rope_nd_args": nv.RopeNdArgs, "flux_linear_lora_args": nv.LinearLoraArgs}
 
 
 def text():
@@ -105,3 +105,33 @@ def test_rope_table_refusals():
     at, call = ctypes.byref(rope_ids()), nv.lib().flux_rope_table
     assert call(at, None, 1, 1, None) == -1 and call(None, P, 1, 1, None) == -1 and call(at, P, -1, 1, None) == -2 and call(at, P, 1, 2**31, None) == -2
     assert call(at, P + 4, 1, 1, None) == -4 and call(at, P, 2**20, 2**20, None) == -2 and call(at, P, 0, 5, None) == 0
+
+
+def lora_args(**kw):
+    return nv.LinearLoraArgs(**{**dict(x=P, w=P, bias=P, y=P, lora_a=P, lora_b=P, adapter=P, scaling=P, M=4, N=16, K=8, ldx=8, ldw=8, ldy=16, requests=2, adapters=3, rank=4), **kw})
+
+
+WS = ctypes.create_string_buffer(1 << 16)
+WS_AT = (ctypes.addressof(WS) + 255) // 256 * 256
+
+
+@pytest.mark.parametrize("change,rc", [(dict(x=None), -1), (dict(w=None), -1), (dict(y=None), -1), (dict(lora_a=None), -1), (dict(lora_b=None), -1), (dict(adapter=None), -1), (dict(M=-1), -2),
+                                       (dict(N=2**31), -2), (dict(ldx=7), -2), (dict(ldw=7), -2), (dict(ldy=15), -2), (dict(adapters=0), -2), (dict(rank=0), -2), (dict(rank=257), -2),
+                                       (dict(requests=3), -2), (dict(requests=0), -2), (dict(requests=-4), -2), (dict(act=2), -6), (dict(M=2**28, requests=1), -2),
+                                       (dict(M=2**20, N=2**14, K=7, ldx=7, ldw=7, ldy=2**14), -2), (dict(M=0), 0), (dict(N=0), 0)])
+def test_linear_lora_refusals(change, rc):
+    a = ctypes.byref(lora_args(**change))
+    assert nv.lib().flux_linear_lora_bf16(a, WS_AT, 1 << 15, None) == rc
+    if rc:
+        assert nv.lib().flux_linear_lora_workspace_bytes(a) == nv.lib().flux_linear_lora_least_bytes(a) == 0
+
+
+def test_linear_lora_workspace():
+    call, a = nv.lib().flux_linear_lora_bf16, lora_args()
+    least = nv.lib().flux_linear_lora_least_bytes(ctypes.byref(a))
+    assert least == nv.lib().flux_linear_lora_workspace_bytes(ctypes.byref(a)) == 512                # 4 rows of 32 values, 4 adapters' numbers
+    assert call(ctypes.byref(a), None, 1 << 15, None) == -1 and call(ctypes.byref(a), WS_AT + 16, 1 << 15, None) == -1
+    assert call(ctypes.byref(a), WS_AT, least - 1, None) == -2 and call(None, WS_AT, least, None) == -1
+    cut = lora_args(M=64, N=2048, K=16384, ldx=16384, ldw=16384, ldy=2048, rank=40)
+    assert nv.lib().flux_linear_lora_least_bytes(ctypes.byref(cut)) == 64 * 64 * 2 + 256
+    assert nv.lib().flux_linear_lora_workspace_bytes(ctypes.byref(cut)) > 64 * 64 * 2 + 256            # K in parts

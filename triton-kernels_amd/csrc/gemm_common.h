@@ -560,5 +560,8 @@ inline unsigned grid_of(const GemmLaunch& L) { return static_cast<unsigned>((L.t
 
 // Eight-wave tiles (gemm_pair.hip). K range in `splits` parts, which then need `partial`.
 void launch_pair_tiles(int fm, int fn, const GemmSet& g, int splits, float* partial, hipStream_t st);
+// Their first half: the sums of the parts, which the launch that comes back has in its `partial` (splits == 1 there: nothing was launched, K is one part).
+GemmLaunch launch_pair_parts(int fm, int fn, const GemmSet& g, int splits, float* partial, hipStream_t st);
+GemmLaunch make_pair_launch(const GemmSet& g, int fm, int fn);
 
 }  // namespace flux

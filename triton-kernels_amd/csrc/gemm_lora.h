@@ -1,0 +1,184 @@
+// Low-rank adapters beside a shared projection: what the kernels add to the sums of a tile before its epilogue.
+//
+//   y[m] = act(x[m] W^T + bias + s_i (x[m] a_i^T) b_i^T),  i = the adapter of row m's request
+//
+// Two launches. The first one (lora_low_kernel) works out low[m] = s_i x[m] a_i^T, a few values a row, and rounds it to bf16, which the matrix
+// instructions of the second take: an error of 2^-9 of the adapter's own terms, below what y's rounding to bf16 leaves. The second one is
+// the product with W as ever; when a tile's sums are complete, low b_i^T is multiplied onto them from registers, K = 32 of the rank a step. So y
+// is written once and rounded once, and the adapter costs rank / K of the product's own time.
+#pragma once
+
+#include "gemm_common.h"
+#include "gemm_rows.h"
+
+namespace flux {
+
+struct LoraTail {
+    const bf16_t* low;     // [M][width]: zero from the rank on
+    const int* owner;      // [M]: the row's adapter, -1: none
+    const bf16_t* b;       // [adapters][N][rank]
+    int rank, width;       // width: rank rounded up to whole steps of 32
+    int vec;               // 1: rows of b may be read 16 bytes at a time
+
+    // Adds to the fragment rows of a wave: rows m0 .. of the product, columns n0 ... The adapters among the wave's rows are taken one after the
+    // other in rising order, each with one read of its columns of b; rows of another adapter count as zeros. 0 * inf would still reach them, so
+    // where a wave's rows are not of one adapter, what is not finite in b is taken out and makes its own rows NaN by itself: products of 3e38
+    // and 3e38 and of 3e38 and -3e38, which are zero for all other rows. (The sums are touched by matrix instructions only: choosing
+    // between old and new sums by row, with vector instructions, spilled 600 registers of the 256-wide tile.)
+    template <int ROWS, int FN>
+    __device__ __forceinline__ void operator()(f32x4 (&acc)[ROWS][FN], int m0, int n0, const GemmParams& p) const {
+        if (m0 >= p.M || n0 >= p.N) return;
+        const int lane = threadIdx.x & 63, frow = lane & 15, fq = lane >> 4;
+        int own[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) own[i] = owner[min(m0 + i * 16 + frow, p.M - 1)];
+        constexpr int kNone = 0x7fffffff;
+        auto behind = [&](int last) {   // the next adapter of these rows
+            int next = kNone;
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) next = own[i] > last ? min(next, own[i]) : next;
+            return first_of_rows(next);
+        };
+        int a = behind(-1);
+        if (a == kNone) return;
+        bool same = true;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) same = same && own[i] == a;
+        const bool all = __ballot(same) == ~uint64_t{0};
+        for (int k = 0;;) {
+            u32x4 wb[FN], xa[ROWS];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) wb[j] = piece(b + (static_cast<int64_t>(a) * p.N + min(n0 + j * 16 + frow, p.N - 1)) * rank, k + fq * 8);
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) xa[i] = *reinterpret_cast<const u32x4*>(low + static_cast<int64_t>(min(m0 + i * 16 + frow, p.M - 1)) * width + k + fq * 8);
+            __builtin_amdgcn_sched_barrier(0);   // the loads stay in front of the products
+            auto multiply = [&](const u32x4 (&w)[FN], auto x) {
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) {
+                    const bf16x8 xi = __builtin_bit_cast(bf16x8, x(i));
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[j]), xi, acc[i][j], 0, 0, 0);
+                }
+            };
+            if (!all) {
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) xa[i] = own[i] == a ? xa[i] : u32x4{0, 0, 0, 0};
+                uint32_t bad = 0;
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) bad |= not_finite(wb[j][e]);
+                if (__ballot(bad != 0) != 0) {
+                    u32x4 huge[FN];
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t n = not_finite(wb[j][e]);
+                            huge[j][e] = n & 0x7f7f7f7fu;
+                            wb[j][e] &= ~n;
+                        }
+                    multiply(huge, [&](int i) { const uint32_t h = own[i] == a ? 0x7f7f7f7fu : 0u; return u32x4{h, h, h, h}; });
+                    multiply(huge, [&](int i) { const uint32_t h = own[i] == a ? 0xff7fff7fu : 0u; return u32x4{h, h, h, h}; });
+                }
+            }
+            multiply(wb, [&](int i) { return xa[i]; });
+            k += 32;
+            if (k >= width) {
+                k = 0;
+                a = behind(a);
+                if (a == kNone) break;
+            }
+        }
+    }
+
+    // All ones in the halves of a word that are infinite or NaN.
+    static __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+        return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+    }
+
+    // The smallest value of the wave's 16 rows (lanes 16 apart hold the same row), as a scalar.
+    static __device__ __forceinline__ int first_of_rows(int v) {
+        v = min(v, __shfl_xor(v, 1));
+        v = min(v, __shfl_xor(v, 2));
+        v = min(v, __shfl_xor(v, 4));
+        v = min(v, __shfl_xor(v, 8));
+        return __builtin_amdgcn_readfirstlane(v);
+    }
+
+    // Values k .. k + 7 of a row of `rank` values, zero from its end on.
+    __device__ __forceinline__ u32x4 piece(const bf16_t* row, int k) const {
+        if (vec) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(row + (k < rank ? k : 0));
+            return k < rank ? v : u32x4{0, 0, 0, 0};
+        }
+        u32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            v[e] = (k + 2 * e < rank ? row[k + 2 * e] : 0u) | (k + 2 * e + 1 < rank ? static_cast<uint32_t>(row[k + 2 * e + 1]) << 16 : 0u);
+        return v;
+    }
+};
+
+// The same for row vectors (gemm_rows.h): lane l adds the products of the rank's values l, l + 64, ... to its share of a sum. The first 64 of
+// them are requested in front of W.
+template <int MM>
+struct LoraRowTail {
+    LoraTail t;
+    int own[MM];
+    bf16_t low[MM], b[kGemvCols][MM];
+    int64_t row_b[kGemvCols][MM];
+
+    __device__ __forceinline__ void request(int n0, int lane, const GemmParams& p) {
+        const int r = lane < t.rank ? lane : 0;
+#pragma unroll
+        for (int m = 0; m < MM; ++m) {
+            own[m] = t.owner[m];
+            low[m] = t.low[static_cast<int64_t>(m) * t.width + r];
+#pragma unroll
+            for (int c = 0; c < kGemvCols; ++c) {
+                row_b[c][m] = (static_cast<int64_t>(max(own[m], 0)) * p.N + min(n0 + c, p.N - 1)) * t.rank;
+                b[c][m] = t.b[row_b[c][m] + r];
+            }
+        }
+    }
+    __device__ __forceinline__ void add(float (&acc)[kGemvCols][MM], int lane) {
+#pragma unroll
+        for (int m = 0; m < MM; ++m)
+#pragma unroll
+            for (int c = 0; c < kGemvCols; ++c) acc[c][m] += own[m] >= 0 && lane < t.rank ? bf2f(low[m]) * bf2f(b[c][m]) : 0.0f;
+        for (int r = 64 + lane; r < t.rank; r += 64)
+#pragma unroll
+            for (int m = 0; m < MM; ++m) {
+                const float l = bf2f(t.low[static_cast<int64_t>(m) * t.width + r]);
+#pragma unroll
+                for (int c = 0; c < kGemvCols; ++c) acc[c][m] += own[m] >= 0 ? l * bf2f(t.b[row_b[c][m] + r]) : 0.0f;
+            }
+    }
+};
+
+// The tail of a launch whose rows begin `rows` further on.
+inline LoraTail tail_behind(LoraTail t, int64_t rows) {
+    t.low += rows * t.width;
+    t.owner += rows;
+    return t;
+}
+
+void launch_lora_square(const GemmSet& g, const LoraTail& tail, hipStream_t st);
+void launch_lora_rect(int fm, int fn, const GemmSet& g, const LoraTail& tail, hipStream_t st);
+void launch_lora_pair(int fm, int fn, const GemmSet& g, int splits, float* partial, const LoraTail& tail, hipStream_t st);
+void launch_lora_rows(const GemmParams& p, const LoraTail& tail, hipStream_t st);
+void launch_lora_scalar(const GemmParams& p, const LoraTail& tail, hipStream_t st);
+
+// The first launch: low and owner.
+struct LoraLow {
+    const bf16_t* x; const bf16_t* a; const void* adapter; const float* scaling;
+    bf16_t* low; int* owner;
+    int64_t lda, rows_per_request;
+    int M, K, rank, width, adapters;
+    int wide_ids;      // 1: adapter is int64
+    int vec;           // 1: x and a may be read 16 bytes at a time
+};
+void launch_lora_low(const LoraLow& p, hipStream_t st);
+
+}  // namespace flux

@@ -59,8 +59,13 @@ constexpr int kGemvSiluLds = 48 * 1024;  // bytes of LDS for the (activated) inp
 // EXACT: K = 512 * U, so every lane has exactly U vectors per row and the K loop runs once, without tests.
 // ONCE: W is read with the non-temporal hint (see launch_gemv).
 // block: which 4 * kGemvCols columns; act_lds: MM * K * 2 bytes with SILU_LDS.
-template <int MM, bool SILU_LDS, int U, bool EXACT, bool ONCE>
-__device__ __forceinline__ void gemv_small_m(const GemmParams& p, int block, char* act_lds) {
+// tail: request(first column, lane, p) goes out in front of W, add(sums, lane) to what each lane has summed up (NoRowTail: nothing).
+struct NoRowTail {
+    __device__ __forceinline__ void request(int, int, const GemmParams&) {}
+    template <int MM> __device__ __forceinline__ void add(float (&)[kGemvCols][MM], int) {}
+};
+template <int MM, bool SILU_LDS, int U, bool EXACT, bool ONCE, typename Tail = NoRowTail>
+__device__ __forceinline__ void gemv_small_m(const GemmParams& p, int block, char* act_lds, Tail tail = Tail()) {
     constexpr int CPW = kGemvCols;  // CPW * U 16-byte loads of W in flight per lane
     // Activation vectors a thread requests in front: its share at K = 3072 where a whole such row of W is in flight, one or
     // two where half of it is (four rows of K = 1536: 5.4 us, 5.6 with two, 6.2 with all six).
@@ -79,6 +84,7 @@ __device__ __forceinline__ void gemv_small_m(const GemmParams& p, int block, cha
     bf16_t bias_raw[CPW];
 #pragma unroll
     for (int c = 0; c < CPW; ++c) bias_raw[c] = p.bias ? p.bias[min(n0 + c, p.N - 1)] : static_cast<bf16_t>(0);
+    tail.request(n0, lane, p);
     Vec16<bf16_t> pre[PRE];
     if (SILU_LDS) {
 #pragma unroll
@@ -160,6 +166,7 @@ __device__ __forceinline__ void gemv_small_m(const GemmParams& p, int block, cha
                 }
         }
     }
+    tail.add(acc, lane);
 #pragma unroll
     for (int c = 0; c < CPW; ++c)
 #pragma unroll

@@ -8,6 +8,7 @@ from triton_kernels.functional import (
     layer_norm_modulation_torch,
     layer_norm_modulation_torch_compile,
     layer_norm_torch,
+    linear_lora_torch,
     rms_norm_torch,
     rms_norm_torch_compile,
 )
@@ -19,6 +20,7 @@ from triton_kernels.kernels import (
     layer_norm_modulation,
     linear,
     linear_into,
+    linear_lora,
     qkv_prep,
     rms_norm,
     rope_table,
@@ -28,8 +30,8 @@ from triton_kernels.modules import DoubleStreamBlock, EmbedND, LayerNorm, QKNorm
 
 __all__ = [
     "apply_rope_nd_torch", "apply_rope_torch", "apply_rope_torch_compile", "layer_norm_modulation_torch",
-    "layer_norm_modulation_torch_compile", "layer_norm_torch", "rms_norm_torch", "rms_norm_torch_compile",
+    "layer_norm_modulation_torch_compile", "layer_norm_torch", "linear_lora_torch", "rms_norm_torch", "rms_norm_torch_compile",
     "apply_rope", "apply_rope_nd", "layer_norm", "layer_norm_modulation", "linear", "rms_norm", "scaled_dot_product_attention",
-    "attention_into", "linear_into", "qkv_prep", "rope_table",
+    "attention_into", "linear_into", "linear_lora", "qkv_prep", "rope_table",
     "DoubleStreamBlock", "EmbedND", "LayerNorm", "QKNorm", "RMSNorm", "SingleStreamBlock",
 ]

@@ -131,6 +131,15 @@ class RopeNdArgs(Structure):
     ]
 
 
+class LinearLoraArgs(Structure):
+    _fields_ = [
+        ("x", c_void_p), ("w", c_void_p), ("bias", c_void_p), ("y", c_void_p),
+        ("lora_a", c_void_p), ("lora_b", c_void_p), ("adapter", c_void_p), ("scaling", c_void_p),
+        ("M", c_int64), ("N", c_int64), ("K", c_int64), ("ldx", c_int64), ("ldw", c_int64), ("ldy", c_int64), ("requests", c_int64),
+        ("adapters", c_int32), ("rank", c_int32), ("wide_ids", c_int32), ("act", c_int32),
+    ]
+
+
 # name -> (restype, argtypes); also the list the symbol-export test walks.
 SIGNATURES = {
     "flux_abi_version": (c_int32, []),
@@ -176,6 +185,9 @@ TUNE_SIGNATURES = {
     "flux_layer_norm_bwd": (c_int32, [POINTER(LayerNormBwdArgs), c_void_p, c_int64, c_void_p]),
     "flux_rope_nd": (c_int32, [POINTER(RopeNdArgs), c_void_p]),
     "flux_rope_table": (c_int32, [POINTER(RopeIds), c_void_p, c_int64, c_int64, c_void_p]),
+    "flux_linear_lora_workspace_bytes": (c_int64, [POINTER(LinearLoraArgs)]),
+    "flux_linear_lora_least_bytes": (c_int64, [POINTER(LinearLoraArgs)]),
+    "flux_linear_lora_bf16": (c_int32, [POINTER(LinearLoraArgs), c_void_p, c_int64, c_void_p]),
 }
 
 
@@ -311,7 +323,7 @@ def src4(t: torch.Tensor | None) -> Src4:
 
 __all__ = [
     "lib", "lib_path", "check", "last_error", "dtype_code", "require_gpu", "stream_ptr", "on_device", "ptr", "src4",
-    "Src4", "QkvPrepArgs", "LinearArgs", "LinearPairArgs", "LinearPlan", "RmsNormArgs", "LayerNormArgs", "AttnArgs", "LayerNormFwdArgs", "LayerNormBwdArgs", "RopeIds", "RopeNdArgs",
+    "Src4", "QkvPrepArgs", "LinearArgs", "LinearPairArgs", "LinearPlan", "RmsNormArgs", "LayerNormArgs", "AttnArgs", "LayerNormFwdArgs", "LayerNormBwdArgs", "RopeIds", "RopeNdArgs", "LinearLoraArgs",
     "SIGNATURES", "TUNE_SIGNATURES", "byref",
     "FLUX_BF16", "FLUX_F32", "ACT_NONE", "ACT_GELU_TANH", "ACT_SILU", "LINEAR_SHARED_GPU", "MAX_ROW",
 ]

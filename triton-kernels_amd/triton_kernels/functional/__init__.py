@@ -1,3 +1,4 @@
+from triton_kernels.functional.linear import linear_lora_torch
 from triton_kernels.functional.normalization import (
     layer_norm_modulation_torch,
     layer_norm_modulation_torch_compile,
@@ -10,5 +11,5 @@ from triton_kernels.functional.positional_embedding import apply_rope_nd_torch, 
 
 __all__ = [
     "apply_rope_nd_torch", "apply_rope_torch", "apply_rope_torch_compile", "layer_norm_modulation_torch",
-    "layer_norm_modulation_torch_compile", "layer_norm_torch", "modulate", "rms_norm_torch", "rms_norm_torch_compile",
+    "layer_norm_modulation_torch_compile", "layer_norm_torch", "linear_lora_torch", "modulate", "rms_norm_torch", "rms_norm_torch_compile",
 ]

@@ -1,5 +1,6 @@
 """linear: y = act(x @ w.T + b) on the bf16 matrix cores (kernels/linear.py:104-151 of the reference),
-with the extra epilogues the fused Flux blocks use."""
+with the extra epilogues the fused Flux blocks use; linear_lora, which the reference does not have, is the same with
+a low-rank adapter of each request's own."""
 from __future__ import annotations
 
 import ctypes
@@ -275,3 +276,58 @@ def linear(x: Tensor, w: Tensor, b: Tensor | None, activation: str = "", shared_
     N = w.shape[0]
     y = linear_into(x, w, b, activation=activation, shared_gpu=shared_gpu)
     return y.reshape(*x.shape[:-1], N)
+
+
+def linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, lora_b: Tensor, adapter: Tensor, scaling: Tensor | None = None, activation: str = "") -> Tensor:
+    """A projection that many requests share, each with a low-rank adapter of its own:
+    y = act(x w^T + b + s (x lora_a[i]^T) lora_b[i]^T) with i = the request's adapter and s = scaling[i].
+
+    x, w, b, activation : as in linear; x [..., K], w [N, K], bf16
+    lora_a : [adapters, rank, K], lora_b : [adapters, N, rank], the stacks of all adapters, rank up to 256 (adapters of lower rank end in zeros)
+    adapter : whole numbers on the GPU, one for each index of x's leading dimensions that it has: [B] beside an x of [B, L, K] (a request a batch
+              element), [B, L] or [rows] (an adapter by row), [] (one for all). A number that is no adapter's, -1 for one, means none.
+    scaling : fp32 [adapters], or None for 1
+
+    Like linear it is not differentiated. x lora_a[i]^T is rounded to bf16, the sum of both products only as the result. What is not
+    finite in an adapter does not reach other requests' rows.
+    """
+    assert x.shape[-1] == w.shape[-1], "Incompatible dimensions"
+    assert x.dtype == w.dtype and lora_a.dtype == x.dtype and lora_b.dtype == x.dtype, "Incompatible dtypes"
+    _PLANS[x.dtype]  # KeyError for anything but bfloat16, as linear
+    act = _ACTIVATIONS[activation]
+    dev = nv.require_gpu(x, w, b, lora_a, lora_b, adapter, scaling)
+    N, K = w.shape
+    assert lora_a.dim() == 3 and lora_b.dim() == 3 and lora_a.shape[2] == K and lora_b.shape == (lora_a.shape[0], N, lora_a.shape[1]), \
+        f"adapters are [n, rank, {K}] and [n, {N}, rank], not {tuple(lora_a.shape)} and {tuple(lora_b.shape)}"
+    if adapter.is_floating_point() or adapter.is_complex() or adapter.dtype == torch.bool:
+        raise TypeError(f"unsupported dtype {adapter.dtype} of adapter numbers")
+    assert adapter.dim() < x.dim() and adapter.shape == x.shape[:adapter.dim()], f"adapter numbers {tuple(adapter.shape)} beside x {tuple(x.shape)}"
+    adapters, rank = lora_a.shape[:2]
+    if adapter.dtype not in (torch.int32, torch.int64):
+        adapter = adapter.to(torch.int32)
+    adapter, lora_a, lora_b = adapter.contiguous(), lora_a.contiguous(), lora_b.contiguous()
+    if scaling is not None:
+        assert scaling.shape == (adapters,), f"scaling is [{adapters}], not {tuple(scaling.shape)}"
+        scaling = scaling.float().contiguous()
+    x2 = _rows_2d(x, K)
+    M = x2.shape[0]
+    if w.stride(1) != 1 or (N > 1 and w.stride(0) < K):
+        w = w.contiguous()
+    if b is not None:
+        assert b.shape[-1] == N
+        b = b.to(x.dtype).contiguous()
+    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+    if y.numel() == 0:
+        return y
+    a = nv.LinearLoraArgs(x2.data_ptr(), w.data_ptr(), nv.ptr(b), y.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), adapter.data_ptr(), nv.ptr(scaling),
+                          M, N, K, x2.stride(0) if M > 1 else K, w.stride(0) if N > 1 else K, N, adapter.numel(), adapters, rank, adapter.dtype == torch.int64, act)
+    if launch_hook is not None:
+        note = linear_launch_metadata(M, N, K, x.element_size(), "+".join(p for p in (activation, f"adapters {adapters} x {rank}") if p))
+        note["flops16"] += 2.0 * M * rank * (K + N)
+        launch_hook(note)
+    with nv.on_device(dev):
+        need = nv.lib().flux_linear_lora_workspace_bytes(nv.byref(a))
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        rc = nv.lib().flux_linear_lora_bf16(nv.byref(a), nv.ptr(ws), need, nv.stream_ptr(dev))
+    nv.check(rc, "flux_linear_lora_bf16")
+    return y
