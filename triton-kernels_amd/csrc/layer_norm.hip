@@ -9,6 +9,8 @@
 #include "common.h"
 #include "../../include/flux_hip_tune.h"
 #include <algorithm>
+#include <initializer_list>
+#include <utility>
 
 namespace flux {
 
@@ -521,6 +523,13 @@ static int ln_bwd_launch(const flux_layer_norm_bwd_args& a, float* ws, hipStream
     return check_launch("flux_layer_norm_bwd");
 }
 
+// One row a batch element and a weight for all rows: the rows are what is evenly strided.
+static void ln_rows_of(int64_t& batch, int64_t& seq, int64_t groups, std::initializer_list<std::pair<int64_t*, int64_t*>> strides) {
+    if (groups != 1 || seq != 1) return;
+    std::swap(batch, seq);
+    for (const auto& s : strides) *s.second = *s.first;
+}
+
 static int ln_shape(const char* what, int64_t batch, int64_t seq, int64_t groups, int32_t n) {
     if (batch < 0 || seq < 0 || n <= 0) return fail(FLUX_E_SHAPE, "%s: bad shape [%lld,%lld,%d]", what, (long long)batch, (long long)seq, n);
     if (n > FLUX_MAX_ROW) return fail(FLUX_E_TOO_WIDE, "%s: n = %d exceeds the maximum row length %d", what, n, FLUX_MAX_ROW);
@@ -550,7 +559,9 @@ extern "C" int flux_layer_norm(const flux_layer_norm_fwd_args* a, void* stream) 
     if (!a->x || !a->y) return fail(FLUX_E_NULL, "flux_layer_norm: null pointer");
     if ((a->mean == nullptr) != (a->rstd == nullptr)) return fail(FLUX_E_NULL, "flux_layer_norm: mean and rstd go together");
     const hipStream_t st = static_cast<hipStream_t>(stream);
-#define ARGS (*a, st)
+    flux_layer_norm_fwd_args rows = *a;
+    ln_rows_of(rows.batch, rows.seq, rows.groups, {{&rows.x_sb, &rows.x_sl}});
+#define ARGS (rows, st)
     BY_TYPES("flux_layer_norm", ln_fwd_launch);
 #undef ARGS
 }
@@ -571,7 +582,9 @@ extern "C" int flux_layer_norm_bwd(const flux_layer_norm_bwd_args* a, void* ws, 
     if (need > 0 && (!ws || reinterpret_cast<uintptr_t>(ws) % 4 != 0)) return fail(FLUX_E_NULL, "flux_layer_norm_bwd: the workspace must be 4-byte aligned memory");
     if (ws_bytes < need) return fail(FLUX_E_SHAPE, "flux_layer_norm_bwd: workspace of %lld bytes is too small", (long long)ws_bytes);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-#define ARGS (*a, static_cast<float*>(ws), st)
+    flux_layer_norm_bwd_args by_row = *a;
+    ln_rows_of(by_row.batch, by_row.seq, by_row.groups, {{&by_row.x_sb, &by_row.x_sl}, {&by_row.dy_sb, &by_row.dy_sl}});
+#define ARGS (by_row, static_cast<float*>(ws), st)
     BY_TYPES("flux_layer_norm_bwd", ln_bwd_launch);
 #undef ARGS
 }

@@ -26,9 +26,12 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
+#include <optional>
 #include <string>
 
 #include "../../include/flux_hip.h"
+#include "../../include/flux_hip_tune.h"
 
 namespace {
 
@@ -104,6 +107,24 @@ bool vector_rows(const Tensor& t) {
     for (int64_t i = 0; i + 1 < t.dim(); ++i)
         if (t.stride(i) % per16 != 0) return false;
     return true;
+}
+
+// A tensor or None.
+bool optional_tensor(PyObject* o, const Tensor*& t) {
+    t = o == Py_None ? nullptr : tensor_of(o);
+    return t != nullptr || o == Py_None;
+}
+
+PyObject* wrap_or_none(const Tensor& t) {
+    if (t.defined()) return THPVariable_Wrap(t);
+    Py_RETURN_NONE;
+}
+
+bool whole_number(PyObject* o, int64_t& value) {
+    value = PyLong_CheckExact(o) ? PyLong_AsLongLong(o) : -1;
+    if (PyLong_CheckExact(o) && !(value == -1 && PyErr_Occurred())) return true;
+    PyErr_Clear();
+    return false;
 }
 
 // ---- RMS norm ----------------------------------------------------------------------------------
@@ -296,6 +317,159 @@ PyObject* py_layer_norm_modulation_pair(PyObject*, PyObject* const* args, Py_ssi
     END_HANDLE_TH_ERRORS
 }
 
+// ---- layer norm --------------------------------------------------------------------------------
+
+// x seen as [batch, seq, n] without copying it: the strides of the first dimension and of the ones behind it, which are evenly strided.
+bool batches_of_rows(const Tensor& x, int64_t& batch, int64_t& seq, int64_t& sb, int64_t& sl) {
+    const int64_t d = x.dim(), n = d > 0 ? x.size(-1) : 0;
+    if (d < 1 || (n > 1 && x.stride(-1) != 1)) return false;
+    batch = d > 1 ? x.size(0) : 1;
+    sb = d > 1 ? x.stride(0) : 0;
+    seq = 1;
+    sl = n;
+    for (int64_t i = d - 2; i >= 1; --i) {
+        if (x.size(i) == 1) continue;
+        if (seq == 1) sl = x.stride(i);
+        else if (x.stride(i) != sl * seq) return false;
+        seq *= x.size(i);
+    }
+    return batch * seq <= 0x7fff0000;
+}
+
+// An absent tensor as an autograd node's input: it has no edge there.
+std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+// One vector for all rows or one for each batch element.
+bool weight_vectors(const Tensor& t, int64_t batch, int64_t n, int64_t x_dim, int64_t& groups, int64_t& sb) {
+    if (t.dim() < 1 || t.size(-1) != n || (n > 1 && t.stride(-1) != 1)) return false;
+    groups = t.numel() == n ? 1 : batch;
+    sb = groups == 1 ? 0 : t.stride(0);
+    return groups == 1 || (x_dim > 1 && t.dim() > 1 && t.size(0) == batch && t.numel() == batch * n);
+}
+
+struct NormOf {   // a call of layer_norm as the library takes it
+    int64_t batch, seq, x_sb, x_sl, groups, w_sb, b_sb;
+    int32_t n, x_type, w_type, plus_one;
+    float eps;
+};
+
+void launch_layer_norm(const NormOf& c, const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& y, float* mean, float* rstd) {
+    const c10::DeviceGuard guard(x.device());
+    const flux_layer_norm_fwd_args a = {x.data_ptr(), w.defined() ? w.data_ptr() : nullptr, b.defined() ? b.data_ptr() : nullptr, y.data_ptr(), mean, rstd,
+                                        c.batch, c.seq, c.x_sb, c.x_sl, c.groups, c.w_sb, c.b_sb, c.n, c.x_type, c.w_type, c.plus_one, c.eps};
+    check(flux_layer_norm(&a, stream_of(x)), "flux_layer_norm");
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, const NormOf& c) {
+        const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+        const Tensor y = empty(x.sizes(), x.scalar_type(), x), stats = empty({2, c.batch * c.seq}, at::kFloat, x);
+        float* const mean = static_cast<float*>(stats.data_ptr());
+        launch_layer_norm(c, x, w, b, y, mean, mean + c.batch * c.seq);
+        ctx->save_for_backward({x, w, stats});
+        ctx->saved_data["groups"] = c.groups;
+        ctx->saved_data["w"] = static_cast<int64_t>(c.w_type * 2 + c.plus_one);
+        ctx->saved_data["bias"] = b.defined() ? b.sizes().vec() : std::vector<int64_t>();   // (a bias has a dimension at least)
+        return y;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();   // (what saved-tensor hooks gave back, of any type)
+        const int64_t groups = ctx->saved_data["groups"].toInt(), w_flags = ctx->saved_data["w"].toInt();
+        const std::vector<int64_t> bias = ctx->saved_data["bias"].toIntVector();
+        Tensor x = saved[0], w = saved[1], stats = saved[2].to(at::kFloat).contiguous(), dy = grads[0];
+        // edges are those of the tensors that were given, in order
+        const bool want_x = ctx->needs_input_grad(0), want_w = w.defined() && ctx->needs_input_grad(1), want_b = !bias.empty() && ctx->needs_input_grad(w.defined() ? 2 : 1);
+        TORCH_CHECK(x.sizes() == dy.sizes(), "layer_norm: saved tensors came back with other sizes");
+        const int xc = type_code(x), wc = static_cast<int>(w_flags / 2);
+        TORCH_CHECK_TYPE(xc >= 0 && (wc == xc || xc == FLUX_BF16), "unsupported dtype ", x.scalar_type(), ": the HIP kernels take bfloat16 or float32");
+        if (dy.scalar_type() != x.scalar_type()) dy = dy.to(x.scalar_type());
+        flux_layer_norm_bwd_args a = {};
+        int64_t batch, seq;
+        if (!batches_of_rows(x, a.batch, a.seq, a.x_sb, a.x_sl)) {
+            x = x.contiguous();
+            batches_of_rows(x, a.batch, a.seq, a.x_sb, a.x_sl);
+        }
+        if (!batches_of_rows(dy, batch, seq, a.dy_sb, a.dy_sl)) {
+            dy = dy.contiguous();
+            batches_of_rows(dy, batch, seq, a.dy_sb, a.dy_sl);
+        }
+        const at::ScalarType w_type = wc == FLUX_BF16 ? at::kBFloat16 : at::kFloat;
+        a.groups = groups;
+        a.n = static_cast<int32_t>(x.size(-1));
+        a.x_dtype = xc;
+        a.w_dtype = wc;
+        a.plus_one = static_cast<int32_t>(w_flags % 2);
+        TORCH_CHECK(stats.dim() == 2 && stats.size(0) == 2 && stats.size(1) == a.batch * a.seq && (!w.defined() || w.numel() == groups * a.n), "layer_norm: saved tensors came back with other sizes");
+        if (w.defined()) {
+            int64_t found;
+            if (w.scalar_type() != w_type) w = w.to(w_type);
+            if (!weight_vectors(w, a.batch, a.n, x.dim(), found, a.w_sb)) {
+                w = w.contiguous();
+                a.w_sb = groups > 1 ? a.n : 0;
+            }
+        }
+        for (const Tensor* t : std::initializer_list<const Tensor*>{&dy, &w, &stats})
+            TORCH_CHECK(!t->defined() || (t->is_cuda() && t->device() == x.device()), "tensors on different devices: ", t->device(), " and ", x.device());
+        const c10::DeviceGuard guard(x.device());
+        const Tensor dx = want_x ? empty(x.sizes(), x.scalar_type(), x) : Tensor();
+        const Tensor dw = want_w ? empty(w.sizes(), w_type, x) : Tensor();
+        const Tensor db = want_b ? empty(bias, w_type, x) : Tensor();
+        a.dy = dy.data_ptr(); a.x = x.data_ptr();
+        a.w = w.defined() ? w.data_ptr() : nullptr;
+        a.mean = static_cast<const float*>(stats.data_ptr());
+        a.rstd = a.mean + a.batch * a.seq;
+        a.dx = want_x ? dx.data_ptr() : nullptr;
+        a.dw = want_w ? dw.data_ptr() : nullptr;
+        a.db = want_b ? db.data_ptr() : nullptr;
+        const int64_t need = flux_layer_norm_bwd_workspace_bytes(&a);
+        const Tensor ws = need ? empty({need}, at::kByte, x) : Tensor();
+        check(flux_layer_norm_bwd(&a, need ? ws.data_ptr() : nullptr, need, stream_of(x)), "flux_layer_norm_bwd");
+        return {dx, dw, db, Tensor()};
+    }
+};
+
+// layer_norm(x, weight or None, bias or None, eps, plus_one)
+PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(nargs == 5, "layer_norm takes 5 arguments");
+    const Tensor *x = tensor_of(args[0]), *w, *b;
+    if (!x || !optional_tensor(args[1], w) || !optional_tensor(args[2], b) || !quiet() || type_code(*x) < 0) Py_RETURN_NONE;
+    NormOf c = {};
+    double eps;
+    if (!number(args[3], eps) || (args[4] != Py_True && args[4] != Py_False) || !batches_of_rows(*x, c.batch, c.seq, c.x_sb, c.x_sl) || x->size(-1) > kMaxRow) Py_RETURN_NONE;
+    c.n = static_cast<int32_t>(x->size(-1));
+    c.x_type = c.w_type = type_code(*x);
+    c.plus_one = args[4] == Py_True;
+    c.eps = static_cast<float>(eps);
+    c.groups = 1;
+    int64_t groups[2] = {0, 0};
+    const Tensor* const t[2] = {w, b};
+    for (int i = 0; i < 2; ++i) {
+        if (!t[i]) continue;
+        const int type = type_code(*t[i]);
+        if (type < 0 || (type != c.x_type && c.x_type != FLUX_BF16) || t[i]->device() != x->device() || !weight_vectors(*t[i], c.batch, c.n, x->dim(), groups[i], i == 0 ? c.w_sb : c.b_sb))
+            Py_RETURN_NONE;
+        c.w_type = type;
+        c.groups = groups[i];
+    }
+    if (w && b && (groups[0] != groups[1] || w->scalar_type() != b->scalar_type())) Py_RETURN_NONE;
+    const bool recorded = at::GradMode::is_enabled() && (x->requires_grad() || (w && w->requires_grad()) || (b && b->requires_grad()));
+    Tensor y;
+    {
+        const Tensor xa = *x, wa = w ? *w : Tensor(), ba = b ? *b : Tensor();   // (the caller's objects are another thread's to drop from here on)
+        const WithoutInterpreter free;
+        if (recorded) {
+            y = LayerNorm::apply(xa, given(wa), given(ba), c);
+        } else {
+            y = empty(xa.sizes(), xa.scalar_type(), xa);
+            launch_layer_norm(c, xa, wa, ba, y, nullptr, nullptr);
+        }
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- rotation ----------------------------------------------------------------------------------
 
 flux_src4 source(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
@@ -346,17 +520,6 @@ PyObject* py_apply_rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     check(rc, "flux_qkv_prep");
     return two(yq, yk);
     END_HANDLE_TH_ERRORS
-}
-
-// A tensor or None.
-bool optional_tensor(PyObject* o, const Tensor*& t) {
-    t = o == Py_None ? nullptr : tensor_of(o);
-    return t != nullptr || o == Py_None;
-}
-
-PyObject* wrap_or_none(const Tensor& t) {
-    if (t.defined()) return THPVariable_Wrap(t);
-    Py_RETURN_NONE;
 }
 
 // qkv_prep(q_img, k_img, v_img, q_txt, k_txt, v_txt, table, q_scale_img, k_scale_img, q_scale_txt, k_scale_txt, eps): (q, k, v), where
@@ -427,6 +590,174 @@ PyObject* py_qkv_prep(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- rotation by positions of several axes -----------------------------------------------------
+
+struct RopeAxes {   // what a call has beside its tensors
+    int64_t sb, sl, sa;
+    double theta;
+    int32_t type, n;
+    int32_t dim[FLUX_ROPE_MOST_AXES];
+};
+
+// (axes, theta) of a call and the layout of its positions; B < 0: any number of batch elements.
+bool read_axes(PyObject* axes, PyObject* theta, const Tensor& ids, int64_t B, int64_t L, int64_t D, RopeAxes& r) {
+    const bool list = PyList_CheckExact(axes);
+    if (!list && !PyTuple_CheckExact(axes)) return false;
+    const Py_ssize_t n = list ? PyList_GET_SIZE(axes) : PyTuple_GET_SIZE(axes);
+    if (n < 1 || n > FLUX_ROPE_MOST_AXES || !number(theta, r.theta)) return false;
+    int64_t total = 0;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        int64_t d;
+        if (!whole_number(list ? PyList_GET_ITEM(axes, i) : PyTuple_GET_ITEM(axes, i), d) || d <= 0 || d > FLUX_ROPE_MOST_DIM || d % 2 != 0) return false;
+        r.dim[i] = static_cast<int32_t>(d);
+        total += d;
+    }
+    r.n = static_cast<int32_t>(n);
+    if (total > FLUX_ROPE_MOST_DIM || (D >= 0 && total != D) || ids.dim() < 2 || ids.dim() > 3 || ids.size(-1) != n || (L >= 0 && ids.size(-2) != L) ||
+        (B >= 0 && ids.dim() == 3 && ids.size(0) != 1 && ids.size(0) != B))
+        return false;
+    switch (ids.scalar_type()) {
+        case at::kFloat: r.type = FLUX_IDS_F32; break;
+        case at::kDouble: r.type = FLUX_IDS_F64; break;
+        case at::kInt: r.type = FLUX_IDS_I32; break;
+        case at::kLong: r.type = FLUX_IDS_I64; break;
+        default: return false;
+    }
+    r.sb = ids.dim() == 3 && ids.size(0) > 1 ? ids.stride(0) : 0;
+    r.sl = ids.stride(-2);
+    r.sa = ids.stride(-1);
+    return true;
+}
+
+flux_rope_ids rope_ids(const RopeAxes& r, const Tensor& ids) {
+    flux_rope_ids at = {ids.data_ptr(), r.sb, r.sl, r.sa, r.theta, r.type, r.n, {}};
+    std::copy(r.dim, r.dim + r.n, at.axes_dim);
+    return at;
+}
+
+// q and k turned by their angles or back by them; either may be absent.
+void rotate(const Tensor (&x)[2], const Tensor& ids, const RopeAxes& r, bool inverse, Tensor (&y)[2]) {
+    const Tensor& ref = x[x[0].defined() ? 0 : 1];
+    const c10::DeviceGuard guard(ref.device());
+    flux_rope_nd_args a = {};
+    Tensor kept[2];
+    for (int i = 0; i < 2; ++i) {
+        if (!x[i].defined()) continue;
+        kept[i] = x[i].scalar_type() == ref.scalar_type() ? x[i] : x[i].to(ref.scalar_type());
+        if (kept[i].stride(3) != 1) kept[i] = kept[i].contiguous();
+        y[i] = empty(x[i].sizes(), ref.scalar_type(), ref);
+        (i == 0 ? a.q : a.k) = source(kept[i]);
+        (i == 0 ? a.q_out : a.k_out) = y[i].data_ptr();
+        (i == 0 ? a.Hq : a.Hk) = x[i].size(1);
+    }
+    a.at = rope_ids(r, ids);
+    a.B = ref.size(0);
+    a.L = ref.size(2);
+    a.D = static_cast<int32_t>(ref.size(3));
+    a.dtype = type_code(ref);
+    a.inverse = inverse;
+    check(flux_rope_nd(&a, stream_of(ref)), "flux_rope_nd");
+}
+
+// (Outputs are those of the inputs that are there, q's before k's.)
+struct RopeNd : torch::autograd::Function<RopeNd> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const std::optional<Tensor>& q, const std::optional<Tensor>& k, const Tensor& ids, const RopeAxes& r,
+                                                  bool inverse) {
+        Tensor y[2];
+        rotate({q.value_or(Tensor()), k.value_or(Tensor())}, ids, r, inverse, y);
+        ctx->save_for_backward({ids});
+        ctx->set_materialize_grads(false);
+        std::string call(reinterpret_cast<const char*>(&r), sizeof(r));
+        call += {static_cast<char>(inverse), static_cast<char>(q.has_value()), static_cast<char>(k.has_value())};
+        ctx->saved_data["call"] = std::move(call);
+        torch::autograd::variable_list out;
+        for (const Tensor& t : y)
+            if (t.defined()) out.push_back(t);
+        return out;
+    }
+
+    // The rotation by the negative angles, recorded in its turn where it is to be differentiated again.
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        Tensor ids = ctx->get_saved_variables()[0], d[2];
+        const std::string call = ctx->saved_data["call"].toStringRef();
+        RopeAxes r;
+        std::memcpy(&r, call.data(), sizeof(r));
+        const char* const flags = call.data() + sizeof(r);
+        for (int i = 0, at = 0; i < 2; ++i) {
+            if (!flags[1 + i]) continue;
+            if (ctx->needs_input_grad(at)) d[i] = grads[at];   // (edges and outputs alike are those of the tensors that were given)
+            ++at;
+        }
+        torch::autograd::variable_list out(5);
+        const Tensor& ref = d[d[0].defined() ? 0 : 1];
+        if (!ref.defined()) return out;
+        const at::ScalarType types[] = {at::kFloat, at::kDouble, at::kInt, at::kLong};
+        TORCH_CHECK(ids.dim() >= 2 && ids.size(-1) == r.n && ids.device() == ref.device() && ids.size(-2) == ref.size(2) &&
+                    (ids.dim() == 2 || ids.size(0) == 1 || ids.size(0) == ref.size(0)), "apply_rope_nd: saved positions came back with another shape");
+        if (ids.scalar_type() != types[r.type]) ids = ids.to(types[r.type]);
+        r.sb = ids.dim() == 3 && ids.size(0) > 1 ? ids.stride(0) : 0;
+        r.sl = ids.stride(-2);
+        r.sa = ids.stride(-1);
+        const auto back = RopeNd::apply(given(d[0]), given(d[1]), ids, r, !flags[0]);
+        if (d[0].defined()) out[0] = back.front();
+        if (d[1].defined()) out[1] = back.back();
+        return out;
+    }
+};
+
+// apply_rope_nd(q, k or None, ids, axes, theta)
+PyObject* py_apply_rope_nd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(nargs == 5, "apply_rope_nd takes 5 arguments");
+    const Tensor *q = tensor_of(args[0]), *k, *ids = tensor_of(args[2]);
+    RopeAxes r = {};
+    if (!q || !ids || !optional_tensor(args[1], k) || !quiet() || q->dim() != 4 || type_code(*q) < 0 || ids->device() != q->device() ||
+        (k && (k->dim() != 4 || !same_kind(*q, *k) || k->size(0) != q->size(0) || k->size(2) != q->size(2) || k->size(3) != q->size(3))) ||
+        !read_axes(args[3], args[4], *ids, q->size(0), q->size(2), q->size(3), r) || ids->requires_grad())
+        Py_RETURN_NONE;
+    const bool recorded = at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()));
+    Tensor y[2];
+    {
+        const Tensor x[2] = {*q, k ? *k : Tensor()}, at = *ids;   // (the caller's objects are another thread's to drop from here on)
+        const WithoutInterpreter free;
+        if (recorded) {
+            const auto both = RopeNd::apply(given(x[0]), given(x[1]), at, r, false);
+            y[0] = both[0];
+            if (both.size() > 1) y[1] = both[1];
+        } else {
+            rotate(x, at, r, false, y);
+        }
+    }
+    PyObject* const t = PyTuple_New(2);
+    if (!t) return nullptr;
+    for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(t, i, wrap_or_none(y[i]));
+    return t;
+    END_HANDLE_TH_ERRORS
+}
+
+// rope_table(ids, axes, theta)
+PyObject* py_rope_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(nargs == 3, "rope_table takes 3 arguments");
+    const Tensor* ids = tensor_of(args[0]);
+    RopeAxes r = {};
+    if (!ids || !quiet() || !read_axes(args[1], args[2], *ids, -1, -1, -1, r) || ids->requires_grad()) Py_RETURN_NONE;
+    Tensor out;
+    {
+        const Tensor at = *ids;
+        const WithoutInterpreter free;
+        const c10::DeviceGuard guard(at.device());
+        const int64_t B = at.dim() == 3 ? at.size(0) : 1, L = at.size(-2);
+        int64_t pairs = 0;
+        for (int i = 0; i < r.n; ++i) pairs += r.dim[i] / 2;
+        out = empty({B, 1, L, pairs, 2, 2}, at::kFloat, at);
+        const flux_rope_ids a = rope_ids(r, at);
+        check(flux_rope_table(&a, static_cast<float*>(out.data_ptr()), B, L, stream_of(at)), "flux_rope_table");
+    }
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- linear ------------------------------------------------------------------------------------
 
 // linear(x, w, b or None, activation): y = act(x w^T + b), activation 0 or 1 (tanh GELU)
@@ -477,13 +808,6 @@ struct Product {
     c10::SmallVector<Tensor, 12> keep;
     bool out_given = false;
 };
-
-bool whole_number(PyObject* o, int64_t& value) {
-    value = PyLong_CheckExact(o) ? PyLong_AsLongLong(o) : -1;
-    if (PyLong_CheckExact(o) && !(value == -1 && PyErr_Occurred())) return true;
-    PyErr_Clear();
-    return false;
-}
 
 // x as [rows, n] without copying it.
 bool flat_rows(const Tensor& x, int64_t n, int64_t& rows, int64_t& ld) {
@@ -657,6 +981,45 @@ PyObject* py_linear_pair_into(PyObject*, PyObject* const* args, Py_ssize_t nargs
     END_HANDLE_TH_ERRORS
 }
 
+// ---- linear with adapters ----------------------------------------------------------------------
+
+// linear_lora(x, w, b or None, lora_a, lora_b, adapter, scaling or None, activation)
+PyObject* py_linear_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(nargs == 8, "linear_lora takes 8 arguments");
+    const Tensor *x = tensor_of(args[0]), *w = tensor_of(args[1]), *b, *la = tensor_of(args[3]), *lb = tensor_of(args[4]), *id = tensor_of(args[5]), *scaling;
+    int64_t act, M, ld;
+    if (!x || !w || !la || !lb || !id || !optional_tensor(args[2], b) || !optional_tensor(args[6], scaling) || !whole_number(args[7], act) || !quiet() || x->dim() < 1 || w->dim() != 2 ||
+        la->dim() != 3 || lb->dim() != 3 || x->scalar_type() != at::kBFloat16 || !is_bf16(*w, *x) || !is_bf16(*la, *x) || !is_bf16(*lb, *x) || id->device() != x->device())
+        Py_RETURN_NONE;
+    const int64_t N = w->size(0), K = w->size(1), adapters = la->size(0), rank = la->size(1);
+    if (!flat_rows(*x, K, M, ld) || (K > 1 && w->stride(1) != 1) || (N > 1 && w->stride(0) < K) || la->size(2) != K || lb->size(0) != adapters || lb->size(1) != N || lb->size(2) != rank ||
+        !la->is_contiguous() || !lb->is_contiguous() || !id->is_contiguous() || (id->scalar_type() != at::kInt && id->scalar_type() != at::kLong) || id->dim() >= x->dim() ||
+        id->sizes() != x->sizes().slice(0, id->dim()) || (b && (!is_bf16(*b, *x) || b->dim() != 1 || b->numel() != N || b->stride(0) != 1)) ||
+        (scaling && (scaling->scalar_type() != at::kFloat || scaling->device() != x->device() || scaling->dim() != 1 || scaling->numel() != adapters || !scaling->is_contiguous())))
+        Py_RETURN_NONE;
+    Tensor y;
+    int rc;
+    {
+        const Tensor xa = *x, wa = *w, ba = b ? *b : Tensor(), a1 = *la, a2 = *lb, ids = *id, sc = scaling ? *scaling : Tensor();
+        const WithoutInterpreter free;
+        const c10::DeviceGuard guard(xa.device());
+        at::DimVector sizes(xa.sizes().begin(), xa.sizes().end());
+        sizes.back() = N;
+        y = empty(sizes, at::kBFloat16, xa);
+        const flux_linear_lora_args a = {xa.data_ptr(), wa.data_ptr(), ba.defined() ? ba.data_ptr() : nullptr, y.data_ptr(), a1.data_ptr(), a2.data_ptr(), ids.data_ptr(),
+                                         sc.defined() ? static_cast<const float*>(sc.data_ptr()) : nullptr, M, N, K, M > 1 ? ld : K, N > 1 ? wa.stride(0) : K, N, ids.numel(),
+                                         static_cast<int32_t>(adapters), static_cast<int32_t>(rank), ids.scalar_type() == at::kLong, static_cast<int32_t>(act)};
+        const int64_t need = may_cut_k(M, N, K) ? flux_linear_lora_workspace_bytes(&a) : flux_linear_lora_least_bytes(&a);
+        const Tensor ws = empty({need}, at::kByte, xa);
+        rc = flux_linear_lora_bf16(&a, need ? ws.data_ptr() : nullptr, need, stream_of(xa));
+    }
+    if (rc < 0) Py_RETURN_NONE;   // (a refusal: its kind of error is the launcher's)
+    check(rc, "flux_linear_lora_bf16");
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- attention ---------------------------------------------------------------------------------
 
 // attention(q, k, v, scale or None): all of [B, H, L, D]; attention(q, k, v, scale or None, out, calls): to a tensor that is there, beside up to two
@@ -714,8 +1077,8 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 #define FLUX_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FLUX_METHOD(rms_norm), FLUX_METHOD(rms_norm_pair), FLUX_METHOD(layer_norm_modulation), FLUX_METHOD(layer_norm_modulation_pair), FLUX_METHOD(apply_rope),
-                         FLUX_METHOD(qkv_prep), FLUX_METHOD(linear), FLUX_METHOD(linear_into), FLUX_METHOD(linear_pair_into), FLUX_METHOD(attention), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {FLUX_METHOD(rms_norm), FLUX_METHOD(rms_norm_pair), FLUX_METHOD(layer_norm), FLUX_METHOD(layer_norm_modulation), FLUX_METHOD(layer_norm_modulation_pair), FLUX_METHOD(apply_rope), FLUX_METHOD(apply_rope_nd), FLUX_METHOD(rope_table),
+                         FLUX_METHOD(qkv_prep), FLUX_METHOD(linear), FLUX_METHOD(linear_into), FLUX_METHOD(linear_pair_into), FLUX_METHOD(linear_lora), FLUX_METHOD(attention), {nullptr, nullptr, 0, nullptr}};
 #undef FLUX_METHOD
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

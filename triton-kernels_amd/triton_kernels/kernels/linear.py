@@ -291,6 +291,11 @@ def linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, lora_b: 
     Like linear it is not differentiated. x lora_a[i]^T is rounded to bf16, the sum of both products only as the result. What is not
     finite in an adapter does not reach other requests' rows.
     """
+    known = _ACTIVATIONS.get(activation)
+    if known is not None and launch_hook is None and not is_compiling():
+        y = nv.ops().linear_lora(x, w, b, lora_a, lora_b, adapter, scaling, known)
+        if y is not None:
+            return y
     assert x.shape[-1] == w.shape[-1], "Incompatible dimensions"
     assert x.dtype == w.dtype and lora_a.dtype == x.dtype and lora_b.dtype == x.dtype, "Incompatible dtypes"
     _PLANS[x.dtype]  # KeyError for anything but bfloat16, as linear

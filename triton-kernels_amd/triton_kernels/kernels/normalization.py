@@ -268,6 +268,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     PyTorch's bf16 operations and without gradients.
     x is bf16 or fp32, [..., N] with N up to 65536; a bf16 x takes fp32 weights too.
     """
+    y = None if is_compiling() else nv.ops().layer_norm(x, weight, bias, eps, plus_one)
+    if y is not None:
+        return y
     nv.require_gpu(x, weight, bias)
     assert x.dim() >= 1, "layer_norm needs at least one dimension"
     nv.dtype_code(x)

@@ -214,6 +214,9 @@ def apply_rope_nd(xq: Tensor, xk: Tensor | None, ids: Tensor, axes_dim, theta: f
     Pair j of an axis of d values turns by ids[b, l, axis] * theta^(-2j/d), formed in 64 bits: apply_rope with EmbedND's table, without the
     table. The results are contiguous and rounded once.
     """
+    both = None if is_compiling() else nv.ops().apply_rope_nd(xq, xk, ids, axes_dim, theta)
+    if both is not None:
+        return both
     for x in (xq, xk):
         assert x is None or (x.dim() == 4 and x.dtype == xq.dtype), "q and k are [B, H, L, D] of one type"
     B, _, L, D = xq.shape
@@ -227,6 +230,9 @@ def apply_rope_nd(xq: Tensor, xk: Tensor | None, ids: Tensor, axes_dim, theta: f
 def rope_table(ids: Tensor, axes_dim, theta: float = 10000.0) -> Tensor:
     """The fp32 rotation matrices that the blocks and apply_rope take, [B, 1, L, D/2, 2, 2] for ids [B, L, n] ([1, 1, ...] for [L, n]):
     one kernel for what EmbedND of the plain blocks computes; arguments as in apply_rope_nd."""
+    out = None if is_compiling() else nv.ops().rope_table(ids, axes_dim, theta)
+    if out is not None:
+        return out
     dev = nv.require_gpu(ids)
     _not_differentiated(ids)
     at, _keep = _rope_ids(ids, axes_dim, theta)
