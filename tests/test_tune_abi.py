@@ -118,7 +118,7 @@ WS_AT = (ctypes.addressof(WS) + 255) // 256 * 256
 @pytest.mark.parametrize("change,rc", [(dict(x=None), -1), (dict(w=None), -1), (dict(y=None), -1), (dict(lora_a=None), -1), (dict(lora_b=None), -1), (dict(adapter=None), -1), (dict(M=-1), -2),
                                        (dict(N=2**31), -2), (dict(ldx=7), -2), (dict(ldw=7), -2), (dict(ldy=15), -2), (dict(adapters=0), -2), (dict(rank=0), -2), (dict(rank=257), -2),
                                        (dict(requests=3), -2), (dict(requests=0), -2), (dict(requests=-4), -2), (dict(act=2), -6), (dict(M=2**28, requests=1), -2),
-                                       (dict(M=2**20, N=2**14, K=7, ldx=7, ldw=7, ldy=2**14), -2), (dict(M=0), 0), (dict(N=0), 0)])
+                                       (dict(M=2**20, N=2**14, K=7, ldx=7, ldw=7, ldy=2**14), -2), (dict(N=2**28, ldy=2**28), -2), (dict(M=0), 0), (dict(N=0), 0)])
 def test_linear_lora_refusals(change, rc):
     a = ctypes.byref(lora_args(**change))
     assert nv.lib().flux_linear_lora_bf16(a, WS_AT, 1 << 15, None) == rc

@@ -614,14 +614,16 @@ static int read_lora_args(const flux_linear_lora_args* a, LoraCall& c) {
     if (a->adapters < 1 || a->rank < 1 || a->rank > FLUX_LORA_MOST_RANK) return fail(FLUX_E_SHAPE, "flux_linear_lora_bf16: %d adapters of rank %d, at least 1 of rank 1 to %d are taken", a->adapters, a->rank, FLUX_LORA_MOST_RANK);
     if (a->requests < 1 || a->M % a->requests != 0) return fail(FLUX_E_SHAPE, "flux_linear_lora_bf16: %lld rows for %lld requests", (long long)a->M, (long long)a->requests);
     if (!a->lora_a || !a->lora_b || !a->adapter) return fail(FLUX_E_NULL, "flux_linear_lora_bf16: null adapter operand");
+    if (a->N * a->rank >= (int64_t{1} << 30)) return fail(FLUX_E_SHAPE, "flux_linear_lora_bf16: adapters of 2^30 values in lora_b and more");   // 32-bit offsets
     if (a->M > (int64_t{1} << 27)) return fail(FLUX_E_SHAPE, "flux_linear_lora_bf16: too many rows");
     if (c.route == kScalar && a->N >= ((int64_t{1} << 32) - 256) / a->M) return fail(FLUX_E_SHAPE, "flux_linear_lora_bf16: more than 2^32 results of operands that are not 16-byte addressable");
     const int width = (a->rank + 31) / 32 * 32;
     c.low_bytes = (a->M * width * 2 + 255) / 256 * 256;
     c.owner_bytes = (a->M * 4 + 255) / 256 * 256;
-    c.tail = {nullptr, nullptr, static_cast<const bf16_t*>(a->lora_b), a->rank, width, a->rank % 8 == 0 && aligned16(a->lora_b)};
+    c.tail = {nullptr, nullptr, static_cast<const bf16_t*>(a->lora_b), a->rank, width,
+              a->rank % 8 == 0 && aligned16(a->lora_b) ? 8 : a->rank % 4 == 0 && (reinterpret_cast<uintptr_t>(a->lora_b) & 7u) == 0 ? 4 : 1};
     c.low = {static_cast<const bf16_t*>(a->x), static_cast<const bf16_t*>(a->lora_a), a->adapter, a->scaling, nullptr, nullptr, a->ldx, a->M / a->requests,
-             static_cast<int>(a->M), static_cast<int>(a->K), a->rank, width, a->adapters, a->wide_ids != 0, a->K % 8 == 0 && a->ldx % 8 == 0 && aligned16(a->x) && aligned16(a->lora_a)};
+             static_cast<int>(a->M), static_cast<int>(a->K), a->rank, width, a->adapters, a->wide_ids != 0, a->K % 8 == 0 && a->ldx % 8 == 0 && aligned16(a->x) && aligned16(a->lora_a) && a->ldx * 2 * 16 < 0x7fffffffLL && a->K * 2 * 64 < 0x7fffffffLL};
     return FLUX_OK;
 }
 

@@ -18,7 +18,7 @@ struct LoraTail {
     const int* owner;      // [M]: the row's adapter, -1: none
     const bf16_t* b;       // [adapters][N][rank]
     int rank, width;       // width: rank rounded up to whole steps of 32
-    int vec;               // 1: rows of b may be read 16 bytes at a time
+    int vec;               // rows of b may be read so many values at a time: 8, 4 or 1
 
     // Adds to the fragment rows of a wave: rows m0 .. of the product, columns n0 ... The adapters among the wave's rows are taken one after the
     // other in rising order, each with one read of its columns of b; rows of another adapter count as zeros. 0 * inf would still reach them, so
@@ -47,10 +47,32 @@ struct LoraTail {
         const bool all = __ballot(same) == ~uint64_t{0};
         for (int k = 0;;) {
             u32x4 wb[FN], xa[ROWS];
+            // Scalar bases and 32-bit offsets: sixteen pointers would not fit the registers. Past the rank's end: values of the same row of b
+            // again. They meet zeros of low, and where they are not finite, neither is the result.
+            const int at = k + fq * 8;
+            const bf16_t* const col = b + static_cast<int64_t>(a) * p.N * rank;
+            const bf16_t* const row = low + static_cast<int64_t>(m0) * width;
+            auto column = [&](int j) { return static_cast<uint32_t>(min(n0 + j * 16 + frow, p.N - 1)) * rank; };
+            if (vec == 8) {
 #pragma unroll
-            for (int j = 0; j < FN; ++j) wb[j] = piece(b + (static_cast<int64_t>(a) * p.N + min(n0 + j * 16 + frow, p.N - 1)) * rank, k + fq * 8);
+                for (int j = 0; j < FN; ++j) wb[j] = *reinterpret_cast<const u32x4*>(col + (column(j) + (at < rank ? at : 0)));
+            } else if (vec == 4) {
 #pragma unroll
-            for (int i = 0; i < ROWS; ++i) xa[i] = *reinterpret_cast<const u32x4*>(low + static_cast<int64_t>(min(m0 + i * 16 + frow, p.M - 1)) * width + k + fq * 8);
+                for (int j = 0; j < FN; ++j) {
+                    const u32x2 lo = *reinterpret_cast<const u32x2*>(col + (column(j) + (at < rank ? at : 0)));
+                    const u32x2 hi = *reinterpret_cast<const u32x2*>(col + (column(j) + (at + 4 < rank ? at + 4 : 0)));
+                    wb[j] = u32x4{lo.x, lo.y, hi.x, hi.y};
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) wb[j][e] = col[column(j) + min(at + 2 * e, rank - 1)] | static_cast<uint32_t>(col[column(j) + min(at + 2 * e + 1, rank - 1)]) << 16;
+                    asm volatile("" ::: "memory");   // (a column at a time: eight registers of loads)
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) xa[i] = *reinterpret_cast<const u32x4*>(row + (static_cast<uint32_t>(min(i * 16 + frow, p.M - 1 - m0)) * width + at));
             __builtin_amdgcn_sched_barrier(0);   // the loads stay in front of the products
             auto multiply = [&](const u32x4 (&w)[FN], auto x) {
 #pragma unroll
@@ -105,20 +127,17 @@ struct LoraTail {
         v = min(v, __shfl_xor(v, 8));
         return __builtin_amdgcn_readfirstlane(v);
     }
-
-    // Values k .. k + 7 of a row of `rank` values, zero from its end on.
-    __device__ __forceinline__ u32x4 piece(const bf16_t* row, int k) const {
-        if (vec) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(row + (k < rank ? k : 0));
-            return k < rank ? v : u32x4{0, 0, 0, 0};
-        }
-        u32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            v[e] = (k + 2 * e < rank ? row[k + 2 * e] : 0u) | (k + 2 * e + 1 < rank ? static_cast<uint32_t>(row[k + 2 * e + 1]) << 16 : 0u);
-        return v;
-    }
 };
+
+// The sums are in accumulation registers from here on. Without it the compiler settles the whole kernel's registers by what happens behind the loop
+// over K: 360 moves between accumulation and ordinary registers a slab inside it, 1071 us for 783 at 13008 x 12288 x 3072.
+template <int ROWS, int FN>
+__device__ __forceinline__ void hold(f32x4 (&acc)[ROWS][FN]) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
 
 // The same for row vectors (gemm_rows.h): lane l adds the products of the rank's values l, l + 64, ... to its share of a sum. The first 64 of
 // them are requested in front of W.

@@ -7,73 +7,133 @@
 namespace flux {
 
 // low[m] = s_i x[m] a_i^T for the rows of a tile of 16 that belong to one adapter: blockIdx.y says which of the tile's adapters, in rising order;
-// there are fewer of them than that in most tiles, and a workgroup without one leaves at once. The waves take every n-th 64 of K and add up
-// their sums through LDS. NF * 16 columns of the rank from blockIdx.z on. Bound by x coming from HBM once (M x K) and by a_i coming from the L2 once
-// a tile.
-constexpr int kLowThreads = 1024;
-template <int NF>
-__global__ __launch_bounds__(kLowThreads) void lora_low_kernel(LoraLow p) {
-    __shared__ float part[kLowThreads / 64][NF * 256];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int frow = lane & 15, fq = lane >> 4;
-    const int m0 = blockIdx.x * 16, m = min(m0 + frow, p.M - 1);
+// there are fewer of them than that in most tiles, and a workgroup without one leaves at once. NF * 16 columns of the rank from blockIdx.z on.
+// The waves take every n-th 64 of K, each through LDS of its own and without a barrier, and add up their sums at the end.
+// Bound by the loads: x comes from HBM once, a_i from the L2 once a tile. They go to LDS eight rows of 128 bytes at a time: straight to the
+// registers of the matrix instructions, whose lanes side by side belong to rows, each lane's 16 bytes are a cache line of their own to the
+// address unit (4608 x 3072, rank 64: 34 us).
+struct LowOfTile {
+    int own, a;            // the adapter of this lane's row, and the one of this workgroup; a < 0: none is left for it
+    int row0;
+};
+template <typename P>
+__device__ __forceinline__ LowOfTile low_of_tile(const P& p) {
+    const int frow = threadIdx.x & 15, m0 = blockIdx.x * 16, m = min(m0 + frow, p.M - 1);
     const int64_t request = m / p.rows_per_request;
     const int64_t id = p.wide_ids ? static_cast<const int64_t*>(p.adapter)[request] : static_cast<const int32_t*>(p.adapter)[request];
-    const int own = id >= 0 && id < p.adapters ? static_cast<int>(id) : -1;
-    if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 16 && m0 + frow < p.M) p.owner[m0 + frow] = own;
+    LowOfTile t = {id >= 0 && id < p.adapters ? static_cast<int>(id) : -1, -1, m0};
+    if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 16 && m0 + frow < p.M) p.owner[m0 + frow] = t.own;
     constexpr int kNone = 0x7fffffff;
-    int a = -1;
     for (unsigned i = 0; i <= blockIdx.y; ++i) {
-        a = LoraTail::first_of_rows(own > a ? own : kNone);
-        if (a == kNone) return;   // (alike in every wave)
+        t.a = LoraTail::first_of_rows(t.own > t.a ? t.own : kNone);
+        if (t.a == kNone) {   // (alike in every wave)
+            t.a = -1;
+            break;
+        }
     }
+    return t;
+}
+
+// The waves' sums, in LDS as [wave][NF][64 lanes][4], added in order, scaled, rounded and stored. Lane l of fragment f holds row l % 16 and ranks
+// 16 f + l / 16 * 4 ...
+template <int NF>
+__device__ __forceinline__ void low_store(const LoraLow& p, const LowOfTile& t, const float* part, int waves, int r0) {
+    const float scale = p.scaling != nullptr ? p.scaling[t.a] : 1.0f;
+    for (int i = threadIdx.x; i < NF * 256; i += blockDim.x) {
+        const int row = (i >> 2) & 15, r = r0 + (i >> 8) * 16 + ((i & 255) >> 6) * 4 + (i & 3);
+        float sum = 0.0f;
+        for (int w = 0; w < waves; ++w) sum += part[w * (NF * 256) + i];
+        const bool mine = __shfl(t.own, row) == t.a;
+        if (mine && t.row0 + row < p.M && r < p.width) p.low[static_cast<int64_t>(t.row0 + row) * p.width + r] = r < p.rank ? f2bf(sum * scale) : static_cast<bf16_t>(0);
+    }
+}
+
+template <int NF, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void lora_low_kernel(LoraLow p) {
+    constexpr int BYTES = (1 + NF) * 2048;   // of a wave: 16 rows of x and NF * 16 of a, 64 of K each
+    __shared__ __attribute__((aligned(1024))) char lds[WAVES * BYTES];
+    static_assert(NF * 1024 <= BYTES, "the sums take the operands' place");
+    const LowOfTile t = low_of_tile(p);
+    if (t.a < 0) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), frow = lane & 15, fq = lane >> 4;
     const int r0 = blockIdx.z * (NF * 16);
-    const bf16_t* const xr = p.x + m * p.lda;
-    const bf16_t* const ar = p.a + static_cast<int64_t>(a) * p.rank * p.K;
+    char* const mine = lds + wave * BYTES;
+    // slot (row, position lane % 8) of 8 rows holds chunk position ^ (row / 2 % 8) of its row, so that 16 rows' chunks are read without conflicts
+    const int rows_x = min(p.M - t.row0, 16), rows_a = min(p.rank - r0, NF * 16);
+    bf16_t* const x = const_cast<bf16_t*>(p.x + t.row0 * p.lda);
+    bf16_t* const a = const_cast<bf16_t*>(p.a + (static_cast<int64_t>(t.a) * p.rank + r0) * p.K);
+    const int bytes_x = static_cast<int>(((rows_x - 1) * p.lda + p.K) * 2), bytes_a = rows_a * p.K * 2;
+    uint32_t off_x[2], off_a[2 * NF];
+    int chunk[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = i * 8 + (lane >> 3);
+        chunk[i] = (lane & 7) ^ ((row >> 1) & 7);
+        off_x[i] = row < rows_x ? static_cast<uint32_t>((row * p.lda + chunk[i] * 8) * 2) : kOutOfRange;
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NF; ++i) {
+        const int row = i * 8 + (lane >> 3);
+        off_a[i] = row < rows_a ? static_cast<uint32_t>((row * p.K + chunk[i & 1] * 8) * 2) : kOutOfRange;
+    }
     f32x4 acc[NF];
 #pragma unroll
     for (int f = 0; f < NF; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto piece = [&](const bf16_t* row, int k, bool ok) -> bf16x8 {
-        Vec16<bf16_t> v;
-        if (p.vec) {   // (K is a multiple of 8)
-            ok = ok && k < p.K;
-            v = ld16(row + (ok ? k : 0));
-            if (!ok) v = Vec16<bf16_t>{};
-        } else {
+    for (int k0 = wave * 64; k0 < p.K; k0 += WAVES * 64) {   // (what lies past K, M and the rank reads as zeros)
+        const uint32_t end[2] = {k0 + chunk[0] * 8 < p.K ? 0u : kOutOfRange, k0 + chunk[1] * 8 < p.K ? 0u : kOutOfRange};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v.v[e] = ok && k + e < p.K ? row[k + e] : static_cast<bf16_t>(0);
+        for (int i = 0; i < 2; ++i) load_chunk(__builtin_amdgcn_make_buffer_rsrc(x, 0, bytes_x, kRsrcFlags), mine + i * 1024, off_x[i] | end[i], k0 * 2);
+#pragma unroll
+        for (int i = 0; i < 2 * NF; ++i) load_chunk(__builtin_amdgcn_make_buffer_rsrc(a, 0, bytes_a, kRsrcFlags), mine + 2048 + i * 1024, off_a[i] | end[i & 1], k0 * 2);
+        wait_vmem_all();
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int at = frow * 128 + (((s * 4 + fq) ^ ((frow >> 1) & 7)) * 16);
+            const bf16x8 xf = *reinterpret_cast<const bf16x8*>(mine + at);
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+                acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(mine + 2048 + f * 2048 + at), xf, acc[f], 0, 0, 0);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the operands have been read: their place is free
+    }
+    __syncthreads();
+    float* const part = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) *reinterpret_cast<f32x4*>(part + (wave * NF + f) * 256 + lane * 4) = acc[f];
+    __syncthreads();
+    low_store<NF>(p, t, part, WAVES, r0);
+}
+
+// The same for operands without 16-byte rows: straight from memory, a value at a time.
+__global__ __launch_bounds__(256) void lora_low_any_kernel(LoraLow p) {
+    constexpr int NF = 2;
+    __shared__ float part[4 * NF * 256];
+    const LowOfTile t = low_of_tile(p);
+    if (t.a < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, frow = lane & 15, fq = lane >> 4;
+    const int r0 = blockIdx.z * (NF * 16);
+    const bf16_t* const x = p.x + min(t.row0 + frow, p.M - 1) * p.lda;
+    f32x4 acc[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto piece = [&](const bf16_t* row, int k, bool ok) {
+        Vec16<bf16_t> v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.v[e] = ok && k + e < p.K ? row[k + e] : static_cast<bf16_t>(0);
         return __builtin_bit_cast(bf16x8, v);
     };
-    constexpr int STEPS = 4;   // of 32 of K whose operands are requested at once
-    for (int k0 = wave * 64; k0 < p.K; k0 += waves * (STEPS * 32)) {
-        bf16x8 xf[STEPS], af[STEPS][NF];
+    for (int k0 = wave * 32; k0 < p.K; k0 += 128) {
+        const bf16x8 xf = piece(x, k0 + fq * 8, true);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const int k = k0 + (s / 2) * (waves * 64) + (s % 2) * 32 + fq * 8;
-            xf[s] = piece(xr, k, true);
-#pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                const int r = r0 + f * 16 + frow;
-                af[s][f] = piece(ar + static_cast<int64_t>(r < p.rank ? r : 0) * p.K, k, r < p.rank);
-            }
+        for (int f = 0; f < NF; ++f) {
+            const int r = r0 + f * 16 + frow;
+            acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(piece(p.a + (static_cast<int64_t>(t.a) * p.rank + min(r, p.rank - 1)) * p.K, k0 + fq * 8, r < p.rank), xf, acc[f], 0, 0, 0);
         }
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int f = 0; f < NF; ++f) acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[s][f], xf[s], acc[f], 0, 0, 0);
     }
 #pragma unroll
-    for (int f = 0; f < NF; ++f) *reinterpret_cast<f32x4*>(&part[wave][f * 256 + lane * 4]) = acc[f];
+    for (int f = 0; f < NF; ++f) *reinterpret_cast<f32x4*>(part + (wave * NF + f) * 256 + lane * 4) = acc[f];
     __syncthreads();
-    const float scale = p.scaling != nullptr ? p.scaling[a] : 1.0f;
-    for (int t = threadIdx.x; t < NF * 256; t += blockDim.x) {   // lane l of fragment f holds row l % 16 and ranks 16 f + l / 16 * 4 ...
-        const int row = (t >> 2) & 15, r = r0 + (t >> 8) * 16 + ((t & 255) >> 6) * 4 + (t & 3);
-        float sum = 0.0f;
-        for (int w = 0; w < waves; ++w) sum += part[w][t];
-        const bool mine = __shfl(own, row) == a;
-        if (mine && m0 + row < p.M && r < p.width) p.low[static_cast<int64_t>(m0 + row) * p.width + r] = r < p.rank ? f2bf(sum * scale) : static_cast<bf16_t>(0);
-    }
+    low_store<NF>(p, t, part, 4, r0);
 }
 
 void launch_lora_low(const LoraLow& p, hipStream_t st) {
@@ -81,9 +141,36 @@ void launch_lora_low(const LoraLow& p, hipStream_t st) {
     // adapters a tile can hold: requests that touch 16 rows
     const int64_t requests = p.rows_per_request % 16 == 0 ? 1 : std::min<int64_t>(16, 14 / p.rows_per_request + 2);
     const unsigned slots = static_cast<unsigned>(std::min<int64_t>(requests, p.adapters));
-    const unsigned threads = tiles >= 512 ? 256 : tiles >= 128 ? 512 : kLowThreads;
-    if (p.width <= 32) hipLaunchKernelGGL((lora_low_kernel<2>), dim3((unsigned)tiles, slots), dim3(threads), 0, st, p);
-    else hipLaunchKernelGGL((lora_low_kernel<4>), dim3((unsigned)tiles, slots, (unsigned)((p.width + 63) / 64)), dim3(threads), 0, st, p);
+    auto grid = [&](int ranks) { return dim3((unsigned)tiles, slots, (unsigned)((p.width + ranks - 1) / ranks)); };
+    if (!p.vec) {
+        hipLaunchKernelGGL(lora_low_any_kernel, grid(32), dim3(256), 0, st, p);
+        return;
+    }
+#define CALL(NF, W) hipLaunchKernelGGL((lora_low_kernel<NF, W>), grid(NF * 16), dim3(W * 64), 0, st, p)
+    const int waves = tiles >= 512 ? 4 : tiles >= 128 ? 8 : 16;
+    if (p.width <= 32) {
+        if (waves == 4) CALL(2, 4);
+        else if (waves == 8) CALL(2, 8);
+        else CALL(2, 16);
+    } else {
+        if (waves == 4) CALL(4, 4);
+        else if (waves == 8) CALL(4, 8);
+        else CALL(4, 16);
+    }
+#undef CALL
+}
+
+// A product with adapters has one output, no residual and no q/k columns: what serves those is left out of its kernels.
+__device__ __forceinline__ GemmParams one_output(const GemmLaunch& L) {
+    GemmParams p = L.p[0];
+    p.gate = p.resid = nullptr;
+    p.Y2 = nullptr;
+    p.split_n = p.N;
+    p.y2_col0 = p.qk_cols = p.act_begin = p.in_silu = 0;
+    p.rows_per_batch = 1;
+    p.a_skip = 0;
+    p.ldy2 = p.ldresid = 0;
+    return p;
 }
 
 // The four-wave tiles of gemm_bf16.hip with the adapter's product in front of their epilogue.
@@ -93,12 +180,13 @@ __global__ __launch_bounds__(kGemmThreads) void lora_ring_kernel(GemmLaunch L, L
     __shared__ __attribute__((aligned(1024))) char lds[NU * UNIT];
     int tm, tn;
     if (!tile_of_block(L, tm, tn)) return;
-    const GemmParams& p = L.p[0];
+    const GemmParams p = one_output(L);
     const int m0 = tm * BM, n0 = tn * BM;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x4 acc[2 * MI][2 * MI];
     gemm_tile_slabs<MI, KTAIL>(p, lds, m0, n0, (p.K + BK - 1) / BK, acc);
+    hold(acc);
     tail(acc, m0 + (wave >> 1) * (32 * MI), n0 + (wave & 1) * (32 * MI), p);
     gemm_epilogue<MI, MI>(p, acc, lds, m0, n0, wave, lane);
 }
@@ -109,12 +197,13 @@ __global__ __launch_bounds__(kGemmThreads) void lora_rect_kernel(GemmLaunch L, L
     __shared__ __attribute__((aligned(1024))) char lds[(3 * BM + 2 * BN) * BK * 2];
     int tm, tn;
     if (!tile_of_block(L, tm, tn)) return;
-    const GemmParams p = L.p[0];
+    const GemmParams p = one_output(L);
     const int m0 = tm * BM, n0 = tn * BN;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x4 acc[FM][FN];
     gemm_rect_slabs<FM, FN, KTAIL>(p, lds, m0, n0, (p.K + BK - 1) / BK, acc);
+    hold(acc);
     tail(acc, m0 + (wave >> 1) * (16 * FM), n0 + (wave & 1) * (16 * FN), p);
     gemm_finish_rect<FM, FN, FM, false>(p, acc, lds, m0, n0, 0, wave, lane);
 }
