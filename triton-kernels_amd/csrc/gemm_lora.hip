@@ -12,20 +12,31 @@ namespace flux {
 // Bound by the loads: x comes from HBM once, a_i from the L2 once a tile. They go to LDS eight rows of 128 bytes at a time: straight to the
 // registers of the matrix instructions, whose lanes side by side belong to rows, each lane's 16 bytes are a cache line of their own to the
 // address unit (4608 x 3072, rank 64: 34 us).
+template <int R>           // row fragments of a tile: R * 16 rows
 struct LowOfTile {
-    int own, a;            // the adapter of this lane's row, and the one of this workgroup; a < 0: none is left for it
+    int own[R], a;         // the adapters of this lane's rows, and the one of this workgroup; a < 0: none is left for it
     int row0;
 };
-template <typename P>
-__device__ __forceinline__ LowOfTile low_of_tile(const P& p) {
-    const int frow = threadIdx.x & 15, m0 = blockIdx.x * 16, m = min(m0 + frow, p.M - 1);
-    const int64_t request = m / p.rows_per_request;
-    const int64_t id = p.wide_ids ? static_cast<const int64_t*>(p.adapter)[request] : static_cast<const int32_t*>(p.adapter)[request];
-    LowOfTile t = {id >= 0 && id < p.adapters ? static_cast<int>(id) : -1, -1, m0};
-    if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 16 && m0 + frow < p.M) p.owner[m0 + frow] = t.own;
+template <int R>
+__device__ __forceinline__ LowOfTile<R> low_of_tile(const LoraLow& p) {
+    const int frow = threadIdx.x & 15;
+    LowOfTile<R> t;
+    t.row0 = blockIdx.x * (R * 16);
+    t.a = -1;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int m = t.row0 + i * 16 + frow;
+        const int64_t request = min(m, p.M - 1) / p.rows_per_request;
+        const int64_t id = p.wide_ids ? static_cast<const int64_t*>(p.adapter)[request] : static_cast<const int32_t*>(p.adapter)[request];
+        t.own[i] = id >= 0 && id < p.adapters ? static_cast<int>(id) : -1;
+        if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 16 && m < p.M) p.owner[m] = t.own[i];
+    }
     constexpr int kNone = 0x7fffffff;
-    for (unsigned i = 0; i <= blockIdx.y; ++i) {
-        t.a = LoraTail::first_of_rows(t.own > t.a ? t.own : kNone);
+    for (unsigned n = 0; n <= blockIdx.y; ++n) {
+        int next = kNone;
+#pragma unroll
+        for (int i = 0; i < R; ++i) next = t.own[i] > t.a ? min(next, t.own[i]) : next;
+        t.a = LoraTail::first_of_rows(next);
         if (t.a == kNone) {   // (alike in every wave)
             t.a = -1;
             break;
@@ -34,81 +45,93 @@ __device__ __forceinline__ LowOfTile low_of_tile(const P& p) {
     return t;
 }
 
-// The waves' sums, in LDS as [wave][NF][64 lanes][4], added in order, scaled, rounded and stored. Lane l of fragment f holds row l % 16 and ranks
-// 16 f + l / 16 * 4 ...
-template <int NF>
-__device__ __forceinline__ void low_store(const LoraLow& p, const LowOfTile& t, const float* part, int waves, int r0) {
+// The waves' sums, in LDS as [wave][R][NF][64 lanes][4], added in order, scaled, rounded and stored. Lane l of a fragment holds row l % 16 and
+// ranks l / 16 * 4 ...
+template <int R, int NF>
+__device__ __forceinline__ void low_store(const LoraLow& p, const LowOfTile<R>& t, const float* part, int waves, int r0) {
     const float scale = p.scaling != nullptr ? p.scaling[t.a] : 1.0f;
-    for (int i = threadIdx.x; i < NF * 256; i += blockDim.x) {
-        const int row = (i >> 2) & 15, r = r0 + (i >> 8) * 16 + ((i & 255) >> 6) * 4 + (i & 3);
-        float sum = 0.0f;
-        for (int w = 0; w < waves; ++w) sum += part[w * (NF * 256) + i];
-        const bool mine = __shfl(t.own, row) == t.a;
-        if (mine && t.row0 + row < p.M && r < p.width) p.low[static_cast<int64_t>(t.row0 + row) * p.width + r] = r < p.rank ? f2bf(sum * scale) : static_cast<bf16_t>(0);
-    }
+#pragma unroll
+    for (int f = 0; f < R; ++f)
+        for (int i = threadIdx.x; i < NF * 256; i += blockDim.x) {
+            const int row = (i >> 2) & 15, m = t.row0 + f * 16 + row, r = r0 + (i >> 8) * 16 + ((i & 255) >> 6) * 4 + (i & 3);
+            float sum = 0.0f;
+            for (int w = 0; w < waves; ++w) sum += part[(w * R + f) * (NF * 256) + i];
+            const bool mine = __shfl(t.own[f], row) == t.a;
+            if (mine && m < p.M && r < p.width) p.low[static_cast<int64_t>(m) * p.width + r] = r < p.rank ? f2bf(sum * scale) : static_cast<bf16_t>(0);
+        }
 }
 
-template <int NF, int WAVES>
+template <int R, int NF, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void lora_low_kernel(LoraLow p) {
-    constexpr int BYTES = (1 + NF) * 2048;   // of a wave: 16 rows of x and NF * 16 of a, 64 of K each
+    constexpr int BYTES = (R + NF) * 2048;   // of a wave: R * 16 rows of x and NF * 16 of a, 64 of K each
     __shared__ __attribute__((aligned(1024))) char lds[WAVES * BYTES];
-    static_assert(NF * 1024 <= BYTES, "the sums take the operands' place");
-    const LowOfTile t = low_of_tile(p);
+    static_assert(R * NF * 1024 <= BYTES, "the sums take the operands' place");
+    const LowOfTile<R> t = low_of_tile<R>(p);
     if (t.a < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), frow = lane & 15, fq = lane >> 4;
     const int r0 = blockIdx.z * (NF * 16);
     char* const mine = lds + wave * BYTES;
     // slot (row, position lane % 8) of 8 rows holds chunk position ^ (row / 2 % 8) of its row, so that 16 rows' chunks are read without conflicts
-    const int rows_x = min(p.M - t.row0, 16), rows_a = min(p.rank - r0, NF * 16);
+    const int rows_x = min(p.M - t.row0, R * 16), rows_a = min(p.rank - r0, NF * 16);
     bf16_t* const x = const_cast<bf16_t*>(p.x + t.row0 * p.lda);
     bf16_t* const a = const_cast<bf16_t*>(p.a + (static_cast<int64_t>(t.a) * p.rank + r0) * p.K);
     const int bytes_x = static_cast<int>(((rows_x - 1) * p.lda + p.K) * 2), bytes_a = rows_a * p.K * 2;
-    uint32_t off_x[2], off_a[2 * NF];
+    uint32_t off_x[2 * R], off_a[2 * NF];
     int chunk[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2; ++i) chunk[i] = (lane & 7) ^ (((i * 8 + (lane >> 3)) >> 1) & 7);
+#pragma unroll
+    for (int i = 0; i < 2 * R; ++i) {
         const int row = i * 8 + (lane >> 3);
-        chunk[i] = (lane & 7) ^ ((row >> 1) & 7);
-        off_x[i] = row < rows_x ? static_cast<uint32_t>((row * p.lda + chunk[i] * 8) * 2) : kOutOfRange;
+        off_x[i] = row < rows_x ? static_cast<uint32_t>((row * p.lda + chunk[i & 1] * 8) * 2) : kOutOfRange;
     }
 #pragma unroll
     for (int i = 0; i < 2 * NF; ++i) {
         const int row = i * 8 + (lane >> 3);
         off_a[i] = row < rows_a ? static_cast<uint32_t>((row * p.K + chunk[i & 1] * 8) * 2) : kOutOfRange;
     }
-    f32x4 acc[NF];
+    f32x4 acc[R][NF];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) acc[i][f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int k0 = wave * 64; k0 < p.K; k0 += WAVES * 64) {   // (what lies past K, M and the rank reads as zeros)
         const uint32_t end[2] = {k0 + chunk[0] * 8 < p.K ? 0u : kOutOfRange, k0 + chunk[1] * 8 < p.K ? 0u : kOutOfRange};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) load_chunk(__builtin_amdgcn_make_buffer_rsrc(x, 0, bytes_x, kRsrcFlags), mine + i * 1024, off_x[i] | end[i], k0 * 2);
+        for (int i = 0; i < 2 * R; ++i) load_chunk(__builtin_amdgcn_make_buffer_rsrc(x, 0, bytes_x, kRsrcFlags), mine + i * 1024, off_x[i] | end[i & 1], k0 * 2);
 #pragma unroll
-        for (int i = 0; i < 2 * NF; ++i) load_chunk(__builtin_amdgcn_make_buffer_rsrc(a, 0, bytes_a, kRsrcFlags), mine + 2048 + i * 1024, off_a[i] | end[i & 1], k0 * 2);
+        for (int i = 0; i < 2 * NF; ++i) load_chunk(__builtin_amdgcn_make_buffer_rsrc(a, 0, bytes_a, kRsrcFlags), mine + R * 2048 + i * 1024, off_a[i] | end[i & 1], k0 * 2);
         wait_vmem_all();
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int at = frow * 128 + (((s * 4 + fq) ^ ((frow >> 1) & 7)) * 16);
-            const bf16x8 xf = *reinterpret_cast<const bf16x8*>(mine + at);
+            bf16x8 xf[R];
 #pragma unroll
-            for (int f = 0; f < NF; ++f)
-                acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(mine + 2048 + f * 2048 + at), xf, acc[f], 0, 0, 0);
+            for (int i = 0; i < R; ++i) xf[i] = *reinterpret_cast<const bf16x8*>(mine + i * 2048 + at);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const bf16x8 af = *reinterpret_cast<const bf16x8*>(mine + (R + f) * 2048 + at);
+#pragma unroll
+                for (int i = 0; i < R; ++i) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, xf[i], acc[i][f], 0, 0, 0);
+            }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the operands have been read: their place is free
     }
     __syncthreads();
     float* const part = reinterpret_cast<float*>(lds);
 #pragma unroll
-    for (int f = 0; f < NF; ++f) *reinterpret_cast<f32x4*>(part + (wave * NF + f) * 256 + lane * 4) = acc[f];
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) *reinterpret_cast<f32x4*>(part + ((wave * R + i) * NF + f) * 256 + lane * 4) = acc[i][f];
     __syncthreads();
-    low_store<NF>(p, t, part, WAVES, r0);
+    low_store<R, NF>(p, t, part, WAVES, r0);
 }
 
 // The same for operands without 16-byte rows: straight from memory, a value at a time.
 __global__ __launch_bounds__(256) void lora_low_any_kernel(LoraLow p) {
     constexpr int NF = 2;
     __shared__ float part[4 * NF * 256];
-    const LowOfTile t = low_of_tile(p);
+    const LowOfTile<1> t = low_of_tile<1>(p);
     if (t.a < 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, frow = lane & 15, fq = lane >> 4;
     const int r0 = blockIdx.z * (NF * 16);
@@ -133,29 +156,30 @@ __global__ __launch_bounds__(256) void lora_low_any_kernel(LoraLow p) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) *reinterpret_cast<f32x4*>(part + (wave * NF + f) * 256 + lane * 4) = acc[f];
     __syncthreads();
-    low_store<NF>(p, t, part, 4, r0);
+    low_store<1, NF>(p, t, part, 4, r0);
 }
 
 void launch_lora_low(const LoraLow& p, hipStream_t st) {
-    const int tiles = (p.M + 15) / 16;
-    // adapters a tile can hold: requests that touch 16 rows
-    const int64_t requests = p.rows_per_request % 16 == 0 ? 1 : std::min<int64_t>(16, 14 / p.rows_per_request + 2);
-    const unsigned slots = static_cast<unsigned>(std::min<int64_t>(requests, p.adapters));
-    auto grid = [&](int ranks) { return dim3((unsigned)tiles, slots, (unsigned)((p.width + ranks - 1) / ranks)); };
+    // adapters a tile can hold: requests that touch so many rows
+    auto grid = [&](int rows, int ranks) {
+        const int64_t requests = p.rows_per_request % rows == 0 ? 1 : std::min<int64_t>(rows, (rows - 2) / p.rows_per_request + 2);
+        return dim3((unsigned)((p.M + rows - 1) / rows), (unsigned)std::min<int64_t>(requests, p.adapters), (unsigned)((p.width + ranks - 1) / ranks));
+    };
     if (!p.vec) {
-        hipLaunchKernelGGL(lora_low_any_kernel, grid(32), dim3(256), 0, st, p);
+        hipLaunchKernelGGL(lora_low_any_kernel, grid(16, 32), dim3(256), 0, st, p);
         return;
     }
-#define CALL(NF, W) hipLaunchKernelGGL((lora_low_kernel<NF, W>), grid(NF * 16), dim3(W * 64), 0, st, p)
-    const int waves = tiles >= 512 ? 4 : tiles >= 128 ? 8 : 16;
+#define CALL(R, NF, W) hipLaunchKernelGGL((lora_low_kernel<R, NF, W>), grid(R * 16, NF * 16), dim3(W * 64), 0, st, p)
+    const int tiles = (p.M + 15) / 16;
     if (p.width <= 32) {
-        if (waves == 4) CALL(2, 4);
-        else if (waves == 8) CALL(2, 8);
-        else CALL(2, 16);
+        if (tiles >= 512) CALL(1, 2, 4);
+        else if (tiles >= 128) CALL(1, 2, 8);
+        else CALL(1, 2, 16);
     } else {
-        if (waves == 4) CALL(4, 4);
-        else if (waves == 8) CALL(4, 8);
-        else CALL(4, 16);
+        // us at 4608 x 3072, rank 64, 16 rows of eight waves and 32 rows of six: 20.6 and 16.0 (a CU takes in about 50 bytes per ns, and a comes once a tile)
+        if (tiles >= 256) CALL(2, 4, 6);
+        else if (tiles >= 128) CALL(1, 4, 8);
+        else CALL(1, 4, 16);
     }
 #undef CALL
 }
