@@ -25,13 +25,82 @@ struct LoraTail {
     // where a wave's rows are not of one adapter, what is not finite in b is taken out and makes its own rows NaN by itself: products of 3e38
     // and 3e38 and of 3e38 and -3e38, which are zero for all other rows. (The sums are touched by matrix instructions only: choosing
     // between old and new sums by row, with vector instructions, spilled 600 registers of the 256-wide tile.)
+    // A step's operands: columns of b of one adapter and the rows' low, 32 values each.
+    template <int ROWS, int FN>
+    struct Step {
+        u32x4 b[FN], low[ROWS];
+    };
+    template <int ROWS, int FN>
+    __device__ __forceinline__ void load(Step<ROWS, FN>& to, int a, int k, int m0, int n0, const GemmParams& p) const {
+        // Scalar bases and 32-bit offsets: sixteen pointers would not fit the registers. Past the rank's end: values of the same row of b
+        // again. They meet zeros of low, and where they are not finite, neither is the result.
+        const int frow = threadIdx.x & 15, at = k + ((threadIdx.x & 63) >> 4) * 8;
+        const bf16_t* const col = b + static_cast<int64_t>(a) * p.N * rank;
+        const bf16_t* const row = low + static_cast<int64_t>(m0) * width;
+        auto column = [&](int j) { return static_cast<uint32_t>(min(n0 + j * 16 + frow, p.N - 1)) * rank; };
+        if (vec == 8) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) to.b[j] = *reinterpret_cast<const u32x4*>(col + (column(j) + (at < rank ? at : 0)));
+        } else if (vec == 4) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const u32x2 lo = *reinterpret_cast<const u32x2*>(col + (column(j) + (at < rank ? at : 0)));
+                const u32x2 hi = *reinterpret_cast<const u32x2*>(col + (column(j) + (at + 4 < rank ? at + 4 : 0)));
+                to.b[j] = u32x4{lo.x, lo.y, hi.x, hi.y};
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to.b[j][e] = col[column(j) + min(at + 2 * e, rank - 1)] | static_cast<uint32_t>(col[column(j) + min(at + 2 * e + 1, rank - 1)]) << 16;
+                asm volatile("" ::: "memory");   // (a column at a time: eight registers of loads)
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) to.low[i] = *reinterpret_cast<const u32x4*>(row + (static_cast<uint32_t>(min(i * 16 + frow, p.M - 1 - m0)) * width + at));
+    }
+
+    // What a wave asks for before its sums are complete: the adapters of its rows, and one value of every row of the first step's operands for the
+    // adapter of its first row (whose number comes through the scalar cache, so that nothing waits for it): they are then in the L2. Requested
+    // behind the loop over K alone, a tile waits for memory three times in a row with nothing beside it. (The operands themselves do not fit
+    // beside the loop's: with them the loop moved 350 registers a slab.)
+    template <int ROWS, int FN>
+    struct Ahead {
+        int own[ROWS];
+        uint32_t touched[(ROWS + 3) / 4 + (FN + 3) / 4];
+    };
+    template <int ROWS, int FN>
+    __device__ __forceinline__ void request(Ahead<ROWS, FN>& to, int a, int m0, int n0, const GemmParams& p) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) to.own[i] = owner[min(m0 + i * 16 + (lane & 15), p.M - 1)];
+#pragma unroll
+        for (int i = 0; i < (ROWS + 3) / 4; ++i) to.touched[i] = *reinterpret_cast<const uint32_t*>(low + static_cast<int64_t>(min(m0 + min(i * 64 + lane, ROWS * 16 - 1), p.M - 1)) * width);
+#pragma unroll
+        for (int i = 0; i < (FN + 3) / 4; ++i) to.touched[(ROWS + 3) / 4 + i] = b[(static_cast<int64_t>(max(a, 0)) * p.N + min(n0 + min(i * 64 + lane, FN * 16 - 1), p.N - 1)) * rank];
+    }
+    __device__ __forceinline__ int first_owner(int m0, const GemmParams& p) const {
+        typedef const __attribute__((address_space(4))) int* scalar;
+        return *(scalar)(reinterpret_cast<uintptr_t>(owner + min(m0, p.M - 1)));
+    }
+
     template <int ROWS, int FN>
     __device__ __forceinline__ void operator()(f32x4 (&acc)[ROWS][FN], int m0, int n0, const GemmParams& p) const {
         if (m0 >= p.M || n0 >= p.N) return;
-        const int lane = threadIdx.x & 63, frow = lane & 15, fq = lane >> 4;
         int own[ROWS];
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) own[i] = owner[min(m0 + i * 16 + frow, p.M - 1)];
+        for (int i = 0; i < ROWS; ++i) own[i] = owner[min(m0 + i * 16 + static_cast<int>(threadIdx.x & 15), p.M - 1)];
+        finish(acc, own, m0, n0, p);
+    }
+
+    template <int ROWS, int FN>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[ROWS][FN], Ahead<ROWS, FN>& have, int m0, int n0, const GemmParams& p) const {
+#pragma unroll
+        for (uint32_t& t : have.touched) asm volatile("" ::"v"(t));
+        if (m0 < p.M && n0 < p.N) finish(acc, have.own, m0, n0, p);
+    }
+    template <int ROWS, int FN>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[ROWS][FN], const int (&own)[ROWS], int m0, int n0, const GemmParams& p) const {
         constexpr int kNone = 0x7fffffff;
         auto behind = [&](int last) {   // the next adapter of these rows
             int next = kNone;
@@ -45,34 +114,9 @@ struct LoraTail {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) same = same && own[i] == a;
         const bool all = __ballot(same) == ~uint64_t{0};
+        Step<ROWS, FN> s;
         for (int k = 0;;) {
-            u32x4 wb[FN], xa[ROWS];
-            // Scalar bases and 32-bit offsets: sixteen pointers would not fit the registers. Past the rank's end: values of the same row of b
-            // again. They meet zeros of low, and where they are not finite, neither is the result.
-            const int at = k + fq * 8;
-            const bf16_t* const col = b + static_cast<int64_t>(a) * p.N * rank;
-            const bf16_t* const row = low + static_cast<int64_t>(m0) * width;
-            auto column = [&](int j) { return static_cast<uint32_t>(min(n0 + j * 16 + frow, p.N - 1)) * rank; };
-            if (vec == 8) {
-#pragma unroll
-                for (int j = 0; j < FN; ++j) wb[j] = *reinterpret_cast<const u32x4*>(col + (column(j) + (at < rank ? at : 0)));
-            } else if (vec == 4) {
-#pragma unroll
-                for (int j = 0; j < FN; ++j) {
-                    const u32x2 lo = *reinterpret_cast<const u32x2*>(col + (column(j) + (at < rank ? at : 0)));
-                    const u32x2 hi = *reinterpret_cast<const u32x2*>(col + (column(j) + (at + 4 < rank ? at + 4 : 0)));
-                    wb[j] = u32x4{lo.x, lo.y, hi.x, hi.y};
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < FN; ++j) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) wb[j][e] = col[column(j) + min(at + 2 * e, rank - 1)] | static_cast<uint32_t>(col[column(j) + min(at + 2 * e + 1, rank - 1)]) << 16;
-                    asm volatile("" ::: "memory");   // (a column at a time: eight registers of loads)
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < ROWS; ++i) xa[i] = *reinterpret_cast<const u32x4*>(row + (static_cast<uint32_t>(min(i * 16 + frow, p.M - 1 - m0)) * width + at));
+            load(s, a, k, m0, n0, p);
             __builtin_amdgcn_sched_barrier(0);   // the loads stay in front of the products
             auto multiply = [&](const u32x4 (&w)[FN], auto x) {
 #pragma unroll
@@ -84,27 +128,27 @@ struct LoraTail {
             };
             if (!all) {
 #pragma unroll
-                for (int i = 0; i < ROWS; ++i) xa[i] = own[i] == a ? xa[i] : u32x4{0, 0, 0, 0};
+                for (int i = 0; i < ROWS; ++i) s.low[i] = own[i] == a ? s.low[i] : u32x4{0, 0, 0, 0};
                 uint32_t bad = 0;
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) bad |= not_finite(wb[j][e]);
+                    for (int e = 0; e < 4; ++e) bad |= not_finite(s.b[j][e]);
                 if (__ballot(bad != 0) != 0) {
                     u32x4 huge[FN];
 #pragma unroll
                     for (int j = 0; j < FN; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const uint32_t n = not_finite(wb[j][e]);
+                            const uint32_t n = not_finite(s.b[j][e]);
                             huge[j][e] = n & 0x7f7f7f7fu;
-                            wb[j][e] &= ~n;
+                            s.b[j][e] &= ~n;
                         }
                     multiply(huge, [&](int i) { const uint32_t h = own[i] == a ? 0x7f7f7f7fu : 0u; return u32x4{h, h, h, h}; });
                     multiply(huge, [&](int i) { const uint32_t h = own[i] == a ? 0xff7fff7fu : 0u; return u32x4{h, h, h, h}; });
                 }
             }
-            multiply(wb, [&](int i) { return xa[i]; });
+            multiply(s.b, [&](int i) { return s.low[i]; });
             k += 32;
             if (k >= width) {
                 k = 0;

@@ -176,9 +176,13 @@ __device__ __forceinline__ void gemm_epilogue(const GemmParams& p, f32x4 (&acc)[
 // Multiplies the first ke K slabs of the tile at (m0, n0) into acc (cleared first). On return every
 // buffer load of the wave has landed and all waves have passed a barrier, so the ring may be
 // reused (the epilogue parks its bf16 blocks there).
-template <int MI, bool KTAIL>
+// ahead(): loads of the caller's own, requested behind those of the first slabs; they have landed on return.
+struct NothingAhead {
+    __device__ __forceinline__ void operator()() const {}
+};
+template <int MI, bool KTAIL, typename Ahead = NothingAhead>
 __device__ __forceinline__ void gemm_tile_slabs(const GemmParams& p, char* lds, int m0, int n0, int ke,
-                                                f32x4 (&acc)[2 * MI][2 * MI]) {
+                                                f32x4 (&acc)[2 * MI][2 * MI], Ahead ahead = Ahead()) {
     constexpr int NJ = MI;
     constexpr int FM = 2 * MI, FN = 2 * NJ;      // 16-row fragments per wave and side
     constexpr int BM = 64 * MI, BN = BM, BK = 64;
@@ -343,6 +347,7 @@ __device__ __forceinline__ void gemm_tile_slabs(const GemmParams& p, char* lds, 
         for (int i = 0; i < PU; ++i) load_a(2 * UNIT, i, 1, k1);
 #pragma unroll
         for (int i = 0; i < EARLY; ++i) load_w(3 * UNIT, i, 1, k1);
+        ahead();
         wait_loads_and_barrier<PU + EARLY>();
 #pragma unroll
         for (int r = 0; r < READS; ++r) read_frag(0, 0, UNIT, 0, r);
@@ -381,8 +386,8 @@ __device__ __forceinline__ void gemm_tile_slabs(const GemmParams& p, char* lds, 
 // issues MFMAs [r * MFMAS / READS, (r + 1) * MFMAS / READS).
 // Rows past M or N read as zeros and are not stored.
 // ------------------------------------------------------------------------------------------------
-template <int FM, int FN, bool KTAIL>
-__device__ __forceinline__ void gemm_rect_slabs(const GemmParams& p, char* lds, int m0, int n0, int ke, f32x4 (&acc)[FM][FN]) {
+template <int FM, int FN, bool KTAIL, typename Ahead = NothingAhead>
+__device__ __forceinline__ void gemm_rect_slabs(const GemmParams& p, char* lds, int m0, int n0, int ke, f32x4 (&acc)[FM][FN], Ahead ahead = Ahead()) {
     constexpr int BM = 32 * FM, BN = 32 * FN, BK = 64;
     constexpr int ROWB = BK * 2, KSUB = BK / 32;
     constexpr int UNIT_A = BM * ROWB, UNIT_W = BN * ROWB, W0 = 3 * UNIT_A;   // W ring behind the A ring
@@ -518,6 +523,7 @@ __device__ __forceinline__ void gemm_rect_slabs(const GemmParams& p, char* lds, 
         for (int i = 0; i < PA; ++i) load_a(UNIT_A, i, 1, k1);
 #pragma unroll
         for (int i = 0; i < PW; ++i) load_w(UNIT_W, i, 1, k1);
+        ahead();
         wait_loads_and_barrier<PA + PW>();
 #pragma unroll
         for (int r = 0; r < READS; ++r) read_frag(0, 0, 0, 0, r);
