@@ -15,16 +15,20 @@ namespace flux {
 constexpr int kRopeBlock = 256;
 constexpr int kRopeHeads = 8;    // heads a thread walks with the same angles
 constexpr int kRopePairs = FLUX_ROPE_MOST_DIM / 2;
+constexpr int kFewPairs = 64;    // of heads of up to 128
 
+// P: pairs that a launch's arguments have room for.
+template <int P>
 struct RopeIds {
     const void* ids;
     int64_t sb, sl, sa;
     int dtype;
-    double turns[kRopePairs];      // theta^(-2j/d) / 2 pi of every pair
-    unsigned char axis[kRopePairs];
+    double turns[P];      // theta^(-2j/d) / 2 pi of every pair
+    unsigned char axis[P];
 };
 
-__device__ __forceinline__ double position(const RopeIds& r, int64_t at) {
+template <int P>
+__device__ __forceinline__ double position(const RopeIds<P>& r, int64_t at) {
     switch (r.dtype) {   // (uniform)
         case FLUX_IDS_F32: return static_cast<const float*>(r.ids)[at];
         case FLUX_IDS_F64: return static_cast<const double*>(r.ids)[at];
@@ -51,17 +55,18 @@ struct RopeSide {
     const void* x; void* y;
     int64_t sb, sh, sl;
 };
+template <int P>
 struct RopeNd {
     RopeSide q, k;
     int64_t L;
     int Hq, H;            // heads of q; of both, k's behind q's
     int D, lanes;         // lanes: threads of a row
     float sign;
-    RopeIds at;
+    RopeIds<P> at;
 };
 
-template <typename T, int VEC>
-__global__ __launch_bounds__(kRopeBlock) void rope_nd_kernel(RopeNd p) {
+template <typename T, int VEC, int P>
+__global__ __launch_bounds__(kRopeBlock) void rope_nd_kernel(RopeNd<P> p) {
     const int rows = kRopeBlock / p.lanes;                 // positions of a workgroup
     const int row = threadIdx.x / p.lanes, lane = threadIdx.x - row * p.lanes;
     // Consecutive workgroups go round the eight XCDs; each of them takes one eighth of the sequence in which the head groups of a
@@ -135,7 +140,8 @@ __global__ __launch_bounds__(kRopeBlock) void rope_nd_kernel(RopeNd p) {
 }
 
 // A thread a matrix.
-__global__ __launch_bounds__(kRopeBlock) void rope_table_kernel(RopeIds at, float* out, int64_t L, int pairs, int64_t total) {
+template <int P>
+__global__ __launch_bounds__(kRopeBlock) void rope_table_kernel(RopeIds<P> at, float* out, int64_t L, int pairs, int64_t total) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * kRopeBlock + threadIdx.x;
     if (i >= total) return;
     const int64_t row = i / pairs, b = row / L, pos = row - b * L;
@@ -148,25 +154,33 @@ __global__ __launch_bounds__(kRopeBlock) void rope_table_kernel(RopeIds at, floa
 
 // The frequencies of every pair, in turns: r^j with r = theta^(-2/d), eight apart from one another by one multiplication, so that pair j
 // carries j / 8 roundings of 2^-53 and the angle as many of the rounding that its product with the position has anyway.
-static int read_ids(const flux_rope_ids& a, RopeIds& r, int& pairs, const char* what) {
-    if (!a.ids) return fail(FLUX_E_NULL, "%s: null ids", what);
-    if (a.dtype < FLUX_IDS_F32 || a.dtype > FLUX_IDS_I64) return fail(FLUX_E_DTYPE, "%s: unsupported type of ids %d", what, a.dtype);
-    if (a.n_axes < 1 || a.n_axes > FLUX_ROPE_MOST_AXES) return fail(FLUX_E_SHAPE, "%s: %d axes, 1 to %d are taken", what, a.n_axes, FLUX_ROPE_MOST_AXES);
-    if (!(a.theta > 0.0) || !std::isfinite(a.theta)) return fail(FLUX_E_SHAPE, "%s: theta must be a positive number", what);
+template <int P>
+static void read_ids(const flux_rope_ids& a, RopeIds<P>& r) {
     r.ids = a.ids;
     r.sb = a.sb;
     r.sl = a.sl;
     r.sa = a.sa;
     r.dtype = a.dtype;
-    pairs = 0;
+    int pairs = 0;
     for (int i = 0; i < a.n_axes; ++i) {
         const int d = a.axes_dim[i];
-        if (d <= 0 || d % 2 != 0 || pairs + d / 2 > kRopePairs) return fail(FLUX_E_SHAPE, "%s: axes of an even number of values, %d in all at most", what, FLUX_ROPE_MOST_DIM);
         const double step = std::log2(a.theta) * -2.0 / d, r8 = std::exp2(8 * step);
         for (int j = 0; j < d / 2; ++j) {
             r.turns[pairs + j] = j < 8 ? std::exp2(j * step) * 0.15915494309189533577 : r.turns[pairs + j - 8] * r8;
             r.axis[pairs + j] = static_cast<unsigned char>(i);
         }
+        pairs += d / 2;
+    }
+}
+static int check_ids(const flux_rope_ids& a, int& pairs, const char* what) {
+    if (!a.ids) return fail(FLUX_E_NULL, "%s: null ids", what);
+    if (a.dtype < FLUX_IDS_F32 || a.dtype > FLUX_IDS_I64) return fail(FLUX_E_DTYPE, "%s: unsupported type of ids %d", what, a.dtype);
+    if (a.n_axes < 1 || a.n_axes > FLUX_ROPE_MOST_AXES) return fail(FLUX_E_SHAPE, "%s: %d axes, 1 to %d are taken", what, a.n_axes, FLUX_ROPE_MOST_AXES);
+    if (!(a.theta > 0.0) || !std::isfinite(a.theta)) return fail(FLUX_E_SHAPE, "%s: theta must be a positive number", what);
+    pairs = 0;
+    for (int i = 0; i < a.n_axes; ++i) {
+        const int d = a.axes_dim[i];
+        if (d <= 0 || d % 2 != 0 || d > FLUX_ROPE_MOST_DIM || pairs + d / 2 > kRopePairs) return fail(FLUX_E_SHAPE, "%s: axes of an even number of values, %d in all at most", what, FLUX_ROPE_MOST_DIM);
         pairs += d / 2;
     }
     return FLUX_OK;
@@ -177,17 +191,33 @@ static bool vectors(const flux_src4& s, const void* out) {
     return s.ptr == nullptr || (aligned16(s.ptr) && aligned16(out) && s.sb % Elem<T>::VEC == 0 && s.sh % Elem<T>::VEC == 0 && s.sl % Elem<T>::VEC == 0);
 }
 
-template <typename T>
-static int rope_launch(const flux_rope_nd_args& a, RopeNd& p, hipStream_t st) {
+template <typename T, int P>
+static int rope_launch(const flux_rope_nd_args& a, hipStream_t st) {
+    RopeNd<P> p;
+    read_ids(a.at, p.at);
+    p.q = {a.q.ptr, a.q_out, a.q.sb, a.q.sh, a.q.sl};
+    p.k = {a.k.ptr, a.k_out, a.k.sb, a.k.sh, a.k.sl};
+    p.L = a.L;
+    p.Hq = static_cast<int>(a.Hq);
+    p.H = static_cast<int>(a.Hq + a.Hk);
+    p.D = a.D;
+    p.sign = a.inverse ? -1.0f : 1.0f;
     const bool wide = a.D % Elem<T>::VEC == 0 && vectors<T>(a.q, a.q_out) && vectors<T>(a.k, a.k_out);
     p.lanes = a.D / (wide ? Elem<T>::VEC : 2);
     const int rows = kRopeBlock / p.lanes;
     const int64_t blocks = (a.L + rows - 1) / rows * ((p.H + kRopeHeads - 1) / kRopeHeads);
     if (a.B > 65535 || blocks > (int64_t{1} << 32) / kRopeBlock - 8) return fail(FLUX_E_SHAPE, "flux_rope_nd: grid too large (B=%lld, L=%lld, %d heads)", (long long)a.B, (long long)a.L, p.H);
     const dim3 grid((unsigned)((blocks + 7) / 8 * 8), (unsigned)a.B);
-    if (wide) hipLaunchKernelGGL((rope_nd_kernel<T, Elem<T>::VEC>), grid, dim3(kRopeBlock), 0, st, p);
-    else hipLaunchKernelGGL((rope_nd_kernel<T, 2>), grid, dim3(kRopeBlock), 0, st, p);
+    if (wide) hipLaunchKernelGGL((rope_nd_kernel<T, Elem<T>::VEC, P>), grid, dim3(kRopeBlock), 0, st, p);
+    else hipLaunchKernelGGL((rope_nd_kernel<T, 2, P>), grid, dim3(kRopeBlock), 0, st, p);
     return check_launch("flux_rope_nd");
+}
+
+template <int P>
+static void table_launch(const flux_rope_ids& at, float* out, int64_t L, int pairs, int64_t total, hipStream_t st) {
+    RopeIds<P> r;
+    read_ids(at, r);
+    hipLaunchKernelGGL((rope_table_kernel<P>), dim3((unsigned)((total + kRopeBlock - 1) / kRopeBlock)), dim3(kRopeBlock), 0, st, r, out, L, pairs, total);
 }
 
 }  // namespace flux
@@ -199,21 +229,13 @@ extern "C" int flux_rope_nd(const flux_rope_nd_args* a, void* stream) {
     if (a->B < 0 || a->L < 0 || a->Hq < 0 || a->Hk < 0 || a->Hq + a->Hk > 0x7ffffff || a->L > 0x7fffffffLL) return fail(FLUX_E_SHAPE, "flux_rope_nd: bad shape B=%lld Hq=%lld Hk=%lld L=%lld", (long long)a->B, (long long)a->Hq, (long long)a->Hk, (long long)a->L);
     if (a->B == 0 || a->L == 0 || a->Hq + a->Hk == 0) return FLUX_OK;
     if ((a->Hq > 0 && (!a->q.ptr || !a->q_out)) || (a->Hk > 0 && (!a->k.ptr || !a->k_out))) return fail(FLUX_E_NULL, "flux_rope_nd: null pointer");
-    RopeNd p = {};
     int pairs;
-    const int rc = read_ids(a->at, p.at, pairs, "flux_rope_nd");
+    const int rc = check_ids(a->at, pairs, "flux_rope_nd");
     if (rc != FLUX_OK) return rc;
     if (a->D != 2 * pairs) return fail(FLUX_E_SHAPE, "flux_rope_nd: axes of %d values in all for rows of %d", 2 * pairs, a->D);
-    p.q = {a->q.ptr, a->q_out, a->q.sb, a->q.sh, a->q.sl};
-    p.k = {a->k.ptr, a->k_out, a->k.sb, a->k.sh, a->k.sl};
-    p.L = a->L;
-    p.Hq = static_cast<int>(a->Hq);
-    p.H = static_cast<int>(a->Hq + a->Hk);
-    p.D = a->D;
-    p.sign = a->inverse ? -1.0f : 1.0f;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a->dtype == FLUX_BF16) return rope_launch<bf16_t>(*a, p, st);
-    if (a->dtype == FLUX_F32) return rope_launch<float>(*a, p, st);
+    if (a->dtype == FLUX_BF16) return pairs <= kFewPairs ? rope_launch<bf16_t, kFewPairs>(*a, st) : rope_launch<bf16_t, kRopePairs>(*a, st);
+    if (a->dtype == FLUX_F32) return pairs <= kFewPairs ? rope_launch<float, kFewPairs>(*a, st) : rope_launch<float, kRopePairs>(*a, st);
     return fail(FLUX_E_DTYPE, "flux_rope_nd: unsupported dtype %d", a->dtype);
 }
 
@@ -221,14 +243,14 @@ extern "C" int flux_rope_table(const flux_rope_ids* at, float* out, int64_t B, i
     if (!at) return fail(FLUX_E_NULL, "flux_rope_table: null args");
     if (B < 0 || L < 0 || B > 0x7fffffffLL || L > 0x7fffffffLL) return fail(FLUX_E_SHAPE, "flux_rope_table: bad shape B=%lld L=%lld", (long long)B, (long long)L);
     if (B == 0 || L == 0) return FLUX_OK;
-    RopeIds r = {};
     int pairs;
-    const int rc = read_ids(*at, r, pairs, "flux_rope_table");
+    const int rc = check_ids(*at, pairs, "flux_rope_table");
     if (rc != FLUX_OK) return rc;
     if (!out) return fail(FLUX_E_NULL, "flux_rope_table: null pointer");
     if (!aligned16(out)) return fail(FLUX_E_ALIGN, "flux_rope_table: the table is not 16-byte aligned");
     if (B * L > ((int64_t{1} << 32) - kRopeBlock) / pairs) return fail(FLUX_E_SHAPE, "flux_rope_table: too many positions");
     const int64_t total = B * L * pairs;
-    hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)((total + kRopeBlock - 1) / kRopeBlock)), dim3(kRopeBlock), 0, static_cast<hipStream_t>(stream), r, out, L, pairs, total);
+    if (pairs <= kFewPairs) table_launch<kFewPairs>(*at, out, L, pairs, total, static_cast<hipStream_t>(stream));
+    else table_launch<kRopePairs>(*at, out, L, pairs, total, static_cast<hipStream_t>(stream));
     return check_launch("flux_rope_table");
 }
