@@ -8,8 +8,9 @@ namespace flux {
 
 constexpr int kPairThreads = 512;
 
-template <int FM, int FN, int ST, bool KTAIL, int G>
-__device__ __forceinline__ void gemm_pair_slabs(const GemmParams& p, char* lds, int m0, int n0, int kb, int ke, int turn, int turns, int w4, int lane, f32x4 (&acc)[FM][FN]) {
+// ahead(): loads of the caller's own, requested behind those of the first slabs; they have landed on return.
+template <int FM, int FN, int ST, bool KTAIL, int G, typename Ahead>
+__device__ __forceinline__ void gemm_pair_slabs(const GemmParams& p, char* lds, int m0, int n0, int kb, int ke, int turn, int turns, int w4, int lane, f32x4 (&acc)[FM][FN], Ahead ahead) {
     constexpr int BM = 32 * FM, BN = 32 * FN, BK = 64, ROWB = BK * 2;
     constexpr int SLAB = (BM + BN) * ROWB;       // A rows, then W rows
     constexpr int NL = (FM + FN + 1 - G) / 2;    // loads of this wave per slab: passes of 32 rows, every other one
@@ -103,6 +104,7 @@ __device__ __forceinline__ void gemm_pair_slabs(const GemmParams& p, char* lds, 
 #pragma unroll
         for (int j = 0; j < NL; ++j) load(s * SLAB, j, k);
     }
+    ahead();
     wait_loads_and_barrier<(ST - 1) * NL>();
 #pragma unroll
     for (int r = 0; r < READS; ++r) read_frag(0, 0, r);
@@ -123,10 +125,13 @@ __device__ __forceinline__ void gemm_pair_slabs(const GemmParams& p, char* lds, 
     wait_vmem_all();
 }
 
-// A workgroup's tile, or its part of one. `tail(acc, first row, first column, p)` adds to the sums of a wave's fragment rows before their epilogue
-// (NoTail: nothing).
+// A workgroup's tile, or its part of one. `tail` adds to the sums of a wave's fragment rows before their epilogue (finish) and may ask for what that
+// takes in front of the first slabs (begin) and behind them (touch). NoTail: nothing.
 struct NoTail {
-    template <int ROWS, int FN> __device__ __forceinline__ void operator()(f32x4 (&)[ROWS][FN], int, int, const GemmParams&) const {}
+    template <int ROWS, int FN> struct Ahead {};
+    template <int ROWS, int FN> __device__ __forceinline__ void begin(Ahead<ROWS, FN>&, int, const GemmParams&) const {}
+    template <int ROWS, int FN> __device__ __forceinline__ void touch(Ahead<ROWS, FN>&, int, int, const GemmParams&) const {}
+    template <int ROWS, int FN> __device__ __forceinline__ void finish(f32x4 (&)[ROWS][FN], Ahead<ROWS, FN>&, int, int, const GemmParams&) const {}
 };
 template <int FM, int FN, int ST, bool KTAIL, bool SPLIT, typename Tail>
 __global__ __launch_bounds__(kPairThreads) void gemm_nt_pair_kernel(GemmLaunch L, Tail tail) {
@@ -157,7 +162,8 @@ __global__ __launch_bounds__(kPairThreads) void gemm_nt_pair_kernel(GemmLaunch L
     const int w4 = wave & 3;
     const int kb = split * L.slabs_per_split, ke = min((p.K + BK - 1) / BK, kb + L.slabs_per_split);
     f32x4* const ex = reinterpret_cast<f32x4*>(lds) + w4 * (FM * FN * 64) + lane;   // exchange: 64 lanes x 16 bytes per fragment
-    auto finish = [&](auto gc, f32x4 (&acc)[FM][FN]) {
+    const int wm0 = m0 + (w4 >> 1) * (16 * FM), wn0 = n0 + (w4 & 1) * (16 * FN);
+    auto finish = [&](auto gc, f32x4 (&acc)[FM][FN], auto& have) {
         constexpr int G = decltype(gc)::value, OWN0 = G == 0 ? 0 : R0, OWN = G == 0 ? R0 : R1, GIVE0 = G == 0 ? R0 : 0, GIVE = FM - OWN;
         __syncthreads();                       // everyone is done with the ring
 #pragma unroll
@@ -177,18 +183,22 @@ __global__ __launch_bounds__(kPairThreads) void gemm_nt_pair_kernel(GemmLaunch L
 #pragma unroll
                 for (int j = 0; j < FN; ++j) dst[((OWN0 + i) * FN + j) * 64] = own[i][j];
         } else {
-            tail(own, m0 + (w4 >> 1) * (16 * FM) + OWN0 * 16, n0 + (w4 & 1) * (16 * FN), p);
+            tail.finish(own, have, wm0 + OWN0 * 16, wn0, p);
             __syncthreads();                   // the exchange has been read: its LDS is the epilogue's now
             gemm_finish_rect<FM, FN, OWN, FN != 8>(p, own, lds + G * (ST * (BM + BN) * BK), m0, n0, OWN0, w4, lane);
         }
     };
     f32x4 acc[FM][FN];
     if (wave < 4) {
-        gemm_pair_slabs<FM, FN, ST, KTAIL, 0>(p, lds, m0, n0, kb, ke, turn, turns, w4, lane, acc);
-        finish(ic<0>(), acc);
+        typename Tail::template Ahead<R0, FN> have;
+        if (!SPLIT) tail.begin(have, wm0, p);
+        gemm_pair_slabs<FM, FN, ST, KTAIL, 0>(p, lds, m0, n0, kb, ke, turn, turns, w4, lane, acc, [&]() { if (!SPLIT) tail.touch(have, wm0, wn0, p); });
+        finish(ic<0>(), acc, have);
     } else {
-        gemm_pair_slabs<FM, FN, ST, KTAIL, 1>(p, lds, m0, n0, kb, ke, turn, turns, w4, lane, acc);
-        finish(ic<1>(), acc);
+        typename Tail::template Ahead<R1, FN> have;
+        if (!SPLIT) tail.begin(have, wm0 + R0 * 16, p);
+        gemm_pair_slabs<FM, FN, ST, KTAIL, 1>(p, lds, m0, n0, kb, ke, turn, turns, w4, lane, acc, [&]() { if (!SPLIT) tail.touch(have, wm0 + R0 * 16, wn0, p); });
+        finish(ic<1>(), acc, have);
     }
 }
 
@@ -206,17 +216,21 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_reduce_kernel(GemmLaunch L,
     const int m0 = tm * BM, n0 = tn * BN;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm0 = m0 + (wave >> 1) * (16 * FM) + row * 16, wn0 = n0 + (wave & 1) * (16 * FN);
+    typename Tail::template Ahead<1, FN> have;
+    tail.begin(have, wm0, p);
     const f32x4* src = reinterpret_cast<const f32x4*>(L.partial) + (static_cast<int64_t>(t) * 4 + wave) * (FM * FN * 64) + row * (FN * 64) + lane;
     const int64_t part = static_cast<int64_t>(tiles) * 4 * (FM * FN * 64);
     f32x4 acc[1][FN];
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[0][j] = src[j * 64];
+    tail.touch(have, wm0, wn0, p);
     for (int s = 1; s < L.splits; ++s) {
         src += part;
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[0][j] += src[j * 64];
     }
-    tail(acc, m0 + (wave >> 1) * (16 * FM) + row * 16, n0 + (wave & 1) * (16 * FN), p);
+    tail.finish(acc, have, wm0, wn0, p);
     gemm_finish_rect<FM, FN, 1, FN != 8>(p, acc, lds, m0, n0, row, wave, lane);
 }
 

@@ -60,55 +60,70 @@ struct LoraTail {
         for (int i = 0; i < ROWS; ++i) to.low[i] = *reinterpret_cast<const u32x4*>(row + (static_cast<uint32_t>(min(i * 16 + frow, p.M - 1 - m0)) * width + at));
     }
 
-    // What a wave asks for before its sums are complete: the adapters of its rows, and one value of every row of the first step's operands for the
-    // adapter of its first row (whose number comes through the scalar cache, so that nothing waits for it): they are then in the L2. Requested
-    // behind the loop over K alone, a tile waits for memory three times in a row with nothing beside it. (The operands themselves do not fit
-    // beside the loop's: with them the loop moved 350 registers a slab.)
+    static constexpr int kNone = 0x7fffffff;
+    // The next adapter behind `last` of a wave's rows.
+    template <int ROWS>
+    static __device__ __forceinline__ int behind(const int (&own)[ROWS], int last) {
+        int next = kNone;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) next = own[i] > last ? min(next, own[i]) : next;
+        return first_of_rows(next);
+    }
+
+    // What a wave asks for before its sums are complete: the adapters of its rows, in front of everything else (begin), and behind its first slabs
+    // one value of every row of the first step's operands for the first adapters, so that they are in the L2 when it comes to them (touch).
+    // Requested behind the loop over K alone, a tile waits for memory three times in a row with nothing beside it. (The operands themselves do not
+    // fit beside the loop's: with them the 256-wide tile moved 450 registers a slab.)
+    static constexpr int kTouch = 3;
+    // Not for the 192 x 192 tile, whose two groups of waves have no registers to spare beside the loop's.
+    template <int ROWS, int FN> static constexpr bool kAhead = !(ROWS == 3 && FN == 6);
     template <int ROWS, int FN>
     struct Ahead {
         int own[ROWS];
-        uint32_t touched[(ROWS + 3) / 4 + (FN + 3) / 4];
+        uint32_t low[(ROWS + 3) / 4], b[kTouch][(FN + 3) / 4];
     };
     template <int ROWS, int FN>
-    __device__ __forceinline__ void request(Ahead<ROWS, FN>& to, int a, int m0, int n0, const GemmParams& p) const {
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) to.own[i] = owner[min(m0 + i * 16 + (lane & 15), p.M - 1)];
-#pragma unroll
-        for (int i = 0; i < (ROWS + 3) / 4; ++i) to.touched[i] = *reinterpret_cast<const uint32_t*>(low + static_cast<int64_t>(min(m0 + min(i * 64 + lane, ROWS * 16 - 1), p.M - 1)) * width);
-#pragma unroll
-        for (int i = 0; i < (FN + 3) / 4; ++i) to.touched[(ROWS + 3) / 4 + i] = b[(static_cast<int64_t>(max(a, 0)) * p.N + min(n0 + min(i * 64 + lane, FN * 16 - 1), p.N - 1)) * rank];
+    __device__ __forceinline__ void begin(Ahead<ROWS, FN>& to, int m0, const GemmParams& p) const {
+        if constexpr (kAhead<ROWS, FN>) owners(to.own, m0, p);
     }
-    __device__ __forceinline__ int first_owner(int m0, const GemmParams& p) const {
-        typedef const __attribute__((address_space(4))) int* scalar;
-        return *(scalar)(reinterpret_cast<uintptr_t>(owner + min(m0, p.M - 1)));
-    }
-
-    template <int ROWS, int FN>
-    __device__ __forceinline__ void operator()(f32x4 (&acc)[ROWS][FN], int m0, int n0, const GemmParams& p) const {
-        if (m0 >= p.M || n0 >= p.N) return;
-        int own[ROWS];
+    template <int ROWS>
+    __device__ __forceinline__ void owners(int (&own)[ROWS], int m0, const GemmParams& p) const {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) own[i] = owner[min(m0 + i * 16 + static_cast<int>(threadIdx.x & 15), p.M - 1)];
-        finish(acc, own, m0, n0, p);
+    }
+    template <int ROWS, int FN>
+    __device__ __forceinline__ void touch(Ahead<ROWS, FN>& to, int m0, int n0, const GemmParams& p) const {
+        if constexpr (!kAhead<ROWS, FN>) return;
+        const int lane = threadIdx.x & 63;
+        int a = behind(to.own, -1), last = 0;
+#pragma unroll
+        for (int t = 0; t < kTouch; ++t) {   // (fewer adapters than that: the last one again)
+            last = a == kNone ? last : a;
+#pragma unroll
+            for (int i = 0; i < (FN + 3) / 4; ++i) to.b[t][i] = b[(static_cast<int64_t>(last) * p.N + min(n0 + min(i * 64 + lane, FN * 16 - 1), p.N - 1)) * rank];
+            if (t + 1 < kTouch) a = a == kNone ? a : behind(to.own, a);
+        }
+#pragma unroll
+        for (int i = 0; i < (ROWS + 3) / 4; ++i) to.low[i] = *reinterpret_cast<const uint32_t*>(low + static_cast<int64_t>(min(m0 + min(i * 64 + lane, ROWS * 16 - 1), p.M - 1)) * width);
     }
 
     template <int ROWS, int FN>
     __device__ __forceinline__ void finish(f32x4 (&acc)[ROWS][FN], Ahead<ROWS, FN>& have, int m0, int n0, const GemmParams& p) const {
+        if constexpr (kAhead<ROWS, FN>) {
 #pragma unroll
-        for (uint32_t& t : have.touched) asm volatile("" ::"v"(t));
+            for (uint32_t& t : have.low) asm volatile("" ::"v"(t));
+#pragma unroll
+            for (auto& t : have.b)
+#pragma unroll
+                for (uint32_t& v : t) asm volatile("" ::"v"(v));
+        } else {
+            owners(have.own, m0, p);
+        }
         if (m0 < p.M && n0 < p.N) finish(acc, have.own, m0, n0, p);
     }
     template <int ROWS, int FN>
     __device__ __forceinline__ void finish(f32x4 (&acc)[ROWS][FN], const int (&own)[ROWS], int m0, int n0, const GemmParams& p) const {
-        constexpr int kNone = 0x7fffffff;
-        auto behind = [&](int last) {   // the next adapter of these rows
-            int next = kNone;
-#pragma unroll
-            for (int i = 0; i < ROWS; ++i) next = own[i] > last ? min(next, own[i]) : next;
-            return first_of_rows(next);
-        };
-        int a = behind(-1);
+        int a = behind(own, -1);
         if (a == kNone) return;
         bool same = true;
 #pragma unroll
@@ -152,7 +167,7 @@ struct LoraTail {
             k += 32;
             if (k >= width) {
                 k = 0;
-                a = behind(a);
+                a = behind(own, a);
                 if (a == kNone) break;
             }
         }
@@ -165,10 +180,10 @@ struct LoraTail {
 
     // The smallest value of the wave's 16 rows (lanes 16 apart hold the same row), as a scalar.
     static __device__ __forceinline__ int first_of_rows(int v) {
-        v = min(v, __shfl_xor(v, 1));
-        v = min(v, __shfl_xor(v, 2));
-        v = min(v, __shfl_xor(v, 4));
-        v = min(v, __shfl_xor(v, 8));
+        v = min(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xf, 0xf, true));    // lane ^ 1
+        v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xf, 0xf, true));    // lane ^ 2
+        v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xf, 0xf, true));   // mirrored within 8
+        v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xf, 0xf, true));   // mirrored within 16
         return __builtin_amdgcn_readfirstlane(v);
     }
 };
@@ -183,8 +198,8 @@ __device__ __forceinline__ void hold(f32x4 (&acc)[ROWS][FN]) {
         for (int j = 0; j < FN; ++j) asm volatile("" : "+a"(acc[i][j]));
 }
 
-// The same for row vectors (gemm_rows.h): lane l adds the products of the rank's values l, l + 64, ... to its share of a sum. The first 64 of
-// them are requested in front of W.
+// The same for row vectors (gemm_rows.h): lane l adds the products of the rank's values l, l + 64, ... to its share of a sum. The adapters' numbers come
+// through the scalar cache and the first 64 values behind the first vectors of W, which so wait for nothing.
 template <int MM>
 struct LoraRowTail {
     LoraTail t;
@@ -192,11 +207,15 @@ struct LoraRowTail {
     bf16_t low[MM], b[kGemvCols][MM];
     int64_t row_b[kGemvCols][MM];
 
+    __device__ __forceinline__ void begin() {
+        typedef const __attribute__((address_space(4))) int* scalar;
+#pragma unroll
+        for (int m = 0; m < MM; ++m) own[m] = ((scalar)(reinterpret_cast<uintptr_t>(t.owner)))[m];
+    }
     __device__ __forceinline__ void request(int n0, int lane, const GemmParams& p) {
         const int r = lane < t.rank ? lane : 0;
 #pragma unroll
         for (int m = 0; m < MM; ++m) {
-            own[m] = t.owner[m];
             low[m] = t.low[static_cast<int64_t>(m) * t.width + r];
 #pragma unroll
             for (int c = 0; c < kGemvCols; ++c) {

@@ -208,10 +208,11 @@ __global__ __launch_bounds__(kGemmThreads) void lora_ring_kernel(GemmLaunch L, L
     const int m0 = tm * BM, n0 = tn * BM;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm0 = m0 + (wave >> 1) * (32 * MI), wn0 = n0 + (wave & 1) * (32 * MI), first = tail.first_owner(wm0, p);
+    const int wm0 = m0 + (wave >> 1) * (32 * MI), wn0 = n0 + (wave & 1) * (32 * MI);
     LoraTail::Ahead<2 * MI, 2 * MI> have;
+    tail.begin(have, wm0, p);
     f32x4 acc[2 * MI][2 * MI];
-    gemm_tile_slabs<MI, KTAIL>(p, lds, m0, n0, (p.K + BK - 1) / BK, acc, [&]() { tail.request(have, first, wm0, wn0, p); });
+    gemm_tile_slabs<MI, KTAIL>(p, lds, m0, n0, (p.K + BK - 1) / BK, acc, [&]() { tail.touch(have, wm0, wn0, p); });
     hold(acc);
     tail.finish(acc, have, wm0, wn0, p);
     gemm_epilogue<MI, MI>(p, acc, lds, m0, n0, wave, lane);
@@ -227,10 +228,11 @@ __global__ __launch_bounds__(kGemmThreads) void lora_rect_kernel(GemmLaunch L, L
     const int m0 = tm * BM, n0 = tn * BN;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm0 = m0 + (wave >> 1) * (16 * FM), wn0 = n0 + (wave & 1) * (16 * FN), first = tail.first_owner(wm0, p);
+    const int wm0 = m0 + (wave >> 1) * (16 * FM), wn0 = n0 + (wave & 1) * (16 * FN);
     LoraTail::Ahead<FM, FN> have;
+    tail.begin(have, wm0, p);
     f32x4 acc[FM][FN];
-    gemm_rect_slabs<FM, FN, KTAIL>(p, lds, m0, n0, (p.K + BK - 1) / BK, acc, [&]() { tail.request(have, first, wm0, wn0, p); });
+    gemm_rect_slabs<FM, FN, KTAIL>(p, lds, m0, n0, (p.K + BK - 1) / BK, acc, [&]() { tail.touch(have, wm0, wn0, p); });
     hold(acc);
     tail.finish(acc, have, wm0, wn0, p);
     gemm_finish_rect<FM, FN, FM, false>(p, acc, lds, m0, n0, 0, wave, lane);

@@ -59,8 +59,10 @@ constexpr int kGemvSiluLds = 48 * 1024;  // bytes of LDS for the (activated) inp
 // EXACT: K = 512 * U, so every lane has exactly U vectors per row and the K loop runs once, without tests.
 // ONCE: W is read with the non-temporal hint (see launch_gemv).
 // block: which 4 * kGemvCols columns; act_lds: MM * K * 2 bytes with SILU_LDS.
-// tail: request(first column, lane, p) goes out in front of W, add(sums, lane) to what each lane has summed up (NoRowTail: nothing).
+// tail: begin() comes first of all, request(first column, lane, p) behind the first vectors of W, add(sums, lane) to what each lane has summed
+// up (NoRowTail: nothing).
 struct NoRowTail {
+    __device__ __forceinline__ void begin() {}
     __device__ __forceinline__ void request(int, int, const GemmParams&) {}
     template <int MM> __device__ __forceinline__ void add(float (&)[kGemvCols][MM], int) {}
 };
@@ -84,7 +86,7 @@ __device__ __forceinline__ void gemv_small_m(const GemmParams& p, int block, cha
     bf16_t bias_raw[CPW];
 #pragma unroll
     for (int c = 0; c < CPW; ++c) bias_raw[c] = p.bias ? p.bias[min(n0 + c, p.N - 1)] : static_cast<bf16_t>(0);
-    tail.request(n0, lane, p);
+    tail.begin();
     Vec16<bf16_t> pre[PRE];
     if (SILU_LDS) {
 #pragma unroll
@@ -109,6 +111,7 @@ __device__ __forceinline__ void gemv_small_m(const GemmParams& p, int block, cha
         }
     };
     if (EXACT || lane * 8 < p.K) request_w(lane * 8);
+    tail.request(n0, lane, p);
     if (SILU_LDS) {
         __builtin_amdgcn_sched_barrier(0);
         bf16_t* dst = reinterpret_cast<bf16_t*>(act_lds);
