@@ -623,7 +623,7 @@ static int read_lora_args(const flux_linear_lora_args* a, LoraCall& c) {
     c.tail = {nullptr, nullptr, static_cast<const bf16_t*>(a->lora_b), a->rank, width,
               a->rank % 8 == 0 && aligned16(a->lora_b) ? 8 : a->rank % 4 == 0 && (reinterpret_cast<uintptr_t>(a->lora_b) & 7u) == 0 ? 4 : 1};
     c.low = {static_cast<const bf16_t*>(a->x), static_cast<const bf16_t*>(a->lora_a), a->adapter, a->scaling, nullptr, nullptr, a->ldx, a->M / a->requests,
-             static_cast<int>(a->M), static_cast<int>(a->K), a->rank, width, a->adapters, a->wide_ids != 0, a->K % 8 == 0 && a->ldx % 8 == 0 && aligned16(a->x) && aligned16(a->lora_a) && a->ldx * 2 * 16 < 0x7fffffffLL && a->K * 2 * 64 < 0x7fffffffLL};
+             static_cast<int>(a->M), static_cast<int>(a->K), a->rank, width, a->adapters, a->wide_ids != 0, a->K % 8 == 0 && a->ldx % 8 == 0 && aligned16(a->x) && aligned16(a->lora_a) && a->ldx * 2 * 32 < 0x7fffffffLL && a->K * 2 * 64 < 0x7fffffffLL};
     return FLUX_OK;
 }
 

@@ -189,7 +189,7 @@ struct LoraTail {
 };
 
 // The sums are in accumulation registers from here on. Without it the compiler settles the whole kernel's registers by what happens behind the loop
-// over K: 360 moves between accumulation and ordinary registers a slab inside it, 1071 us for 783 at 13008 x 12288 x 3072.
+// over K: 360 moves between accumulation and ordinary registers a slab inside it, 1071 us for 814 at 13008 x 12288 x 3072.
 template <int ROWS, int FN>
 __device__ __forceinline__ void hold(f32x4 (&acc)[ROWS][FN]) {
 #pragma unroll

@@ -170,16 +170,21 @@ void launch_lora_low(const LoraLow& p, hipStream_t st) {
         return;
     }
 #define CALL(R, NF, W) hipLaunchKernelGGL((lora_low_kernel<R, NF, W>), grid(R * 16, NF * 16), dim3(W * 64), 0, st, p)
-    const int tiles = (p.M + 15) / 16;
+    // 32 rows a tile where 256 tiles of 16 would be left, since a comes once a tile. As many waves as the CU's 160 KB hold of one workgroup at
+    // a time or two share K, and four where every CU gets several workgroups by itself. us of the whole operator, N = 128, K = 3072, for 16 rows of 8
+    // waves, 32 rows of 8 (rank 64: 6) and 32 rows of 4: rank 32: 19.4, 20.4 and 24.3 at 2304 rows, 28.0, 25.5 and 29.1 at 4608, rank 16: 42.8, 42.2 and
+    // 41.3 at 13008; rank 64: 23.0, 25.1 and 29.1 at 2304, 33.9, 29.9 and 33.0 at 4608, 57.3, 53.0 and 50.2 at 13008. (16 rows of 16 and 4 waves at
+    // 517, rank 16: 18.1 and 21.2, of 8: 18.3.)
+    const bool few = (p.M + 15) / 16 < 256;
+    const int64_t blocks = static_cast<int64_t>((p.M + 31) / 32) * ((p.width + 63) / 64);
     if (p.width <= 32) {
-        if (tiles >= 512) CALL(1, 2, 4);
-        else if (tiles >= 128) CALL(1, 2, 8);
-        else CALL(1, 2, 16);
+        if (few) CALL(1, 2, 8);
+        else if (blocks <= 256) CALL(2, 2, 8);
+        else CALL(2, 2, 4);
     } else {
-        // us at 4608 x 3072, rank 64, 16 rows of eight waves and 32 rows of six: 20.6 and 16.0 (a CU takes in about 50 bytes per ns, and a comes once a tile)
-        if (tiles >= 256) CALL(2, 4, 6);
-        else if (tiles >= 128) CALL(1, 4, 8);
-        else CALL(1, 4, 16);
+        if (few) CALL(1, 4, 8);
+        else if (blocks <= 256) CALL(2, 4, 6);
+        else CALL(2, 4, 4);
     }
 #undef CALL
 }
