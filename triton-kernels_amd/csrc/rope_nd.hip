@@ -3,8 +3,8 @@
 //   (x0, x1) -> (x0 c - x1 s, x0 s + x1 c),  angle = ids[b, l, axis(pair)] theta^(-2j/d)
 //
 // Two reads and two writes of q and k and 3 operations a value: bound by HBM, if the angles are not worked out once for every head. A
-// thread owns one 16-byte vector of a row (4 pairs of bf16, 2 of fp32) and walks the heads of its position, so an angle is worked out once for
-// eight heads and a row needs no exchange between lanes. In turns (angle / 2 pi, as the frequencies arrive here) an angle of any
+// thread owns one 16-byte vector of a row (4 pairs of bf16, 2 of fp32) and walks eight heads of its position, so an angle is worked out once for
+// all of them and a row needs no exchange between lanes. In turns (angle / 2 pi, as the frequencies arrive here) an angle of any
 // size loses its whole turns exactly in 64 bits; what is left of a quarter turn goes through the Taylor series of sine and cosine in fp32.
 #include "common.h"
 #include "../../include/flux_hip_tune.h"
@@ -13,7 +13,6 @@
 namespace flux {
 
 constexpr int kRopeBlock = 256;
-constexpr int kRopeHeads = 8;    // heads a thread walks with the same angles
 constexpr int kRopePairs = FLUX_ROPE_MOST_DIM / 2;
 constexpr int kFewPairs = 64;    // of heads of up to 128
 
@@ -65,22 +64,23 @@ struct RopeNd {
     RopeIds<P> at;
 };
 
-template <typename T, int VEC, int P>
+// HEADS: heads that a thread walks with the same angles.
+template <typename T, int VEC, int HEADS, int P>
 __global__ __launch_bounds__(kRopeBlock) void rope_nd_kernel(RopeNd<P> p) {
     const int rows = kRopeBlock / p.lanes;                 // positions of a workgroup
     const int row = threadIdx.x / p.lanes, lane = threadIdx.x - row * p.lanes;
     // Consecutive workgroups go round the eight XCDs; each of them takes one eighth of the sequence in which the head groups of a
     // stretch of positions follow one another, so that a row of a fused projection is fetched into one L2.
-    const int64_t head_groups = (p.H + kRopeHeads - 1) / kRopeHeads;
+    const int64_t head_groups = (p.H + HEADS - 1) / HEADS;
     const int64_t vb = static_cast<int64_t>(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
     const int64_t stretch = vb / head_groups, pos_raw = stretch * rows + row;
     if (row >= rows || pos_raw >= p.L) return;
-    const int h0 = static_cast<int>(vb - stretch * head_groups) * kRopeHeads;
+    const int h0 = static_cast<int>(vb - stretch * head_groups) * HEADS;
     const int64_t b = blockIdx.y, pos = pos_raw;
     const int c0 = lane * VEC;
 
     // a head's address is one of two affine functions; heads past the last are the last one again, loaded and not stored
-    T in[kRopeHeads][VEC];
+    T in[HEADS][VEC];
     auto side = [&](int h, int64_t& at_x, int64_t& at_y, const T*& x, T*& y) {
         const bool is_k = h >= p.Hq;
         const RopeSide& s = is_k ? p.k : p.q;
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kRopeBlock) void rope_nd_kernel(RopeNd<P> p) {
         at_y = ((b * heads + hs) * p.L + pos) * p.D + c0;
     };
 #pragma unroll
-    for (int i = 0; i < kRopeHeads; ++i) {
+    for (int i = 0; i < HEADS; ++i) {
         int64_t ax, ay;
         const T* x;
         T* y;
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kRopeBlock) void rope_nd_kernel(RopeNd<P> p) {
         s[i] *= p.sign;
     }
 #pragma unroll
-    for (int i = 0; i < kRopeHeads; ++i) {
+    for (int i = 0; i < HEADS; ++i) {
         if (h0 + i >= p.H) break;
         int64_t ax, ay;
         const T* x;
@@ -205,11 +205,23 @@ static int rope_launch(const flux_rope_nd_args& a, hipStream_t st) {
     const bool wide = a.D % Elem<T>::VEC == 0 && vectors<T>(a.q, a.q_out) && vectors<T>(a.k, a.k_out);
     p.lanes = a.D / (wide ? Elem<T>::VEC : 2);
     const int rows = kRopeBlock / p.lanes;
-    const int64_t blocks = (a.L + rows - 1) / rows * ((p.H + kRopeHeads - 1) / kRopeHeads);
+    const int64_t stretches = (a.L + rows - 1) / rows;
+    // Angles for eight heads at once where that leaves a workgroup for every CU, for two otherwise: with 256 of them and more the angles cost, with
+    // fewer the chain of a thread's loads and stores. us for eight, four, two and one (24 + 24 heads of 128, bf16): 155, 156, 178 and 264 at L = 32760,
+    // 21.9, 25.3, 31.3 and 39.7 at 4608, 8.8, 8.9, 9.5 and 11.5 at 1107, 5.2, 4.3, 4.3 and 4.4 at 256, 4.9, 3.9, 3.5 and 3.3 at 1.
+    const int heads = a.B * stretches * ((p.H + 7) / 8) >= 256 ? 8 : 2;
+    const int64_t blocks = stretches * ((p.H + heads - 1) / heads);
     if (a.B > 65535 || blocks > (int64_t{1} << 32) / kRopeBlock - 8) return fail(FLUX_E_SHAPE, "flux_rope_nd: grid too large (B=%lld, L=%lld, %d heads)", (long long)a.B, (long long)a.L, p.H);
     const dim3 grid((unsigned)((blocks + 7) / 8 * 8), (unsigned)a.B);
-    if (wide) hipLaunchKernelGGL((rope_nd_kernel<T, Elem<T>::VEC, P>), grid, dim3(kRopeBlock), 0, st, p);
-    else hipLaunchKernelGGL((rope_nd_kernel<T, 2, P>), grid, dim3(kRopeBlock), 0, st, p);
+#define CALL(V, HEADS) hipLaunchKernelGGL((rope_nd_kernel<T, V, HEADS, P>), grid, dim3(kRopeBlock), 0, st, p)
+    if (wide) {
+        if (heads == 8) CALL(Elem<T>::VEC, 8);
+        else CALL(Elem<T>::VEC, 2);
+    } else {
+        if (heads == 8) CALL(2, 8);
+        else CALL(2, 2);
+    }
+#undef CALL
     return check_launch("flux_rope_nd");
 }
 
