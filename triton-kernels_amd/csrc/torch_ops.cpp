@@ -360,6 +360,12 @@ void launch_layer_norm(const NormOf& c, const Tensor& x, const Tensor& w, const 
     check(flux_layer_norm(&a, stream_of(x)), "flux_layer_norm");
 }
 
+// Gradients that are recorded (create_graph): what they depend on has an edge to an error, not to nothing.
+struct Once : torch::autograd::Function<Once> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, const Tensor&, const Tensor&, const std::optional<Tensor>&, const torch::autograd::variable_list* grads) { return *grads; }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) { TORCH_CHECK(false, "layer_norm is differentiated once only"); }
+};
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, const NormOf& c) {
         const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
@@ -425,6 +431,14 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const int64_t need = flux_layer_norm_bwd_workspace_bytes(&a);
         const Tensor ws = need ? empty({need}, at::kByte, x) : Tensor();
         check(flux_layer_norm_bwd(&a, need ? ws.data_ptr() : nullptr, need, stream_of(x)), "flux_layer_norm_bwd");
+        if (at::GradMode::is_enabled() && (grads[0].requires_grad() || saved[0].requires_grad() || (w.defined() && w.requires_grad()))) {
+            torch::autograd::variable_list some;
+            for (const Tensor* t : {&dx, &dw, &db})
+                if (t->defined()) some.push_back(*t);
+            some = Once::apply(grads[0], saved[0], given(saved[1]), &some);
+            auto next = some.begin();
+            return {want_x ? *next++ : dx, want_w ? *next++ : dw, want_b ? *next++ : db, Tensor()};
+        }
         return {dx, dw, db, Tensor()};
     }
 };

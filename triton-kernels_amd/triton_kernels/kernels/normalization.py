@@ -225,18 +225,24 @@ class _layer_norm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors   # (what saved-tensor hooks gave back)
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        return (*_layer_norm_grads.apply(dy, x, weight, stats, ctx.groups, ctx.plus_one, ctx.bias_dtype, ctx.needs_input_grad[:3]), None, None, None, None)
+
+
+class _layer_norm_grads(torch.autograd.Function):
+    """Its gradients. A Function, so that what they depend on has an edge to an error where they are recorded (create_graph), not to nothing."""
+
+    @staticmethod
+    def forward(ctx, dy, x, weight, stats, groups, plus_one, bias_dtype, wanted):
+        want_x, want_w, want_b = wanted
         dev = nv.require_gpu(dy, x, weight, stats)
         batch, seq, n = dy.shape
-        groups = ctx.groups
         if x.shape != dy.shape or stats.shape != (2, batch * seq) or (weight is not None and weight.shape != (groups, n)):
             raise RuntimeError("layer_norm: saved tensors came back with other sizes")
         x, dy = _unit_stride(x), _unit_stride(dy if dy.dtype == x.dtype else dy.to(x.dtype))
         stats = stats.float().contiguous()
-        w_dtype = weight.dtype if weight is not None else ctx.bias_dtype or x.dtype
+        w_dtype = weight.dtype if weight is not None else bias_dtype or x.dtype
         if weight is not None:
             weight = _unit_stride(weight)
         dx = torch.empty((batch, seq, n), dtype=x.dtype, device=dev) if want_x else None
@@ -246,13 +252,17 @@ class _layer_norm(torch.autograd.Function):
         if batch * seq:
             a = nv.LayerNormBwdArgs(dy.data_ptr(), x.data_ptr(), nv.ptr(weight), stats[0].data_ptr(), stats[1].data_ptr(), nv.ptr(dx), nv.ptr(dw), nv.ptr(db),
                                     batch, seq, dy.stride(0), dy.stride(1), x.stride(0), x.stride(1), groups, weight.stride(0) if weight is not None else 0,
-                                    n, nv.dtype_code(x), nv._DTYPE_CODE[w_dtype], ctx.plus_one)
+                                    n, nv.dtype_code(x), nv._DTYPE_CODE[w_dtype], plus_one)
             need = nv.lib().flux_layer_norm_bwd_workspace_bytes(nv.byref(a))
             ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
             with nv.on_device(dev):
                 rc = nv.lib().flux_layer_norm_bwd(nv.byref(a), nv.ptr(ws), need, nv.stream_ptr(dev))
             nv.check(rc, "flux_layer_norm_bwd")
-        return dx, dw, db, None, None, None, None
+        return dx, dw, db
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("layer_norm is differentiated once only")
 
 
 def _unit_stride(t: torch.Tensor) -> torch.Tensor:
