@@ -222,3 +222,13 @@ def test_refusals_and_launch_hook():
     finally:
         linear.launch_hook = None
     assert len(seen) == 1 and seen[0]["flops16"] == 2.0 * 24 * (64 * 48 + 8 * (64 + 48)) and "M=24" in seen[0]["name"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,rank", [(4081, 64), (4096, 256), (4700, 33), (4609, 32), (8200, 16), (8225, 72)])
+def test_first_launch_of_large_tiles(M, rank):
+    """Rows enough for tiles of 32, in every count of workgroups: adapters mixed by row, in stretches that end inside a tile, and one for all."""
+    g, x, w, b, lora_a, lora_b, scaling = make(M, (M,), 192, 136, 40, rank)
+    for adapter in (torch.randint(-1, 40, (M,), generator=g), torch.arange(M) // 37 % 41 - 1, torch.randint(0, 40, (), generator=g)):
+        check(x, w, b, lora_a, lora_b, adapter.to(DEV), scaling)
+    check(x[:M // 7 * 7].view(-1, 7, 192), w, b, lora_a, lora_b, torch.randint(-1, 40, (M // 7,), generator=g).to(DEV), scaling)
