@@ -148,8 +148,8 @@ struct LoraTail {
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) bad |= not_finite(s.b[j][e]);
-                if (__ballot(bad != 0) != 0) {
+                    for (int e = 0; e < 4; ++e) bad |= (s.b[j][e] & 0x7f807f80u) + 0x00800080u;   // an exponent of all ones carries into its half's top bit
+                if (__ballot((bad & 0x80008000u) != 0) != 0) {
                     u32x4 huge[FN];
 #pragma unroll
                     for (int j = 0; j < FN; ++j)
