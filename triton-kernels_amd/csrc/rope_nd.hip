@@ -6,6 +6,9 @@
 // thread owns one 16-byte vector of a row (4 pairs of bf16, 2 of fp32) and walks eight heads of its position, so an angle is worked out once for
 // all of them and a row needs no exchange between lanes. In turns (angle / 2 pi, as the frequencies arrive here) an angle of any
 // size loses its whole turns exactly in 64 bits; what is left of a quarter turn goes through the Taylor series of sine and cosine in fp32.
+//
+// 24 + 24 heads of 128 at 32760 positions, bf16: 158 us, 5.1 TB/s, which a large copy reaches too; 16 + 4 heads of 128 at 2 x 1133 positions, fp32: 10.2 us
+// (9.1 at that rate); one position of 24 + 8 heads for four requests 4.4 us and a table of 4608 positions 4.2, launches both.
 #include "common.h"
 #include "../../include/flux_hip_tune.h"
 #include <cmath>

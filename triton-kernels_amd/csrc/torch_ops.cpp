@@ -12,6 +12,8 @@
 // x 3072 15.8 -> 15.1 (the GPU's own time). The calls that the fused blocks are made of are here as well. Host time of a pass: the six of a single-stream
 // block at 320 tokens 135 -> 78 (the GPU 120 there), the nine of a double-stream block at 1024 + 256 tokens 327 -> 160, of two batch elements
 // at 256 + 64 338 -> 155; first passes on new weights 304 -> 214, 586 -> 474 and 546 -> 396.
+// A training step of layer_norm at [1, 4608, 3072] 177 -> 67 and of apply_rope_nd at 2 x 1133 tokens 75 -> 62 (autograd.grad of a product of two
+// tensors takes 34 of either), layer_norm of 77 rows 19.6 -> 5.1, one rotated token 21.9 -> 6.5, linear_lora of six rows 20.8 -> 14.1.
 #include <torch/csrc/python_headers.h>
 #include <ATen/ATen.h>
 #include <torch/csrc/Exceptions.h>
