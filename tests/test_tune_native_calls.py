@@ -279,3 +279,19 @@ def test_calls_from_threads_on_streams_of_their_own():
     for t in threads:
         t.join()
     assert not failed
+
+
+@gpu
+def test_inference_mode_one_row_and_numbers_of_no_adapter(monkeypatch):
+    g = seeded(9)
+    x, w, ids = randn(g, 2, 3, 4, 64, dtype=BF).to(DEV), randn(g, 64, dtype=BF).to(DEV), torch.randint(0, 9, (4, 3), generator=g).to(DEV)
+    weights, la, lb = randn(g, 40, 64, dtype=BF).to(DEV), randn(g, 2, 8, 64, dtype=BF).to(DEV), randn(g, 2, 40, 8, dtype=BF).to(DEV)
+    none = torch.tensor([2 ** 40, -2 ** 63], device=DEV)
+    calls = (lambda: tk.layer_norm(x, w), lambda: tk.layer_norm(x[0, 0, 0], w), lambda: tk.apply_rope_nd(x, None, ids, AXES)[0], lambda: tk.rope_table(ids, AXES),
+             lambda: tk.linear_lora(x, weights, None, la, lb, none), lambda: tk.linear_lora(x[0, 0, 0], weights, None, la, lb, none[0] * 0 + 1))
+    for call in calls:
+        want = call()
+        with torch.inference_mode():
+            assert torch.equal(call(), want)
+        assert torch.equal(launcher(monkeypatch, call), want)
+    assert torch.equal(calls[4](), tk.linear(x, weights, None))

@@ -127,8 +127,9 @@ __global__ __launch_bounds__(kRopeBlock) void rope_nd_kernel(RopeNd<P> p) {
 #pragma unroll
         for (int e = 0; e < VEC; e += 2) {
             const float x0 = Elem<T>::load(in[i][e]), x1 = Elem<T>::load(in[i][e + 1]);
-            out[e] = Elem<T>::store(x0 * c[e / 2] - x1 * s[e / 2]);
-            out[e + 1] = Elem<T>::store(x0 * s[e / 2] + x1 * c[e / 2]);
+            // (which of two products is rounded is not left to the compiler: a token's result does not go with the number of heads a thread walks)
+            out[e] = Elem<T>::store(fmaf(x0, c[e / 2], -(x1 * s[e / 2])));
+            out[e + 1] = Elem<T>::store(fmaf(x0, s[e / 2], x1 * c[e / 2]));
         }
         if constexpr (VEC == 2) {
             y[ay] = out[0];
