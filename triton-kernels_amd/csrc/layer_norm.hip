@@ -385,8 +385,13 @@ __global__ __launch_bounds__(1024) void ln_fold_kernel(const float* part, TD* dw
     const float* const from = part + (static_cast<int64_t>(group) * 2 + which) * parts * n;
     float t = 0.0f;
     if (c < n) {
-#pragma unroll 8
-        for (int i = strip; i < parts; i += 32) t += from[static_cast<int64_t>(i) * n + c];
+        for (int i = strip; i < parts; i += 256) {
+            float v[8];   // (requested at once, also where fewer are left)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = from[static_cast<int64_t>(min(i + j * 32, parts - 1)) * n + c];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t += i + j * 32 < parts ? v[j] : 0.0f;
+        }
     }
     sums[strip][col] = t;
     __syncthreads();
