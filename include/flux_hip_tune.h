@@ -36,7 +36,7 @@ int flux_layer_norm(const flux_layer_norm_fwd_args* args, void* stream);
  *   dx = rstd * (g - mean_n(g) - h * mean_n(g * h)),  dw = sum over the rows of a weight of dy * h,  db = the same of dy.
  * x and dy have strides of their own, dx is contiguous. dw and db are contiguous [groups, n] in w_dtype; each of
  * dx, dw and db may be null. Sums over rows are formed in fp32 in a fixed order, whose parts go through the
- * workspace (flux_layer_norm_bwd_workspace_bytes, 0 where neither dw nor db is wanted; it need not be cleared), and rounded once. */
+ * workspace (flux_layer_norm_bwd_workspace_bytes, 0 for few rows and where neither dw nor db is wanted; it need not be cleared), and rounded once. */
 typedef struct flux_layer_norm_bwd_args {
     const void* dy; const void* x; const void* w; const float* mean; const float* rstd;
     void* dx; void* dw; void* db;

@@ -260,3 +260,16 @@ def test_refusals():
         tk.layer_norm(torch.zeros(1, 65537, device=DEV))
     with pytest.raises(RuntimeError, match="different devices|GPU"):
         tk.layer_norm(x, w.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,tokens,n", [(2, 63, 96), (1, 128, 3000), (1, 129, 512), (4, 128, 4096), (5, 128, 4096), (64, 8, 320), (70, 3, 1001), (1, 2, 16384), (255, 2, 64), (3, 128, 1003), (300, 1, 72)])
+@pytest.mark.parametrize("each", [False, True])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_few_rows_and_many_weights(batch, tokens, n, each, dtype):
+    """Around the bounds of the backward pass in one launch, with any of its outputs left out, and the sums of few parts for many weights."""
+    (x, dy), g = inputs((batch, tokens, n), dtype, n + batch)
+    w, b = (randn(g, *((batch, 1, n) if each else (n,)), dtype=dtype).to(DEV) for _ in range(2))
+    for wanted in ("xwb", "wb", "xw", "b"):
+        check(x, w, b, dy, plus_one=each, wanted=wanted)
+    check(x, None, b, dy)

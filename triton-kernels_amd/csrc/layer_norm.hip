@@ -326,6 +326,84 @@ __global__ __launch_bounds__(kLnMost) void ln_bwd_kernel(LnBwd<T, TW> p) {
     }
 }
 
+// Few rows: dx by the first `dx_blocks` workgroups, dw and db whole by the others, 64 columns each, which read x and dy once more, from the caches.
+// One launch and no workspace.
+template <typename T, typename TW, int VEC, int ITER>
+__global__ __launch_bounds__(kLnMost) void ln_bwd_few_kernel(LnBwd<T, TW> p, TW* dw_out, TW* db_out, int dx_blocks) {
+    __shared__ float box[16][2];
+    __shared__ float fold[2][16][64];
+    const int group = blockIdx.y;
+    if (static_cast<int>(blockIdx.x) < dx_blocks) {
+        const int G = p.T_, grp = threadIdx.x / G, lane = threadIdx.x - grp * G;
+        const int row_raw = blockIdx.x * (blockDim.x / G) + grp, row = min(row_raw, p.rows - 1), all = group * p.rows + row;
+        int b;
+        const T* const xr = p.x + row_offset(all, p.seq, p.x_sb, p.x_sl, b);
+        const T* const dr = p.dy + row_offset(all, p.seq, p.dy_sb, p.dy_sl, b);
+        const TW* const wr = p.w == nullptr ? nullptr : p.w + group * p.w_sb;
+        Pack<T, VEC> x[ITER], dy[ITER];
+        Pack<TW, VEC> w[ITER] = {};
+        int at[ITER];
+        bool in[ITER];
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+            const int c = (it * G + lane) * VEC;
+            in[it] = c < p.n;
+            at[it] = in[it] ? c : 0;
+            x[it] = ld_pack<T, VEC>(xr + at[it]);
+            dy[it] = ld_pack<T, VEC>(dr + at[it]);
+            if (wr != nullptr) w[it] = ld_pack<TW, VEC>(wr + at[it]);
+        }
+        const float mean = p.mean[all], rstd = p.rstd[all], inv = 1.0f / static_cast<float>(p.n);
+        auto scaled = [&](int it, int e) { return wr != nullptr ? dy[it].at(e) * (p.one + w[it].at(e)) : dy[it].at(e); };
+        float a = 0.0f, c = 0.0f;
+#pragma unroll
+        for (int it = 0; it < ITER; ++it)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float g = scaled(it, e);
+                a += in[it] ? g : 0.0f;
+                c += in[it] ? g * ((x[it].at(e) - mean) * rstd) : 0.0f;
+            }
+        row_sums(a, c, G, box);
+        a *= inv;
+        c *= inv;
+        if (row_raw >= p.rows) return;
+        T* const dxr = p.dx + static_cast<int64_t>(all) * p.n;
+#pragma unroll
+        for (int it = 0; it < ITER; ++it)
+            if (in[it]) st_pack<T, VEC>(dxr + at[it], [&](int e) { return rstd * (scaled(it, e) - (a + (x[it].at(e) - mean) * rstd * c)); });
+        return;
+    }
+    const int lane = threadIdx.x & 63, strip = threadIdx.x >> 6, strips = blockDim.x >> 6;
+    const int col = (blockIdx.x - dx_blocks) * 64 + lane, c = min(col, p.n - 1);
+    float dw = 0.0f, db = 0.0f;
+    for (int row = strip; row < p.rows; row += strips * 8) {
+        float d[8], h[8];   // (requested at once, also where fewer are left)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int all = group * p.rows + min(row + i * strips, p.rows - 1);
+            int b;
+            d[i] = Elem<T>::load(p.dy[row_offset(all, p.seq, p.dy_sb, p.dy_sl, b) + c]);
+            h[i] = (Elem<T>::load(p.x[row_offset(all, p.seq, p.x_sb, p.x_sl, b) + c]) - p.mean[all]) * p.rstd[all];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool ok = row + i * strips < p.rows;
+            dw += ok ? d[i] * h[i] : 0.0f;
+            db += ok ? d[i] : 0.0f;
+        }
+    }
+    fold[0][strip][lane] = dw;
+    fold[1][strip][lane] = db;
+    __syncthreads();
+    TW* const out = strip == 0 ? dw_out : db_out;
+    if (strip < 2 && col < p.n && out != nullptr) {
+        float t = 0.0f;
+        for (int i = 0; i < strips; ++i) t += fold[strip][i][lane];
+        out[static_cast<int64_t>(group) * p.n + col] = Elem<TW>::store(t);
+    }
+}
+
 // Rows of any length: dx, a workgroup per row.
 template <typename T, typename TW>
 __global__ __launch_bounds__(kLnMost) void ln_bwd_wide_dx_kernel(LnBwd<T, TW> p) {
@@ -375,30 +453,29 @@ __global__ __launch_bounds__(kLnMost) void ln_bwd_wide_sums_kernel(LnBwd<T, TW> 
     }
 }
 
-// dw[group] and db[group] = the sums of their parts in order, rounded once. A workgroup takes 32 columns with 32 threads each.
+// dw[group] and db[group] = the sums of their parts in order, rounded once. A workgroup takes 1024 / strips columns with `strips` threads each.
 template <typename TD>
-__global__ __launch_bounds__(1024) void ln_fold_kernel(const float* part, TD* dw, TD* db, int parts, int n) {
-    __shared__ float sums[32][33];
-    const int col = threadIdx.x & 31, strip = threadIdx.x >> 5, c = blockIdx.x * 32 + col, which = blockIdx.y, group = blockIdx.z;
+__global__ __launch_bounds__(1024) void ln_fold_kernel(const float* part, TD* dw, TD* db, int parts, int n, int strips) {
+    __shared__ float sums[1024 + 32];
+    const int cols = 1024 / strips, strip = threadIdx.x / cols, col = threadIdx.x - strip * cols, c = blockIdx.x * cols + col, which = blockIdx.y, group = blockIdx.z;
     TD* const out = which == 0 ? dw : db;
     if (out == nullptr) return;
     const float* const from = part + (static_cast<int64_t>(group) * 2 + which) * parts * n;
     float t = 0.0f;
     if (c < n) {
-        for (int i = strip; i < parts; i += 256) {
+        for (int i = strip; i < parts; i += strips * 8) {
             float v[8];   // (requested at once, also where fewer are left)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = from[static_cast<int64_t>(min(i + j * 32, parts - 1)) * n + c];
+            for (int j = 0; j < 8; ++j) v[j] = from[static_cast<int64_t>(min(i + j * strips, parts - 1)) * n + c];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t += i + j * 32 < parts ? v[j] : 0.0f;
+            for (int j = 0; j < 8; ++j) t += i + j * strips < parts ? v[j] : 0.0f;
         }
     }
-    sums[strip][col] = t;
+    sums[strip * (cols + 1) + col] = t;
     __syncthreads();
     if (strip == 0 && c < n) {
         float total = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) total += sums[i][col];
+        for (int i = 0; i < strips; ++i) total += sums[i * (cols + 1) + col];
         out[static_cast<int64_t>(group) * n + c] = Elem<TD>::store(total);
     }
 }
@@ -473,7 +550,7 @@ static int ln_fwd_launch(const flux_layer_norm_fwd_args& a, hipStream_t st) {
 }
 
 // How the backward pass is cut: `blocks` workgroups of `threads` a weight group, each with a part of dw and db.
-struct LnBwdPlan { LnPlan row; int threads, blocks; };
+struct LnBwdPlan { LnPlan row; int threads, blocks; bool few; };
 
 static LnBwdPlan ln_bwd_plan(const flux_layer_norm_bwd_args& a) {
     const int vec = a.x_dtype == FLUX_BF16 ? 8 : 4;
@@ -483,6 +560,7 @@ static LnBwdPlan ln_bwd_plan(const flux_layer_norm_bwd_args& a) {
     // x and dy of two rows and two sums a column: 16 columns of bf16 or 12 of fp32 a lane are what the 128 registers of 16 waves a CU hold
     static const int iters[] = {1, 2, 3, 4, 8};
     LnBwdPlan p;
+    p.few = false;
     p.row = ln_plan(a.n, wide ? vec : 1, iters, wide ? (vec == 8 ? 2 : 3) : 5);
     const int64_t most = std::max<int64_t>(1, 256 / a.groups);   // workgroups a weight group
     if (p.row.T == 0) {
@@ -496,6 +574,16 @@ static LnBwdPlan ln_bwd_plan(const flux_layer_norm_bwd_args& a) {
     while (per_block > 1 && per_block * p.row.T > 256 && (rows + per_block - 1) / per_block < most) per_block /= 2;  
     p.threads = per_block * p.row.T;
     p.blocks = static_cast<int>(std::min<int64_t>((rows + per_block - 1) / per_block, most));
+    // Up to 128 rows the waves of a workgroup request all of a column's values at once, and with no more such workgroups than CUs that is quicker. us of
+    // the kernels, one launch and two: 77 x 768 5.2 and 9.3, 128 x 3072 6.8 and 13.5 (bf16), 256 x 1024 8.2 and 9.6, 512 x 768 13.6 and 9.7; with a
+    // weight each 3 x 128 x 3072 7.3 and 17.0, 8 x 128 x 2048 8.9 and 12.6, 32 x 64 x 1024 11.6 and 9.7. And 3 us less of the host's time (27 -> 24, or
+    // 49 -> 45 where the engine's thread is slow).
+    p.few = (a.dw != nullptr || a.db != nullptr) && rows <= 128 && (a.n + 63) / 64 * a.groups <= 256;
+    if (p.few) {
+        per_block = kLnMost / p.row.T;
+        p.threads = per_block * p.row.T;
+        p.blocks = static_cast<int>((rows + per_block - 1) / per_block);
+    }
     return p;
 }
 
@@ -517,8 +605,11 @@ static int ln_bwd_launch(const flux_layer_norm_bwd_args& a, float* ws, hipStream
         if (sums) hipLaunchKernelGGL((ln_bwd_wide_sums_kernel<T, TW>), dim3((unsigned)((a.n + 63) / 64), (unsigned)plan.blocks, (unsigned)a.groups), dim3(kLnMost), 0, st, p);
     } else {
         const dim3 grid((unsigned)plan.blocks, (unsigned)a.groups), threads(plan.threads);
+        const int dx_blocks = a.dx != nullptr ? plan.blocks : 0;
+        const dim3 both((unsigned)(dx_blocks + (a.n + 63) / 64), (unsigned)a.groups);
 #define CALL(V, I)                                                                                                                               \
-    if (V == 1 || plan.row.T * I * V != a.n) hipLaunchKernelGGL((ln_bwd_kernel<T, TW, V, I, false, false>), grid, threads, 0, st, p);            \
+    if (plan.few) hipLaunchKernelGGL((ln_bwd_few_kernel<T, TW, V, I>), both, threads, 0, st, p, static_cast<TW*>(a.dw), static_cast<TW*>(a.db), dx_blocks); \
+    else if (V == 1 || plan.row.T * I * V != a.n) hipLaunchKernelGGL((ln_bwd_kernel<T, TW, V, I, false, false>), grid, threads, 0, st, p);            \
     else if (once) hipLaunchKernelGGL((ln_bwd_kernel<T, TW, V, I, (V > 1), (V > 1)>), grid, threads, 0, st, p);                                  \
     else hipLaunchKernelGGL((ln_bwd_kernel<T, TW, V, I, (V > 1), false>), grid, threads, 0, st, p)
         if (plan.row.vec == 1) {
@@ -535,15 +626,18 @@ static int ln_bwd_launch(const flux_layer_norm_bwd_args& a, float* ws, hipStream
                 case 1: CALL(V, 1); break;
                 case 2: CALL(V, 2); break;
                 default:
-                    if constexpr (V == 4) CALL(V, 3);
+                    if constexpr (V == 4) { CALL(V, 3); }
                     break;
             }
         }
 #undef CALL
     }
-    if (sums) {
-        const dim3 grid((unsigned)((a.n + 31) / 32), 2, (unsigned)a.groups);
-        hipLaunchKernelGGL((ln_fold_kernel<TW>), grid, dim3(1024), 0, st, ws, static_cast<TW*>(a.dw), static_cast<TW*>(a.db), plan.blocks, a.n);
+    if (sums && !plan.few) {
+        int strips = 1;   // eight parts a thread
+        while (strips < 32 && strips * 8 < plan.blocks) strips *= 2;
+        const int cols = 1024 / strips;
+        const dim3 grid((unsigned)((a.n + cols - 1) / cols), 2, (unsigned)a.groups);
+        hipLaunchKernelGGL((ln_fold_kernel<TW>), grid, dim3(1024), 0, st, ws, static_cast<TW*>(a.dw), static_cast<TW*>(a.db), plan.blocks, a.n, strips);
     }
     return check_launch("flux_layer_norm_bwd");
 }
@@ -593,7 +687,8 @@ extern "C" int flux_layer_norm(const flux_layer_norm_fwd_args* a, void* stream) 
 
 extern "C" int64_t flux_layer_norm_bwd_workspace_bytes(const flux_layer_norm_bwd_args* a) {
     if (!a || (!a->dw && !a->db) || ln_shape("flux_layer_norm_bwd", a->batch, a->seq, a->groups, a->n) != FLUX_OK || a->batch * a->seq == 0) return 0;
-    return static_cast<int64_t>(sizeof(float)) * 2 * a->groups * ln_bwd_plan(*a).blocks * a->n;
+    const LnBwdPlan plan = ln_bwd_plan(*a);
+    return plan.few ? 0 : static_cast<int64_t>(sizeof(float)) * 2 * a->groups * plan.blocks * a->n;
 }
 
 extern "C" int flux_layer_norm_bwd(const flux_layer_norm_bwd_args* a, void* ws, int64_t ws_bytes, void* stream) {
