@@ -57,7 +57,7 @@ def test_layer_norm_refusals(change, rc):
     assert nv.lib().flux_layer_norm(None, None) == -1
 
 
-@pytest.mark.parametrize("change,ws,rc", [(dict(dy=None), 1 << 20, -1), (dict(mean=None), 1 << 20, -1), (dict(groups=3), 1 << 20, -2), (dict(), 0, -1), (dict(n=70000), 1 << 20, -5),
+@pytest.mark.parametrize("change,ws,rc", [(dict(dy=None), 1 << 20, -1), (dict(mean=None), 1 << 20, -1), (dict(groups=3), 1 << 20, -2), (dict(seq=300), 0, -1), (dict(n=70000), 1 << 20, -5),
                                           (dict(x_dtype=1), 1 << 20, -3), (dict(dx=None, dw=None, db=None), 0, 0), (dict(batch=0), 1 << 20, -2), (dict(batch=0, dw=None, db=None), 0, 0)])
 def test_layer_norm_bwd_refusals(change, ws, rc):
     a = nv.LayerNormBwdArgs(**{**dict(dy=P, x=P, w=P, mean=P, rstd=P, dx=P, dw=P, db=P, batch=2, seq=3, dy_sb=24, dy_sl=8, x_sb=24, x_sl=8, groups=1, n=8, x_dtype=0, w_dtype=0), **change})
@@ -70,7 +70,9 @@ def test_layer_norm_bwd_workspace():
     assert need > 0 and need % (2 * 4 * 8 * 4) == 0
     assert nv.lib().flux_layer_norm_bwd(ctypes.byref(a), P, need - 1, None) == -2      # too small
     assert nv.lib().flux_layer_norm_bwd(ctypes.byref(a), P + 2, need, None) == -1      # not aligned
-    a.dw = a.db = None
+    a.seq = 128                                                                        # few rows: one launch, without parts
+    assert nv.lib().flux_layer_norm_bwd_workspace_bytes(ctypes.byref(a)) == 0
+    a.seq, a.dw, a.db = 1000, None, None
     assert nv.lib().flux_layer_norm_bwd_workspace_bytes(ctypes.byref(a)) == 0
 
 
