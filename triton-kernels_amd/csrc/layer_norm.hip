@@ -7,9 +7,9 @@
 // a DPP butterfly inside a wave and one exchange through LDS between the waves of a longer row. Rows that are not 16-byte
 // addressable are held the same way, an element at a time (VEC = 1). Only rows beyond 1024 lanes are read again, from the caches.
 //
-// us of the kernels alone (bytes at 5.1 TB/s, a large copy's rate): [4608, 3072] bf16 forward 12.8 (11.1), backward 24.7 (16.6) and 4.0 for the sums of
-// the parts; [3, 4336, 3072] bf16 with a weight for each batch element 30.9 (31.2), 56.5 (46.8) and 4.7; [4004, 1024] fp32 8.8 (6.4), 13.2 (9.6)
-// and 3.2; 77 rows of 768 3.5, a launch.
+// us of the kernels alone (bytes at 5.1 TB/s, a large copy's rate): [4608, 3072] bf16 forward 12.8 (11.1), backward 24.6 (16.6) and 4.0 for the sums of
+// the parts; [3, 4336, 3072] bf16 with a weight for each batch element 31.2 (31.2), 55.6 (46.8) and 4.0; [4004, 1024] fp32 8.8 (6.4), 13.2 (9.6)
+// and 3.8; 77 rows of 768 3.5, a launch, and 5.2.
 #include "common.h"
 #include "../../include/flux_hip_tune.h"
 #include <algorithm>
