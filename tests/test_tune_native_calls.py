@@ -295,3 +295,28 @@ def test_inference_mode_one_row_and_numbers_of_no_adapter(monkeypatch):
             assert torch.equal(call(), want)
         assert torch.equal(launcher(monkeypatch, call), want)
     assert torch.equal(calls[4](), tk.linear(x, weights, None))
+
+
+@gpu
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_under_activation_checkpoints(monkeypatch, reentrant):
+    from torch.utils.checkpoint import checkpoint
+
+    g = seeded(10)
+    x, w = randn(g, 2, 6, 64, dtype=BF).to(DEV).requires_grad_(True), randn(g, 64, dtype=BF).to(DEV).requires_grad_(True)
+    ids = torch.randint(0, 9, (6, 3), generator=g).to(DEV)
+
+    def block(x, w):
+        q, k = tk.apply_rope_nd(tk.layer_norm(x, w, w).unsqueeze(1), tk.layer_norm(x, None, w).unsqueeze(1), ids, AXES)
+        return (q * k).float().sum()
+
+    def both():
+        grads = []
+        for y in (block(x, w), checkpoint(block, x, w, use_reentrant=reentrant)):
+            x.grad = w.grad = None
+            y.backward()
+            grads.append((x.grad, w.grad))
+        same(*grads)
+
+    both()
+    launcher(monkeypatch, both)
