@@ -588,8 +588,7 @@ static LnBwdPlan ln_bwd_plan(const flux_layer_norm_bwd_args& a) {
 }
 
 template <typename T, typename TW>
-static int ln_bwd_launch(const flux_layer_norm_bwd_args& a, float* ws, hipStream_t st) {
-    const LnBwdPlan plan = ln_bwd_plan(a);
+static int ln_bwd_launch(const flux_layer_norm_bwd_args& a, const LnBwdPlan& plan, float* ws, hipStream_t st) {
     const int64_t rows = a.groups > 1 ? a.seq : a.batch * a.seq;
     const bool sums = a.dw != nullptr || a.db != nullptr;
     LnBwd<T, TW> p = {static_cast<const T*>(a.dy), static_cast<const T*>(a.x), static_cast<const TW*>(a.w), a.mean, a.rstd, static_cast<T*>(a.dx), sums ? ws : nullptr,
@@ -642,11 +641,29 @@ static int ln_bwd_launch(const flux_layer_norm_bwd_args& a, float* ws, hipStream
     return check_launch("flux_layer_norm_bwd");
 }
 
-// One row a batch element and a weight for all rows: the rows are what is evenly strided.
-static void ln_rows_of(int64_t& batch, int64_t& seq, int64_t groups, std::initializer_list<std::pair<int64_t*, int64_t*>> strides) {
-    if (groups != 1 || seq != 1) return;
-    std::swap(batch, seq);
-    for (const auto& s : strides) *s.second = *s.first;
+// One row a batch element and a weight for all rows: the rows are what is evenly strided. Strides that nothing reads become those of contiguous
+// rows: plans look at all of them.
+static void ln_rows_of(int64_t& batch, int64_t& seq, int64_t groups, int32_t n, std::initializer_list<std::pair<int64_t*, int64_t*>> strides, std::initializer_list<int64_t*> weights) {
+    const bool rows = groups == 1 && seq == 1;
+    if (rows) std::swap(batch, seq);
+    for (const auto& s : strides) {
+        if (rows) *s.second = *s.first;
+        if (seq == 1) *s.second = n;
+        if (batch == 1) *s.first = seq * *s.second;
+    }
+    for (int64_t* w : weights)
+        if (groups == 1) *w = 0;
+}
+
+// The backward pass's arguments as its plan and its launch take them, both from here.
+static flux_layer_norm_bwd_args ln_bwd_rows(const flux_layer_norm_bwd_args& a) {
+    flux_layer_norm_bwd_args r = a;
+    ln_rows_of(r.batch, r.seq, r.groups, r.n, {{&r.x_sb, &r.x_sl}, {&r.dy_sb, &r.dy_sl}}, {&r.w_sb});
+    return r;
+}
+
+static int64_t ln_bwd_bytes(const flux_layer_norm_bwd_args& a, const LnBwdPlan& plan) {
+    return plan.few || (!a.dw && !a.db) ? 0 : static_cast<int64_t>(sizeof(float)) * 2 * a.groups * plan.blocks * a.n;
 }
 
 static int ln_shape(const char* what, int64_t batch, int64_t seq, int64_t groups, int32_t n) {
@@ -679,7 +696,7 @@ extern "C" int flux_layer_norm(const flux_layer_norm_fwd_args* a, void* stream) 
     if ((a->mean == nullptr) != (a->rstd == nullptr)) return fail(FLUX_E_NULL, "flux_layer_norm: mean and rstd go together");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     flux_layer_norm_fwd_args rows = *a;
-    ln_rows_of(rows.batch, rows.seq, rows.groups, {{&rows.x_sb, &rows.x_sl}});
+    ln_rows_of(rows.batch, rows.seq, rows.groups, rows.n, {{&rows.x_sb, &rows.x_sl}}, {&rows.w_sb, &rows.b_sb});
 #define ARGS (rows, st)
     BY_TYPES("flux_layer_norm", ln_fwd_launch);
 #undef ARGS
@@ -687,8 +704,8 @@ extern "C" int flux_layer_norm(const flux_layer_norm_fwd_args* a, void* stream) 
 
 extern "C" int64_t flux_layer_norm_bwd_workspace_bytes(const flux_layer_norm_bwd_args* a) {
     if (!a || (!a->dw && !a->db) || ln_shape("flux_layer_norm_bwd", a->batch, a->seq, a->groups, a->n) != FLUX_OK || a->batch * a->seq == 0) return 0;
-    const LnBwdPlan plan = ln_bwd_plan(*a);
-    return plan.few ? 0 : static_cast<int64_t>(sizeof(float)) * 2 * a->groups * plan.blocks * a->n;
+    const flux_layer_norm_bwd_args by_row = ln_bwd_rows(*a);
+    return ln_bwd_bytes(by_row, ln_bwd_plan(by_row));
 }
 
 extern "C" int flux_layer_norm_bwd(const flux_layer_norm_bwd_args* a, void* ws, int64_t ws_bytes, void* stream) {
@@ -698,13 +715,13 @@ extern "C" int flux_layer_norm_bwd(const flux_layer_norm_bwd_args* a, void* ws, 
     if (!a->dx && !a->dw && !a->db) return FLUX_OK;
     if (a->batch * a->seq == 0) return a->dw || a->db ? fail(FLUX_E_SHAPE, "flux_layer_norm_bwd: no rows to sum over") : FLUX_OK;
     if (!a->x || !a->dy || !a->mean || !a->rstd) return fail(FLUX_E_NULL, "flux_layer_norm_bwd: null pointer");
-    const int64_t need = flux_layer_norm_bwd_workspace_bytes(a);
+    const flux_layer_norm_bwd_args by_row = ln_bwd_rows(*a);
+    const LnBwdPlan plan = ln_bwd_plan(by_row);
+    const int64_t need = ln_bwd_bytes(by_row, plan);
     if (need > 0 && (!ws || reinterpret_cast<uintptr_t>(ws) % 4 != 0)) return fail(FLUX_E_NULL, "flux_layer_norm_bwd: the workspace must be 4-byte aligned memory");
     if (ws_bytes < need) return fail(FLUX_E_SHAPE, "flux_layer_norm_bwd: workspace of %lld bytes is too small", (long long)ws_bytes);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    flux_layer_norm_bwd_args by_row = *a;
-    ln_rows_of(by_row.batch, by_row.seq, by_row.groups, {{&by_row.x_sb, &by_row.x_sl}, {&by_row.dy_sb, &by_row.dy_sl}});
-#define ARGS (by_row, static_cast<float*>(ws), st)
+#define ARGS (by_row, plan, static_cast<float*>(ws), st)
     BY_TYPES("flux_layer_norm_bwd", ln_bwd_launch);
 #undef ARGS
 }
