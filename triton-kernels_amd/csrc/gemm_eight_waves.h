@@ -126,8 +126,9 @@ __device__ __forceinline__ void gemm_pair_slabs(const GemmParams& p, char* lds, 
 }
 
 // A workgroup's tile, or its part of one. `tail` adds to the sums of a wave's fragment rows before their epilogue (finish) and may ask for what that
-// takes in front of the first slabs (begin) and behind them (touch). NoTail: nothing.
+// takes in front of the first slabs (begin) and behind them (touch). lane(): the lane's number behind finish. NoTail: nothing.
 struct NoTail {
+    static __device__ __forceinline__ int lane(int known) { return known; }
     template <int ROWS, int FN> struct Ahead {};
     template <int ROWS, int FN> __device__ __forceinline__ void begin(Ahead<ROWS, FN>&, int, const GemmParams&) const {}
     template <int ROWS, int FN> __device__ __forceinline__ void touch(Ahead<ROWS, FN>&, int, int, const GemmParams&) const {}
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(kPairThreads) void gemm_nt_pair_kernel(GemmLaunch L
         } else {
             tail.finish(own, have, wm0 + OWN0 * 16, wn0, p);
             __syncthreads();                   // the exchange has been read: its LDS is the epilogue's now
-            gemm_finish_rect<FM, FN, OWN, FN != 8>(p, own, lds + G * (ST * (BM + BN) * BK), m0, n0, OWN0, w4, lane);
+            gemm_finish_rect<FM, FN, OWN, FN != 8>(p, own, lds + G * (ST * (BM + BN) * BK), m0, n0, OWN0, w4, tail.lane(lane));
         }
     };
     f32x4 acc[FM][FN];

@@ -26,10 +26,10 @@ struct LoraTail {
     int vec;               // rows of b may be read so many values at a time: 8, 4 or 1
 
     // Adds to the fragment rows of a wave: rows m0 .. of the product, columns n0 ... The adapters among the wave's rows are taken one after the
-    // other in rising order, each with one read of its columns of b; rows of another adapter count as zeros. 0 * inf would still reach them, so
-    // where a wave's rows are not of one adapter, what is not finite in b is taken out and makes its own rows NaN by itself: products of 3e38
-    // and 3e38 and of 3e38 and -3e38, which are zero for all other rows. (The sums are touched by matrix instructions only: choosing
-    // between old and new sums by row, with vector instructions, spilled 600 registers of the 256-wide tile.)
+    // other in rising order, each with one read of its columns of b; rows of another adapter count as zeros, and so do values past the rank's end. 0 * inf
+    // would still reach them, so what is not finite in b is taken out of the product and reaches its own rows by itself (not_finite_terms). (The sums are
+    // touched by matrix instructions only: choosing between old and new sums by row, with vector instructions, spilled 600 registers of the
+    // 256-wide tile.)
     // A step's operands: columns of b of one adapter and the rows' low, 32 values each.
     template <int ROWS, int FN>
     struct Step {
@@ -38,7 +38,7 @@ struct LoraTail {
     template <int ROWS, int FN>
     __device__ __forceinline__ void load(Step<ROWS, FN>& to, int a, int k, int m0, int n0, const GemmParams& p) const {
         // Scalar bases and 32-bit offsets: sixteen pointers would not fit the registers. Past the rank's end: values of the same row of b
-        // again. They meet zeros of low, and where they are not finite, neither is the result.
+        // again, which meet zeros of low.
         const int frow = threadIdx.x & 15, at = k + ((threadIdx.x & 63) >> 4) * 8;
         const bf16_t* const col = b + static_cast<int64_t>(a) * p.N * rank;
         const bf16_t* const row = low + static_cast<int64_t>(m0) * width;
@@ -138,37 +138,20 @@ struct LoraTail {
         for (int k = 0;;) {
             load(s, a, k, m0, n0, p);
             __builtin_amdgcn_sched_barrier(0);   // the loads stay in front of the products
-            auto multiply = [&](const u32x4 (&w)[FN], auto x) {
-#pragma unroll
-                for (int i = 0; i < ROWS; ++i) {
-                    const bf16x8 xi = __builtin_bit_cast(bf16x8, x(i));
-#pragma unroll
-                    for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[j]), xi, acc[i][j], 0, 0, 0);
-                }
-            };
             if (!all) {
 #pragma unroll
                 for (int i = 0; i < ROWS; ++i) s.low[i] = own[i] == a ? s.low[i] : u32x4{0, 0, 0, 0};
-                uint32_t bad = 0;
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) bad |= (s.b[j][e] & 0x7f807f80u) + 0x00800080u;   // an exponent of all ones carries into its half's top bit
-                if (__ballot((bad & 0x80008000u) != 0) != 0) {
-                    u32x4 huge[FN];
-#pragma unroll
-                    for (int j = 0; j < FN; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t n = not_finite(s.b[j][e]);
-                            huge[j][e] = n & 0x7f7f7f7fu;
-                            s.b[j][e] &= ~n;
-                        }
-                    multiply(huge, [&](int i) { const uint32_t h = own[i] == a ? 0x7f7f7f7fu : 0u; return u32x4{h, h, h, h}; });
-                    multiply(huge, [&](int i) { const uint32_t h = own[i] == a ? 0xff7fff7fu : 0u; return u32x4{h, h, h, h}; });
-                }
             }
-            multiply(s.b, [&](int i) { return s.low[i]; });
+            uint32_t bad = 0;
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= not_finite(s.b[j][e]);
+            if (__ballot((bad & 0x80008000u) != 0) != 0) not_finite_terms(acc, s, own, a, k);
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, s.b[j]), __builtin_bit_cast(bf16x8, s.low[i]), acc[i][j], 0, 0, 0);
             k += 32;
             if (k >= width) {
                 k = 0;
@@ -178,9 +161,58 @@ struct LoraTail {
         }
     }
 
-    // All ones in the halves of a word that are infinite or NaN.
-    static __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-        return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+    // Of the halves of a word, in their top bits: infinite or NaN, mantissa not zero, value not zero; and all ones where the top bit is set.
+    static __device__ __forceinline__ uint32_t not_finite(uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; }
+    static __device__ __forceinline__ uint32_t fraction(uint32_t w) { return ((w & 0x007f007fu) + 0x007f007fu) << 8; }
+    static __device__ __forceinline__ uint32_t not_zero(uint32_t w) { return (w & 0x7fff7fffu) + 0x7fff7fffu; }
+    static __device__ __forceinline__ uint32_t filled(uint32_t top) {
+        top &= 0x80008000u;
+        return (top << 1) - (top >> 15);
+    }
+
+    // The lane's number, worked out anew: a register that is live across the loop over K is one too many in the 192 x 192 tile.
+    static __device__ __forceinline__ int lane_again() { return static_cast<int>(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u))); }
+    static __device__ __forceinline__ int lane(int) { return lane_again(); }
+
+    // What is not finite in a step's columns of b, for the rows of adapter a, as low * b would have it: +inf and -inf by the signs, NaN where b is NaN or
+    // low is zero. Both factors become 3.4e38 of their signs, whose product is infinite, and zero everywhere else; one combination of signs at a
+    // time, so that terms of one instruction do not cancel before they are rounded, and NaN and zero are of either sign: +inf - inf. b itself is left with 1 of its sign
+    // (which keeps an infinite or NaN low what it is).
+    template <int ROWS, int FN>
+    __device__ __forceinline__ void not_finite_terms(f32x4 (&acc)[ROWS][FN], Step<ROWS, FN>& s, const int (&own)[ROWS], int a, int k) const {
+        const int at = k + (lane_again() >> 4) * 8;
+#pragma unroll 1
+        for (int signs = 0; signs < 4; ++signs) {
+            // (the words count as new ones in every turn: what is worked out from them is not kept in registers over the turns)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(s.b[j]));
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) asm volatile("" : "+v"(s.low[i]));
+            const uint32_t sign_b = (signs & 1) ? 0x80008000u : 0u, sign_low = (signs & 2) ? 0x80008000u : 0u;
+            u32x4 x[ROWS];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t in = (at + 2 * e < rank ? 0x7f7fu : 0u) | (at + 2 * e + 1 < rank ? 0x7f7f0000u : 0u), with_sign = in | ((in << 1) & sign_low);
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) x[i][e] = own[i] == a ? filled((s.low[i][e] ^ ~sign_low) | ~not_zero(s.low[i][e])) & with_sign : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                u32x4 huge;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) huge[e] = filled(not_finite(s.b[j][e]) & ((s.b[j][e] ^ ~sign_b) | fraction(s.b[j][e]))) & (0x7f7f7f7fu | sign_b);
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, huge), __builtin_bit_cast(bf16x8, x[i]), acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);   // (a column at a time)
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t w = s.b[j][e], n = filled(not_finite(w));
+                s.b[j][e] = (w & (~n | 0x80008000u)) | (n & 0x3f803f80u);
+            }
     }
 
     // The smallest value of the wave's 16 rows (lanes 16 apart hold the same row), as a scalar.

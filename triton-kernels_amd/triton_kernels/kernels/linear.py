@@ -289,7 +289,7 @@ def linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, lora_b: 
     scaling : fp32 [adapters], or None for 1
 
     Like linear it is not differentiated. x lora_a[i]^T is rounded to bf16, the sum of both products only as the result. What is not
-    finite in an adapter does not reach other requests' rows.
+    finite in an adapter does not reach other requests' rows, and its own rows as the formula has it, whatever else is in the call.
     """
     known = _ACTIVATIONS.get(activation)
     if known is not None and launch_hook is None and not is_compiling():
