@@ -599,7 +599,8 @@ struct LoraCall {
     LinearRoute route;
     int64_t low_bytes, owner_bytes;   // of the workspace, in this order; the parts of K behind them
 };
-static int read_lora_args(const flux_linear_lora_args* a, LoraCall& c) {
+// workspace_bytes: what there is of it; beyond rank 16 it may have no room for the second numbers of x a^T (LoraPlace).
+static int read_lora_args(const flux_linear_lora_args* a, int64_t workspace_bytes, LoraCall& c) {
     if (!a) return fail(FLUX_E_NULL, "flux_linear_lora_bf16: null args");
     flux_linear_args l = {};
     l.A = a->x; l.W = a->w; l.bias = a->bias; l.Y = a->y;
@@ -617,37 +618,39 @@ static int read_lora_args(const flux_linear_lora_args* a, LoraCall& c) {
     if (a->N * a->rank >= (int64_t{1} << 30)) return fail(FLUX_E_SHAPE, "flux_linear_lora_bf16: adapters of 2^30 values in lora_b and more");   // 32-bit offsets
     if (a->M > (int64_t{1} << 27)) return fail(FLUX_E_SHAPE, "flux_linear_lora_bf16: too many rows");
     if (c.route == kScalar && a->N >= ((int64_t{1} << 32) - 256) / a->M) return fail(FLUX_E_SHAPE, "flux_linear_lora_bf16: more than 2^32 results of operands that are not 16-byte addressable");
-    const int width = (a->rank + 31) / 32 * 32;
-    c.low_bytes = (a->M * width * 2 + 255) / 256 * 256;
-    c.owner_bytes = (a->M * 4 + 255) / 256 * 256;
-    c.tail = {nullptr, nullptr, static_cast<const bf16_t*>(a->lora_b), a->rank, width,
+    const auto whole = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
+    LoraPlace at = {a->rank, (a->rank + 31) / 32 * 32, c.route != kTiles ? 0 : a->rank > 16 ? 2 : 1};
+    c.owner_bytes = whole(a->M * 4);
+    if (at.planes == 2 && whole(at.bytes(a->M)) + c.owner_bytes > workspace_bytes) at.planes = 1;
+    c.low_bytes = whole(at.bytes(a->M));
+    c.tail = {nullptr, nullptr, static_cast<const bf16_t*>(a->lora_b), at,
               a->rank % 8 == 0 && aligned16(a->lora_b) ? 8 : a->rank % 4 == 0 && (reinterpret_cast<uintptr_t>(a->lora_b) & 7u) == 0 ? 4 : 1};
-    c.low = {static_cast<const bf16_t*>(a->x), static_cast<const bf16_t*>(a->lora_a), a->adapter, a->scaling, nullptr, nullptr, a->ldx, a->M / a->requests,
-             static_cast<int>(a->M), static_cast<int>(a->K), a->rank, width, a->adapters, a->wide_ids != 0, a->K % 8 == 0 && a->ldx % 8 == 0 && aligned16(a->x) && aligned16(a->lora_a) && a->ldx * 2 * 32 < 0x7fffffffLL && a->K * 2 * 64 < 0x7fffffffLL};
+    c.low = {static_cast<const bf16_t*>(a->x), static_cast<const bf16_t*>(a->lora_a), a->adapter, a->scaling, nullptr, nullptr, at, a->ldx, a->M / a->requests,
+             static_cast<int>(a->M), static_cast<int>(a->K), a->adapters, a->wide_ids != 0, a->K % 8 == 0 && a->ldx % 8 == 0 && aligned16(a->x) && aligned16(a->lora_a) && a->ldx * 2 * 32 < 0x7fffffffLL && a->K * 2 * 64 < 0x7fffffffLL};
     return FLUX_OK;
 }
 
 extern "C" int64_t flux_linear_lora_least_bytes(const flux_linear_lora_args* a) {
     LoraCall c;
-    return read_lora_args(a, c) == FLUX_OK ? c.low_bytes + c.owner_bytes : 0;
+    return read_lora_args(a, 0, c) == FLUX_OK ? c.low_bytes + c.owner_bytes : 0;
 }
 
 extern "C" int64_t flux_linear_lora_workspace_bytes(const flux_linear_lora_args* a) {
     LoraCall c;
     int64_t parts = 0;
-    if (read_lora_args(a, c) != FLUX_OK || c.route == kNothing) return 0;
+    if (read_lora_args(a, INT64_MAX, c) != FLUX_OK || c.route == kNothing) return 0;
     if (c.route == kTiles && launch_tiles(c.g, false, nullptr, 0, &parts, nullptr) != FLUX_OK) return 0;
     return c.low_bytes + c.owner_bytes + parts;
 }
 
 extern "C" int flux_linear_lora_bf16(const flux_linear_lora_args* a, void* workspace, int64_t workspace_bytes, void* stream) {
     LoraCall c;
-    const int rc = read_lora_args(a, c);
+    const int rc = read_lora_args(a, workspace_bytes, c);
     if (rc != FLUX_OK || c.route == kNothing) return rc;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return fail(FLUX_E_NULL, "flux_linear_lora_bf16: the workspace must be 256-byte aligned memory");
     if (workspace_bytes < c.low_bytes + c.owner_bytes) return fail(FLUX_E_SHAPE, "flux_linear_lora_bf16: workspace of %lld bytes is too small", (long long)workspace_bytes);
     char* const ws = static_cast<char*>(workspace);
-    c.tail.low = c.low.low = reinterpret_cast<bf16_t*>(ws);
+    c.tail.low = c.low.low = ws;
     c.tail.owner = c.low.owner = reinterpret_cast<int*>(ws + c.low_bytes);
     float* const partial = reinterpret_cast<float*>(ws + c.low_bytes + c.owner_bytes);
     const hipStream_t st = static_cast<hipStream_t>(stream);

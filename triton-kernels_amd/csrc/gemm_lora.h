@@ -2,10 +2,12 @@
 //
 //   y[m] = act(x[m] W^T + bias + s_i (x[m] a_i^T) b_i^T),  i = the adapter of row m's request
 //
-// Two launches. The first one (lora_low_kernel) works out low[m] = s_i x[m] a_i^T, a few values a row, and rounds it to bf16, which the matrix
-// instructions of the second take: an error of 2^-9 of the adapter's own terms, below what y's rounding to bf16 leaves. The second one is
-// the product with W as ever; when a tile's sums are complete, low b_i^T is multiplied onto them from registers, K = 32 of the rank a step. So y
-// is written once and rounded once, and the adapter costs rank / K of the product's own time.
+// Two launches. The first one (lora_low_kernel) works out low[m] = s_i x[m] a_i^T, a few values a row, in fp32 and leaves it as the bf16 numbers that
+// the matrix instructions of the second take: the nearest one and the nearest to what that leaves over, 2^-16 of the value off. (One number
+// alone is 2^-8 of the adapter's terms off, not of y: where they cancel the rest of y, it is what y's error consists of.) The second one is
+// the product with W as ever; when a tile's sums are complete, low b_i^T is multiplied onto them from registers, K = 32 a step: both numbers of 16
+// ranks side by side or, beyond rank 16, both of 32 ranks one after the other onto the same columns of b. So y
+// is written once and rounded once, and the adapter costs a few times rank / K of the product's own time.
 //
 // Measured, us (the product with W by itself, then the first launch, then the second): 13008 x 12288 x 3072 rank 16 with GELU 738, 15.8 and 738; 4608 x 9216 x
 // 3072 rank 64 182, 15.5 and 195; 517 x 2048 x 2048 rank 32, two or three adapters in a tile of rows, 11.7, 4.9 and 14.3; six rows, 6144 x 1024 rank 16, 7.3,
@@ -18,12 +20,28 @@
 
 namespace flux {
 
+// How low lies in memory. For the tiles as a wave loads it: of 16 rows and a step of 32, one KB of first numbers, lane l's eight of row l % 16 at l * 16
+// bytes, and one of second numbers (planes 2); up to rank 16 the second numbers are the step's other 16 (planes 1), and beyond it, in a
+// workspace that has no room for them, there are none (planes 1). (By rows, a load's 64 lanes are 64 requests to the address unit: 4608 x 9216 x 3072, rank
+// 64, both numbers: 228 us for 222.) For the kernels without matrix instructions fp32 by rows (planes 0).
+struct LoraPlace {
+    int rank, width, planes;   // width: rank rounded up to whole steps of 32
+
+    __host__ __device__ bool beside() const { return planes == 1 && rank <= 16; }
+    __host__ __device__ int pitch() const { return (rank + 15) / 16 * 16; }                                 // planes 0
+    __host__ __device__ int64_t block(int64_t block, int k) const { return (block * (width / 32) + k / 32) * planes * 512; }   // 16 rows, a step
+    __host__ __device__ int64_t bytes(int64_t rows) const { return planes == 0 ? rows * pitch() * 4 : block((rows + 15) / 16, 0) * 2; }
+};
+
 struct LoraTail {
-    const bf16_t* low;     // [M][width]: zero from the rank on
+    const void* low;       // LoraPlace: zero from the rank on
     const int* owner;      // [M]: the row's adapter, -1: none
     const bf16_t* b;       // [adapters][N][rank]
-    int rank, width;       // width: rank rounded up to whole steps of 32
+    LoraPlace at;
     int vec;               // rows of b may be read so many values at a time: 8, 4 or 1
+
+    // planes 0
+    __device__ __forceinline__ float value(int64_t m, int r) const { return static_cast<const float*>(low)[m * at.pitch() + r]; }
 
     // Adds to the fragment rows of a wave: rows m0 .. of the product, columns n0 ... The adapters among the wave's rows are taken one after the
     // other in rising order, each with one read of its columns of b; rows of another adapter count as zeros, and so do values past the rank's end. 0 * inf
@@ -33,15 +51,14 @@ struct LoraTail {
     // A step's operands: columns of b of one adapter and the rows' low, 32 values each.
     template <int ROWS, int FN>
     struct Step {
-        u32x4 b[FN], low[ROWS];
+        u32x4 b[FN], low[ROWS], rest[ROWS];
     };
     template <int ROWS, int FN>
-    __device__ __forceinline__ void load(Step<ROWS, FN>& to, int a, int k, int m0, int n0, const GemmParams& p) const {
+    __device__ __forceinline__ void load_b(Step<ROWS, FN>& to, int a, int k, int n0, const GemmParams& p) const {
         // Scalar bases and 32-bit offsets: sixteen pointers would not fit the registers. Past the rank's end: values of the same row of b
         // again, which meet zeros of low.
-        const int frow = threadIdx.x & 15, at = k + ((threadIdx.x & 63) >> 4) * 8;
+        const int rank = this->at.rank, lane = threadIdx.x & 63, frow = lane & 15, slot = k + (lane >> 4) * 8, at = this->at.beside() ? slot & 15 : slot;
         const bf16_t* const col = b + static_cast<int64_t>(a) * p.N * rank;
-        const bf16_t* const row = low + static_cast<int64_t>(m0) * width;
         auto column = [&](int j) { return static_cast<uint32_t>(min(n0 + j * 16 + frow, p.N - 1)) * rank; };
         if (vec == 8) {
 #pragma unroll
@@ -61,8 +78,20 @@ struct LoraTail {
                 asm volatile("" ::: "memory");   // (a column at a time: eight registers of loads)
             }
         }
+    }
+    // Whether fragment rows without rows of a step's adapter are left out. Not in the tiles of more of them, whose registers do not allow the branches.
+    template <int ROWS> static constexpr bool kSkip = ROWS > 1 && ROWS <= 4;
+    // of: the fragment rows that are wanted. (Past M: the last rows' block again.)
+    template <int ROWS, int FN>
+    __device__ __forceinline__ void load_low(Step<ROWS, FN>& to, uint32_t of, int k, int m0, const GemmParams& p) const {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) to.low[i] = *reinterpret_cast<const u32x4*>(row + (static_cast<uint32_t>(min(i * 16 + frow, p.M - 1 - m0)) * width + at));
+        for (int i = 0; i < ROWS; ++i) {
+            if (kSkip<ROWS> && !(of >> i & 1u)) continue;
+            const u32x4* const from = reinterpret_cast<const u32x4*>(static_cast<const bf16_t*>(low) + at.block(min(m0 / 16 + i, (p.M - 1) / 16), k)) + lane;
+            to.low[i] = from[0];
+            if (at.planes == 2) to.rest[i] = from[64];
+        }
     }
 
     static constexpr int kNone = 0x7fffffff;
@@ -76,7 +105,7 @@ struct LoraTail {
     }
 
     // What a wave asks for before its sums are complete: the adapters of its rows, in front of everything else (begin), and behind its first slabs
-    // one value of every row of the first step's operands for the first adapters, so that they are in the L2 when it comes to them (touch).
+    // one value of every line of the first step's operands for the first adapters, so that they are in the L2 when it comes to them (touch).
     // Requested behind the loop over K alone, a tile waits for memory three times in a row with nothing beside it. (The operands themselves do not
     // fit beside the loop's: with them the 256-wide tile moved 450 registers a slab.)
     static constexpr int kTouch = 3;
@@ -105,11 +134,14 @@ struct LoraTail {
         for (int t = 0; t < kTouch; ++t) {   // (fewer adapters than that: the last one again)
             last = a == kNone ? last : a;
 #pragma unroll
-            for (int i = 0; i < (FN + 3) / 4; ++i) to.b[t][i] = b[(static_cast<int64_t>(last) * p.N + min(n0 + min(i * 64 + lane, FN * 16 - 1), p.N - 1)) * rank];
+            for (int i = 0; i < (FN + 3) / 4; ++i) to.b[t][i] = b[(static_cast<int64_t>(last) * p.N + min(n0 + min(i * 64 + lane, FN * 16 - 1), p.N - 1)) * at.rank];
             if (t + 1 < kTouch) a = a == kNone ? a : behind(to.own, a);
         }
 #pragma unroll
-        for (int i = 0; i < (ROWS + 3) / 4; ++i) to.low[i] = *reinterpret_cast<const uint32_t*>(low + static_cast<int64_t>(min(m0 + min(i * 64 + lane, ROWS * 16 - 1), p.M - 1)) * width);
+        for (int i = 0; i < (ROWS + 3) / 4; ++i) {   // (eight lines of either plane)
+            const int line = min(i * 64 + lane, ROWS * 16 - 1);
+            to.low[i] = *reinterpret_cast<const uint32_t*>(static_cast<const bf16_t*>(low) + at.block(min(m0 / 16 + (line >> 4), (p.M - 1) / 16), 0) + (line & (at.planes == 2 ? 15 : 7)) * 64);
+        }
     }
 
     template <int ROWS, int FN>
@@ -130,18 +162,20 @@ struct LoraTail {
     __device__ __forceinline__ void finish(f32x4 (&acc)[ROWS][FN], const int (&own)[ROWS], int m0, int n0, const GemmParams& p) const {
         int a = behind(own, -1);
         if (a == kNone) return;
-        bool same = true;
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) same = same && own[i] == a;
-        const bool all = __ballot(same) == ~uint64_t{0};
         Step<ROWS, FN> s;
+        uint32_t mine = ~0u;   // fragment rows that hold rows of the adapter: the others have no part in its products
+        bool first = true;
         for (int k = 0;;) {
-            load(s, a, k, m0, n0, p);
-            __builtin_amdgcn_sched_barrier(0);   // the loads stay in front of the products
-            if (!all) {
+            if (kSkip<ROWS> && k == 0) {
+                mine = 0;
 #pragma unroll
-                for (int i = 0; i < ROWS; ++i) s.low[i] = own[i] == a ? s.low[i] : u32x4{0, 0, 0, 0};
+                for (int i = 0; i < ROWS; ++i) mine |= __ballot(own[i] == a) != 0 ? 1u << i : 0u;
             }
+            load_b(s, a, k, n0, p);
+            // (low is the same for every adapter: where one step holds the rank it stays in its registers)
+            if (first || at.width > 32) load_low(s, at.width > 32 ? mine : ~0u, k, m0, p);
+            first = false;
+            __builtin_amdgcn_sched_barrier(0);   // the loads stay in front of the products
             uint32_t bad = 0;
 #pragma unroll
             for (int j = 0; j < FN; ++j)
@@ -150,15 +184,26 @@ struct LoraTail {
             if (__ballot((bad & 0x80008000u) != 0) != 0) not_finite_terms(acc, s, own, a, k);
 #pragma unroll
             for (int i = 0; i < ROWS; ++i)
+                if (!kSkip<ROWS> || (mine >> i & 1u)) multiply(acc, s.b, s.low[i], i, own[i] == a);
+            if (at.planes == 2) {
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, s.b[j]), __builtin_bit_cast(bf16x8, s.low[i]), acc[i][j], 0, 0, 0);
+                for (int i = 0; i < ROWS; ++i)
+                    if (!kSkip<ROWS> || (mine >> i & 1u)) multiply(acc, s.b, s.rest[i], i, own[i] == a);
+            }
             k += 32;
-            if (k >= width) {
+            if (k >= at.width) {
                 k = 0;
                 a = behind(own, a);
                 if (a == kNone) break;
             }
         }
+    }
+
+    template <int ROWS, int FN>
+    static __device__ __forceinline__ void multiply(f32x4 (&acc)[ROWS][FN], const u32x4 (&w)[FN], const u32x4& row, int i, bool own) {
+        const bf16x8 x = __builtin_bit_cast(bf16x8, own ? row : u32x4{0, 0, 0, 0});
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[j]), x, acc[i][j], 0, 0, 0);
     }
 
     // Of the halves of a word, in their top bits: infinite or NaN, mantissa not zero, value not zero; and all ones where the top bit is set.
@@ -177,10 +222,10 @@ struct LoraTail {
     // What is not finite in a step's columns of b, for the rows of adapter a, as low * b would have it: +inf and -inf by the signs, NaN where b is NaN or
     // low is zero. Both factors become 3.4e38 of their signs, whose product is infinite, and zero everywhere else; one combination of signs at a
     // time, so that terms of one instruction do not cancel before they are rounded, and NaN and zero are of either sign: +inf - inf. b itself is left with 1 of its sign
-    // (which keeps an infinite or NaN low what it is).
+    // (which keeps an infinite or NaN low what it is, and second numbers without effect beside an infinity).
     template <int ROWS, int FN>
     __device__ __forceinline__ void not_finite_terms(f32x4 (&acc)[ROWS][FN], Step<ROWS, FN>& s, const int (&own)[ROWS], int a, int k) const {
-        const int at = k + (lane_again() >> 4) * 8;
+        const int rank = this->at.rank, at = k + (lane_again() >> 4) * 8;
 #pragma unroll 1
         for (int signs = 0; signs < 4; ++signs) {
             // (the words count as new ones in every turn: what is worked out from them is not kept in registers over the turns)
@@ -225,8 +270,9 @@ struct LoraTail {
     }
 };
 
-// The sums are in accumulation registers from here on. Without it the compiler settles the whole kernel's registers by what happens behind the loop
-// over K: 360 moves between accumulation and ordinary registers a slab inside it, 1071 us for 814 at 13008 x 12288 x 3072.
+// The sums are in accumulation registers from here on: in front of the loop over K and behind it. Without the second the compiler settles the whole
+// kernel's registers by what happens behind the loop: 360 moves between accumulation and ordinary registers a slab inside it, 1071 us for 814 at
+// 13008 x 12288 x 3072. Without the first the tiles of 7 x 8 and 7 x 9 fragments wait for what they touch and put it aside.
 template <int ROWS, int FN>
 __device__ __forceinline__ void hold(f32x4 (&acc)[ROWS][FN]) {
 #pragma unroll
@@ -241,7 +287,8 @@ template <int MM>
 struct LoraRowTail {
     LoraTail t;
     int own[MM];
-    bf16_t low[MM], b[kGemvCols][MM];
+    float low[MM];
+    bf16_t b[kGemvCols][MM];
     int64_t row_b[kGemvCols][MM];
 
     __device__ __forceinline__ void begin() {
@@ -250,13 +297,13 @@ struct LoraRowTail {
         for (int m = 0; m < MM; ++m) own[m] = ((scalar)(reinterpret_cast<uintptr_t>(t.owner)))[m];
     }
     __device__ __forceinline__ void request(int n0, int lane, const GemmParams& p) {
-        const int r = lane < t.rank ? lane : 0;
+        const int r = lane < t.at.rank ? lane : 0;
 #pragma unroll
         for (int m = 0; m < MM; ++m) {
-            low[m] = t.low[static_cast<int64_t>(m) * t.width + r];
+            low[m] = t.value(m, r);
 #pragma unroll
             for (int c = 0; c < kGemvCols; ++c) {
-                row_b[c][m] = (static_cast<int64_t>(max(own[m], 0)) * p.N + min(n0 + c, p.N - 1)) * t.rank;
+                row_b[c][m] = (static_cast<int64_t>(max(own[m], 0)) * p.N + min(n0 + c, p.N - 1)) * t.at.rank;
                 b[c][m] = t.b[row_b[c][m] + r];
             }
         }
@@ -265,20 +312,20 @@ struct LoraRowTail {
 #pragma unroll
         for (int m = 0; m < MM; ++m)
 #pragma unroll
-            for (int c = 0; c < kGemvCols; ++c) acc[c][m] += own[m] >= 0 && lane < t.rank ? bf2f(low[m]) * bf2f(b[c][m]) : 0.0f;
-        for (int r = 64 + lane; r < t.rank; r += 64)
+            for (int c = 0; c < kGemvCols; ++c) acc[c][m] += own[m] >= 0 && lane < t.at.rank ? low[m] * bf2f(b[c][m]) : 0.0f;
+        for (int r = 64 + lane; r < t.at.rank; r += 64)
 #pragma unroll
             for (int m = 0; m < MM; ++m) {
-                const float l = bf2f(t.low[static_cast<int64_t>(m) * t.width + r]);
+                const float l = t.value(m, r);
 #pragma unroll
                 for (int c = 0; c < kGemvCols; ++c) acc[c][m] += own[m] >= 0 ? l * bf2f(t.b[row_b[c][m] + r]) : 0.0f;
             }
     }
 };
 
-// The tail of a launch whose rows begin `rows` further on.
+// The tail of a launch of tiles whose rows begin `rows`, a multiple of 16, further on.
 inline LoraTail tail_behind(LoraTail t, int64_t rows) {
-    t.low += rows * t.width;
+    t.low = static_cast<const bf16_t*>(t.low) + t.at.block(rows / 16, 0);
     t.owner += rows;
     return t;
 }
@@ -292,9 +339,10 @@ void launch_lora_scalar(const GemmParams& p, const LoraTail& tail, hipStream_t s
 // The first launch: low and owner.
 struct LoraLow {
     const bf16_t* x; const bf16_t* a; const void* adapter; const float* scaling;
-    bf16_t* low; int* owner;
+    void* low; int* owner;
+    LoraPlace at;
     int64_t lda, rows_per_request;
-    int M, K, rank, width, adapters;
+    int M, K, adapters;
     int wide_ids;      // 1: adapter is int64
     int vec;           // 1: x and a may be read 16 bytes at a time
 };

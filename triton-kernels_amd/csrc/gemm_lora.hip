@@ -45,19 +45,39 @@ __device__ __forceinline__ LowOfTile<R> low_of_tile(const LoraLow& p) {
     return t;
 }
 
-// The waves' sums, in LDS as [wave][R][NF][64 lanes][4], added in order, scaled, rounded and stored. Lane l of a fragment holds row l % 16 and
-// ranks l / 16 * 4 ...
+// The waves' sums, in LDS as [wave][R][NF][64 lanes][4], added in order, scaled and stored as LoraPlace says. Lane l of a fragment holds row l % 16
+// and four ranks from l / 16 * 4 on. A thread takes V of them: all four where a tile has work for every thread, fewer where threads would be idle.
 template <int R, int NF>
 __device__ __forceinline__ void low_store(const LoraLow& p, const LowOfTile<R>& t, const float* part, int waves, int r0) {
+    constexpr int V = R == 1 ? 1 : 4;
+    typedef float vec __attribute__((ext_vector_type(V)));
     const float scale = p.scaling != nullptr ? p.scaling[t.a] : 1.0f;
+    const bool beside = p.at.beside();
 #pragma unroll
     for (int f = 0; f < R; ++f)
-        for (int i = threadIdx.x; i < NF * 256; i += blockDim.x) {
+        for (int i = threadIdx.x * V; i < NF * 256; i += blockDim.x * V) {
             const int row = (i >> 2) & 15, m = t.row0 + f * 16 + row, r = r0 + (i >> 8) * 16 + ((i & 255) >> 6) * 4 + (i & 3);
-            float sum = 0.0f;
-            for (int w = 0; w < waves; ++w) sum += part[(w * R + f) * (NF * 256) + i];
+            vec sum = {};
+            for (int w = 0; w < waves; ++w) sum += *reinterpret_cast<const vec*>(part + (w * R + f) * (NF * 256) + (beside ? i & 255 : i));
             const bool mine = __shfl(t.own[f], row) == t.a;
-            if (mine && m < p.M && r < p.width) p.low[static_cast<int64_t>(m) * p.width + r] = r < p.rank ? f2bf(sum * scale) : static_cast<bf16_t>(0);
+            if (!mine || m >= p.M || r >= p.at.width) continue;
+            const int rank = beside ? r & 15 : r;   // (the first of V)
+            vec first, left;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                sum[e] = rank + e < p.at.rank ? sum[e] * scale : 0.0f;
+                first[e] = round_bf16(sum[e]);
+                left[e] = __builtin_isfinite(first[e]) ? sum[e] - first[e] : 0.0f;   // (nothing is left over of what is infinite or NaN)
+            }
+            if (p.at.planes == 0) {
+                if (r < p.at.pitch()) *reinterpret_cast<vec*>(static_cast<float*>(p.low) + static_cast<int64_t>(m) * p.at.pitch() + r) = sum;
+                continue;
+            }
+            typedef __bf16 halves __attribute__((ext_vector_type(V)));
+            const halves one = __builtin_convertvector(first, halves), two = __builtin_convertvector(left, halves);
+            bf16_t* const to = static_cast<bf16_t*>(p.low) + p.at.block(m / 16, r) + (((r >> 3) & 3) * 16 + (m & 15)) * 8 + (r & 7);
+            *reinterpret_cast<halves*>(to) = beside && r >= 16 ? two : one;
+            if (p.at.planes == 2) *reinterpret_cast<halves*>(to + 512) = two;
         }
 }
 
@@ -72,9 +92,9 @@ __global__ __launch_bounds__(WAVES * 64) void lora_low_kernel(LoraLow p) {
     const int r0 = blockIdx.z * (NF * 16);
     char* const mine = lds + wave * BYTES;
     // slot (row, position lane % 8) of 8 rows holds chunk position ^ (row / 2 % 8) of its row, so that 16 rows' chunks are read without conflicts
-    const int rows_x = min(p.M - t.row0, R * 16), rows_a = min(p.rank - r0, NF * 16);
+    const int rows_x = min(p.M - t.row0, R * 16), rows_a = min(p.at.rank - r0, NF * 16);
     bf16_t* const x = const_cast<bf16_t*>(p.x + t.row0 * p.lda);
-    bf16_t* const a = const_cast<bf16_t*>(p.a + (static_cast<int64_t>(t.a) * p.rank + r0) * p.K);
+    bf16_t* const a = const_cast<bf16_t*>(p.a + (static_cast<int64_t>(t.a) * p.at.rank + r0) * p.K);
     const int bytes_x = static_cast<int>(((rows_x - 1) * p.lda + p.K) * 2), bytes_a = rows_a * p.K * 2;
     uint32_t off_x[2 * R], off_a[2 * NF];
     int chunk[2];
@@ -150,7 +170,7 @@ __global__ __launch_bounds__(256) void lora_low_any_kernel(LoraLow p) {
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
             const int r = r0 + f * 16 + frow;
-            acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(piece(p.a + (static_cast<int64_t>(t.a) * p.rank + min(r, p.rank - 1)) * p.K, k0 + fq * 8, r < p.rank), xf, acc[f], 0, 0, 0);
+            acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(piece(p.a + (static_cast<int64_t>(t.a) * p.at.rank + min(r, p.at.rank - 1)) * p.K, k0 + fq * 8, r < p.at.rank), xf, acc[f], 0, 0, 0);
         }
     }
 #pragma unroll
@@ -163,7 +183,7 @@ void launch_lora_low(const LoraLow& p, hipStream_t st) {
     // adapters a tile can hold: requests that touch so many rows
     auto grid = [&](int rows, int ranks) {
         const int64_t requests = p.rows_per_request % rows == 0 ? 1 : std::min<int64_t>(rows, (rows - 2) / p.rows_per_request + 2);
-        return dim3((unsigned)((p.M + rows - 1) / rows), (unsigned)std::min<int64_t>(requests, p.adapters), (unsigned)((p.width + ranks - 1) / ranks));
+        return dim3((unsigned)((p.M + rows - 1) / rows), (unsigned)std::min<int64_t>(requests, p.adapters), (unsigned)((p.at.width + ranks - 1) / ranks));
     };
     if (!p.vec) {
         hipLaunchKernelGGL(lora_low_any_kernel, grid(16, 32), dim3(256), 0, st, p);
@@ -176,8 +196,8 @@ void launch_lora_low(const LoraLow& p, hipStream_t st) {
     // 41.3 at 13008; rank 64: 23.0, 25.1 and 29.1 at 2304, 33.9, 29.9 and 33.0 at 4608, 57.3, 53.0 and 50.2 at 13008. (16 rows of 16 and 4 waves at
     // 517, rank 16: 18.1 and 21.2, of 8: 18.3.)
     const bool few = (p.M + 15) / 16 < 256;
-    const int64_t blocks = static_cast<int64_t>((p.M + 31) / 32) * ((p.width + 63) / 64);
-    if (p.width <= 32) {
+    const int64_t blocks = static_cast<int64_t>((p.M + 31) / 32) * ((p.at.width + 63) / 64);
+    if (p.at.width <= 32) {
         if (few) CALL(1, 2, 8);
         else if (blocks <= 256) CALL(2, 2, 8);
         else CALL(2, 2, 4);
@@ -217,7 +237,10 @@ __global__ __launch_bounds__(kGemmThreads) void lora_ring_kernel(GemmLaunch L, L
     LoraTail::Ahead<2 * MI, 2 * MI> have;
     tail.begin(have, wm0, p);
     f32x4 acc[2 * MI][2 * MI];
-    gemm_tile_slabs<MI, KTAIL>(p, lds, m0, n0, (p.K + BK - 1) / BK, acc, [&]() { tail.touch(have, wm0, wn0, p); });
+    gemm_tile_slabs<MI, KTAIL>(p, lds, m0, n0, (p.K + BK - 1) / BK, acc, [&]() {
+        tail.touch(have, wm0, wn0, p);
+        hold(acc);
+    });
     hold(acc);
     tail.finish(acc, have, wm0, wn0, p);
     gemm_epilogue<MI, MI>(p, acc, lds, m0, n0, wave, lane);
@@ -237,7 +260,10 @@ __global__ __launch_bounds__(kGemmThreads) void lora_rect_kernel(GemmLaunch L, L
     LoraTail::Ahead<FM, FN> have;
     tail.begin(have, wm0, p);
     f32x4 acc[FM][FN];
-    gemm_rect_slabs<FM, FN, KTAIL>(p, lds, m0, n0, (p.K + BK - 1) / BK, acc, [&]() { tail.touch(have, wm0, wn0, p); });
+    gemm_rect_slabs<FM, FN, KTAIL>(p, lds, m0, n0, (p.K + BK - 1) / BK, acc, [&]() {
+        tail.touch(have, wm0, wn0, p);
+        hold(acc);
+    });
     hold(acc);
     tail.finish(acc, have, wm0, wn0, p);
     gemm_finish_rect<FM, FN, FM, false>(p, acc, lds, m0, n0, 0, wave, lane);
@@ -314,8 +340,8 @@ __global__ __launch_bounds__(256) void lora_scalar_kernel(GemmParams p, LoraTail
     float sum = 0.0f;
     for (int k = 0; k < p.K; ++k) sum += bf2f(a[k]) * bf2f(w[k]);
     if (own >= 0) {
-        const bf16_t* b = t.b + (static_cast<int64_t>(own) * p.N + n) * t.rank;
-        for (int r = 0; r < t.rank; ++r) sum += bf2f(t.low[static_cast<int64_t>(m) * t.width + r]) * bf2f(b[r]);
+        const bf16_t* b = t.b + (static_cast<int64_t>(own) * p.N + n) * t.at.rank;
+        for (int r = 0; r < t.at.rank; ++r) sum += t.value(m, r) * bf2f(b[r]);
     }
     sum += p.bias ? bf2f(p.bias[n]) : 0.0f;
     if (p.act == FLUX_ACT_GELU_TANH) sum = gelu_tanh_f32(sum);

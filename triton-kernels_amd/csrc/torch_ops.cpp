@@ -1026,7 +1026,7 @@ PyObject* py_linear_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const flux_linear_lora_args a = {xa.data_ptr(), wa.data_ptr(), ba.defined() ? ba.data_ptr() : nullptr, y.data_ptr(), a1.data_ptr(), a2.data_ptr(), ids.data_ptr(),
                                          sc.defined() ? static_cast<const float*>(sc.data_ptr()) : nullptr, M, N, K, M > 1 ? ld : K, N > 1 ? wa.stride(0) : K, N, ids.numel(),
                                          static_cast<int32_t>(adapters), static_cast<int32_t>(rank), ids.scalar_type() == at::kLong, static_cast<int32_t>(act)};
-        const int64_t need = may_cut_k(M, N, K) ? flux_linear_lora_workspace_bytes(&a) : flux_linear_lora_least_bytes(&a);
+        const int64_t need = may_cut_k(M, N, K) ? flux_linear_lora_workspace_bytes(&a) : 2 * flux_linear_lora_least_bytes(&a);
         const Tensor ws = empty({need}, at::kByte, xa);
         rc = flux_linear_lora_bf16(&a, need ? ws.data_ptr() : nullptr, need, stream_of(xa));
     }

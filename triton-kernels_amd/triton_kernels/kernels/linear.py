@@ -288,7 +288,7 @@ def linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, lora_b: 
               element), [B, L] or [rows] (an adapter by row), [] (one for all). A number that is no adapter's, -1 for one, means none.
     scaling : fp32 [adapters], or None for 1
 
-    Like linear it is not differentiated. x lora_a[i]^T is rounded to bf16, the sum of both products only as the result. What is not
+    Like linear it is not differentiated. Sums are fp32, s x lora_a[i]^T is good to 2^-16 of its value, the sum of both products is rounded once, as the result. What is not
     finite in an adapter does not reach other requests' rows, and its own rows as the formula has it, whatever else is in the call.
     """
     known = _ACTIVATIONS.get(activation)
