@@ -999,6 +999,12 @@ PyObject* py_linear_pair_into(PyObject*, PyObject* const* args, Py_ssize_t nargs
 
 // ---- linear with adapters ----------------------------------------------------------------------
 
+// What operands that require gradients have an edge to: an error, not nothing.
+struct NotDifferentiated : torch::autograd::Function<NotDifferentiated> {
+    static Tensor forward(torch::autograd::AutogradContext*, const Tensor&, const Tensor&, const std::optional<Tensor>&, const Tensor&, const Tensor&, const std::optional<Tensor>&, const Tensor* y) { return *y; }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) { TORCH_CHECK_NOT_IMPLEMENTED(false, "linear_lora is not differentiated"); }
+};
+
 // linear_lora(x, w, b or None, lora_a, lora_b, adapter, scaling or None, activation)
 PyObject* py_linear_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
@@ -1014,6 +1020,7 @@ PyObject* py_linear_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         id->sizes() != x->sizes().slice(0, id->dim()) || (b && (!is_bf16(*b, *x) || b->dim() != 1 || b->numel() != N || b->stride(0) != 1)) ||
         (scaling && (scaling->scalar_type() != at::kFloat || scaling->device() != x->device() || scaling->dim() != 1 || scaling->numel() != adapters || !scaling->is_contiguous())))
         Py_RETURN_NONE;
+    const bool recorded = at::GradMode::is_enabled() && (x->requires_grad() || w->requires_grad() || (b && b->requires_grad()) || la->requires_grad() || lb->requires_grad() || (scaling && scaling->requires_grad()));
     Tensor y;
     int rc;
     {
@@ -1029,6 +1036,10 @@ PyObject* py_linear_lora(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const int64_t need = may_cut_k(M, N, K) ? flux_linear_lora_workspace_bytes(&a) : 2 * flux_linear_lora_least_bytes(&a);
         const Tensor ws = empty({need}, at::kByte, xa);
         rc = flux_linear_lora_bf16(&a, need ? ws.data_ptr() : nullptr, need, stream_of(xa));
+        if (rc == FLUX_OK && recorded) {
+            const Tensor out = y;
+            y = NotDifferentiated::apply(xa, wa, given(ba), a1, a2, given(sc), &out);
+        }
     }
     if (rc < 0) Py_RETURN_NONE;   // (a refusal: its kind of error is the launcher's)
     check(rc, "flux_linear_lora_bf16");

@@ -288,7 +288,7 @@ def linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, lora_b: 
               element), [B, L] or [rows] (an adapter by row), [] (one for all). A number that is no adapter's, -1 for one, means none.
     scaling : fp32 [adapters], or None for 1
 
-    Like linear it is not differentiated. Sums are fp32, s x lora_a[i]^T is good to 2^-16 of its value, the sum of both products is rounded once, as the result. What is not
+    It is not differentiated: a gradient that reaches it raises NotImplementedError. Sums are fp32, s x lora_a[i]^T is good to 2^-16 of its value, the sum of both products is rounded once, as the result. What is not
     finite in an adapter does not reach other requests' rows, and its own rows as the formula has it, whatever else is in the call.
     """
     known = _ACTIVATIONS.get(activation)
@@ -296,6 +296,24 @@ def linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, lora_b: 
         y = nv.ops().linear_lora(x, w, b, lora_a, lora_b, adapter, scaling, known)
         if y is not None:
             return y
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, b, lora_a, lora_b, scaling)):
+        return _linear_lora.apply(x, w, b, lora_a, lora_b, adapter, scaling, activation)
+    return _launch_linear_lora(x, w, b, lora_a, lora_b, adapter, scaling, activation)
+
+
+class _linear_lora(torch.autograd.Function):
+    """What operands that require gradients have an edge to: an error, not nothing."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _launch_linear_lora(*args)
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise NotImplementedError("linear_lora is not differentiated")
+
+
+def _launch_linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, lora_b: Tensor, adapter: Tensor, scaling: Tensor | None, activation: str) -> Tensor:
     assert x.shape[-1] == w.shape[-1], "Incompatible dimensions"
     assert x.dtype == w.dtype and lora_a.dtype == x.dtype and lora_b.dtype == x.dtype, "Incompatible dtypes"
     _PLANS[x.dtype]  # KeyError for anything but bfloat16, as linear
