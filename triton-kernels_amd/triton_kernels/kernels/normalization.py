@@ -276,7 +276,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     tensor are read in place); either may be None. Their gradients are sums over the rows that share them, formed in fp32.
     plus_one : the factor is 1 + weight, adaLN's scale. layer_norm_modulation is that operator for inference, in the rounding order of
     PyTorch's bf16 operations and without gradients.
-    x is bf16 or fp32, [..., N] with N up to 65536; a bf16 x takes fp32 weights too.
+    x is bf16 or fp32, [..., N] with N up to 65536. weight and bias may be of other types than x, and each of its own: unless both are of x's they are taken
+    as fp32, and their gradients come in their types.
     """
     y = None if is_compiling() else nv.ops().layer_norm(x, weight, bias, eps, plus_one)
     if y is not None:
@@ -307,11 +308,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         t = t.reshape(-1, n)
         return _unit_stride(t if t.shape[0] == groups else t.expand(groups, n))
 
-    w_dtype = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
-    if w_dtype != x.dtype and not (x.dtype == torch.bfloat16 and w_dtype == torch.float32):
-        w_dtype = x.dtype
+    # fp32 where either holds more than x's type, and where one of the two is shared: its gradient is the sum of the groups', which are not rounded before that
+    w_dtype = x.dtype if all(t is None or t.dtype == x.dtype for t in (weight, bias)) else torch.float32
     if groups > 1 and any(t is not None and t.numel() == n for t in (weight, bias)):
-        w_dtype = torch.float32   # one of the two is shared: its gradient is the sum of the groups', which are not rounded before that
+        w_dtype = torch.float32
     rows = _unit_stride(x.reshape(batch, -1, n)) if x.numel() else x.reshape(batch, x.numel() // max(1, batch * n), n)
     y = _layer_norm.apply(rows, vectors(weight, w_dtype), vectors(bias, w_dtype), groups, float(eps), bool(plus_one), torch.is_grad_enabled())
     return y.reshape(x.shape)
