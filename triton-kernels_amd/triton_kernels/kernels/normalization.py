@@ -305,7 +305,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
             return None
         if t.dtype != dtype:
             t = t.to(dtype)
-        t = t.reshape(-1, n)
+        t = t.reshape(1 if t.numel() == n else groups, n)
         return _unit_stride(t if t.shape[0] == groups else t.expand(groups, n))
 
     # fp32 where either holds more than x's type, and where one of the two is shared: its gradient is the sum of the groups', which are not rounded before that
