@@ -284,7 +284,8 @@ def require_gpu(*tensors: torch.Tensor) -> torch.device:
 
 
 def stream_ptr(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    # (not through a stream object: torch.compile makes one of another class of it in the parts of a launcher that it traces)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev.index is None else dev.index)
 
 
 class on_device:

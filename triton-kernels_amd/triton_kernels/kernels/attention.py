@@ -6,7 +6,7 @@ import math
 
 import torch
 from torch import Tensor
-from torch.compiler import is_compiling
+from torch.compiler import is_dynamo_compiling
 
 from triton_kernels import _native as nv
 from triton_kernels.kernels.linear import hooked, positional, rows_args
@@ -36,7 +36,9 @@ def attention_into(q: Tensor, k: Tensor, v: Tensor, out: Tensor, sm_scale: float
     """q,k,v,out are [B,H,L,D] views (bf16, last dim contiguous, any other strides).
     beside: one or two linear_into calls of a few rows (the keyword arguments of each) that have nothing to do with the
     attention; the library runs them beside it in one launch where it can."""
-    if lse is None and not (beside and hooked()) and not is_compiling():
+    if is_dynamo_compiling():
+        return torch.compiler.disable(attention_into)(q, k, v, out, sm_scale, lse, beside)
+    if lse is None and not (beside and hooked()):
         o = nv.ops().attention(q, k, v, sm_scale, out, tuple(positional(**call) for call in beside))
         if o is not None:
             return o
@@ -73,7 +75,9 @@ def attention_into(q: Tensor, k: Tensor, v: Tensor, out: Tensor, sm_scale: float
 
 
 def scaled_dot_product_attention(q: Tensor, k: Tensor, v: Tensor, sm_scale: float = None) -> Tensor:
-    o = None if is_compiling() else nv.ops().attention(q, k, v, sm_scale)
+    if is_dynamo_compiling():
+        return torch.compiler.disable(scaled_dot_product_attention)(q, k, v, sm_scale)
+    o = nv.ops().attention(q, k, v, sm_scale)
     if o is not None:
         return o
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)

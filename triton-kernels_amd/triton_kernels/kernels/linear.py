@@ -7,7 +7,7 @@ import ctypes
 
 import torch
 from torch import Tensor
-from torch.compiler import is_compiling
+from torch.compiler import is_dynamo_compiling
 
 from triton_kernels import _native as nv
 
@@ -83,7 +83,10 @@ def linear_into(x: Tensor, w: Tensor, b: Tensor | None, *, activation: str = "",
             that leaves CUs free in its last round instead of one that fills the GPU exactly (same
             result, only the schedule differs); for callers that run streams side by side
     """
-    if launch_hook is None and not is_compiling():
+    if is_dynamo_compiling():
+        return torch.compiler.disable(linear_into)(x, w, b, activation=activation, act_begin=act_begin, out=out, out2=out2, split=split, resid=resid, gate=gate, qk=qk,
+                                                   in_activation=in_activation, shared_gpu=shared_gpu)
+    if launch_hook is None:
         y = nv.ops().linear_into(positional(x, w, b, activation=activation, act_begin=act_begin, out=out, out2=out2, split=split, resid=resid, gate=gate, qk=qk,
                                              in_activation=in_activation, shared_gpu=shared_gpu))
         if y is not None:
@@ -105,7 +108,9 @@ def linear_pair_into(first: dict, second: dict) -> tuple[Tensor, Tensor]:
     """Two linear_into calls (each the keyword arguments of one, `x`, `w` and `b` among them) in one library
     call: products of the same N, K and form of epilogue share a launch. An x of [B, L, K] may be a slice of
     a longer sequence, whose batch elements are not evenly strided rows."""
-    if launch_hook is None and not is_compiling():
+    if is_dynamo_compiling():
+        return torch.compiler.disable(linear_pair_into)(first, second)
+    if launch_hook is None:
         both = nv.ops().linear_pair_into(positional(**first), positional(**second))
         if both is not None:
             return both
@@ -268,8 +273,10 @@ def qk_pays(rows: int, w: Tensor, heads: int) -> bool:
 
 
 def linear(x: Tensor, w: Tensor, b: Tensor | None, activation: str = "", shared_gpu: bool = False) -> Tensor:
+    if is_dynamo_compiling():
+        return torch.compiler.disable(linear)(x, w, b, activation, shared_gpu)
     act = _ACTIVATIONS.get(activation)
-    if act is not None and launch_hook is None and not shared_gpu and not is_compiling():
+    if act is not None and launch_hook is None and not shared_gpu:
         y = nv.ops().linear(x, w, b, act)
         if y is not None:
             return y
@@ -288,11 +295,14 @@ def linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, lora_b: 
               element), [B, L] or [rows] (an adapter by row), [] (one for all). A number that is no adapter's, -1 for one, means none.
     scaling : fp32 [adapters], or None for 1
 
-    It is not differentiated: a gradient that reaches it raises NotImplementedError. Sums are fp32, s x lora_a[i]^T is good to 2^-16 of its value, the sum of both products is rounded once, as the result. What is not
-    finite in an adapter does not reach other requests' rows, and its own rows as the formula has it, whatever else is in the call.
+    It is not differentiated: a gradient that reaches it raises NotImplementedError. Sums are fp32, s x lora_a[i]^T is good to 2^-16 of its value, the
+    sum of both products is rounded once, as the result. What is not finite in an adapter does not reach other requests' rows, and its own rows as the
+    formula has it, whatever else is in the call.
     """
+    if is_dynamo_compiling():
+        return torch.compiler.disable(linear_lora)(x, w, b, lora_a, lora_b, adapter, scaling, activation)
     known = _ACTIVATIONS.get(activation)
-    if known is not None and launch_hook is None and not is_compiling():
+    if known is not None and launch_hook is None:
         y = nv.ops().linear_lora(x, w, b, lora_a, lora_b, adapter, scaling, known)
         if y is not None:
             return y

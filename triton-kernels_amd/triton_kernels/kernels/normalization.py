@@ -8,7 +8,7 @@ that can be trained (flux_layer_norm / flux_layer_norm_bwd).
 from __future__ import annotations
 
 import torch
-from torch.compiler import is_compiling
+from torch.compiler import is_dynamo_compiling
 
 from triton_kernels import _native as nv
 from triton_kernels.kernels.utils import calculate_settings
@@ -110,7 +110,9 @@ class _rms_norm(torch.autograd.Function):
 
 
 def rms_norm(x: torch.Tensor, scale: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
-    y = None if is_compiling() else nv.ops().rms_norm(x, scale, eps)
+    if is_dynamo_compiling():
+        return torch.compiler.disable(rms_norm)(x, scale, eps)
+    y = nv.ops().rms_norm(x, scale, eps)
     return _rms_norm.apply(x, scale, eps, torch.is_grad_enabled()) if y is None else y
 
 
@@ -134,7 +136,9 @@ def rms_norm_pair(x0, scale0, x1, scale1, eps: float = 1e-6) -> tuple[torch.Tens
     """(rms_norm(x0, scale0), rms_norm(x1, scale1)): one launch where nothing is differentiated and the two have
     the same width, types and device and 16-byte rows, two calls otherwise. At [1, 24, 256, 128] (q and k of one projection) the
     two calls took 50 us of host time, the copies of the views included; this takes 23, and 8 in native code."""
-    y = None if is_compiling() else nv.ops().rms_norm_pair(x0, scale0, x1, scale1, eps)
+    if is_dynamo_compiling():
+        return torch.compiler.disable(rms_norm_pair)(x0, scale0, x1, scale1, eps)
+    y = nv.ops().rms_norm_pair(x0, scale0, x1, scale1, eps)
     if y is not None:
         return y
     if (torch.is_grad_enabled() or x0.dtype != x1.dtype or x0.device != x1.device or scale0.dtype != scale1.dtype
@@ -146,7 +150,9 @@ def rms_norm_pair(x0, scale0, x1, scale1, eps: float = 1e-6) -> tuple[torch.Tens
 def layer_norm_modulation(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps=1e-5) -> torch.Tensor:
     """(1 + weight) * layer_norm(x) + bias, where weight is the adaLN *scale* and bias the *shift*,
     each [B, 1, N] (or [B, N]); chunks of a wider modulation tensor are read in place."""
-    y = None if is_compiling() else nv.ops().layer_norm_modulation(x, weight, bias, eps)
+    if is_dynamo_compiling():
+        return torch.compiler.disable(layer_norm_modulation)(x, weight, bias, eps)
+    y = nv.ops().layer_norm_modulation(x, weight, bias, eps)
     if y is not None:
         return y
     a, y, _keep = _layer_norm_args(x, weight, bias)
@@ -160,7 +166,9 @@ def layer_norm_modulation(x: torch.Tensor, weight: torch.Tensor, bias: torch.Ten
 
 def layer_norm_modulation_pair(first: tuple, second: tuple, eps=1e-5) -> tuple[torch.Tensor, torch.Tensor]:
     """layer_norm_modulation of two (x, weight, bias) triples of the same width and type in one launch."""
-    y = nv.ops().layer_norm_modulation_pair(*first, *second, eps) if len(first) == len(second) == 3 and not is_compiling() else None
+    if is_dynamo_compiling():
+        return torch.compiler.disable(layer_norm_modulation_pair)(first, second, eps)
+    y = nv.ops().layer_norm_modulation_pair(*first, *second, eps) if len(first) == len(second) == 3 else None
     if y is not None:
         return y
     a0, y0, _keep0 = _layer_norm_args(*first)
@@ -279,7 +287,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     x is bf16 or fp32, [..., N] with N up to 65536. weight and bias may be of other types than x, and each of its own: unless both are of x's they are taken
     as fp32, and their gradients come in their types.
     """
-    y = None if is_compiling() else nv.ops().layer_norm(x, weight, bias, eps, plus_one)
+    if is_dynamo_compiling():
+        return torch.compiler.disable(layer_norm)(x, weight, bias, eps, plus_one=plus_one)
+    y = nv.ops().layer_norm(x, weight, bias, eps, plus_one)
     if y is not None:
         return y
     nv.require_gpu(x, weight, bias)

@@ -7,7 +7,7 @@ import ctypes
 
 import torch
 from torch import Tensor
-from torch.compiler import is_compiling
+from torch.compiler import is_dynamo_compiling
 
 from triton_kernels import _native as nv
 
@@ -52,10 +52,12 @@ def qkv_prep(q_img: Tensor | None, k_img: Tensor | None, v_img: Tensor | None,
     """One streaming pass: concat(txt, img) along the sequence, optional per-head RMS norm of q/k,
     optional RoPE of q/k, v copied. Returns (q, k, v) contiguous [B,H,Lt+Li,D]; entries whose inputs
     were None come back as None. All sources are [B,H,L*,D] views (any batch/head/row strides)."""
-    if not is_compiling():
-        outs = nv.ops().qkv_prep(q_img, k_img, v_img, q_txt, k_txt, v_txt, pe, q_scale_img, k_scale_img, q_scale_txt, k_scale_txt, eps)
-        if outs is not None:
-            return outs
+    if is_dynamo_compiling():
+        return torch.compiler.disable(qkv_prep)(q_img, k_img, v_img, q_txt, k_txt, v_txt, pe=pe, q_scale_img=q_scale_img, k_scale_img=k_scale_img, q_scale_txt=q_scale_txt,
+                                                k_scale_txt=k_scale_txt, eps=eps)
+    outs = nv.ops().qkv_prep(q_img, k_img, v_img, q_txt, k_txt, v_txt, pe, q_scale_img, k_scale_img, q_scale_txt, k_scale_txt, eps)
+    if outs is not None:
+        return outs
     ref = next(t for t in (q_img, k_img, v_img) if t is not None)
     B, H, Li, D = ref.shape
     txt_ref = next((t for t in (q_txt, k_txt, v_txt) if t is not None), None)
@@ -112,7 +114,9 @@ def qkv_prep(q_img: Tensor | None, k_img: Tensor | None, v_img: Tensor | None,
 
 
 def apply_rope(xq: Tensor, xk: Tensor, freqs_cis: Tensor) -> tuple[Tensor, Tensor]:
-    both = None if is_compiling() else nv.ops().apply_rope(xq, xk, freqs_cis)
+    if is_dynamo_compiling():
+        return torch.compiler.disable(apply_rope)(xq, xk, freqs_cis)
+    both = nv.ops().apply_rope(xq, xk, freqs_cis)
     if both is not None:
         return both
     assert xq.dim() == 4 and xq.shape == xk.shape and xq.dtype == xk.dtype
@@ -214,7 +218,9 @@ def apply_rope_nd(xq: Tensor, xk: Tensor | None, ids: Tensor, axes_dim, theta: f
     Pair j of an axis of d values turns by ids[b, l, axis] * theta^(-2j/d), formed in 64 bits: apply_rope with EmbedND's table, without the
     table. The results are contiguous and rounded once.
     """
-    both = None if is_compiling() else nv.ops().apply_rope_nd(xq, xk, ids, axes_dim, theta)
+    if is_dynamo_compiling():
+        return torch.compiler.disable(apply_rope_nd)(xq, xk, ids, axes_dim, theta)
+    both = nv.ops().apply_rope_nd(xq, xk, ids, axes_dim, theta)
     if both is not None:
         return both
     for x in (xq, xk):
@@ -230,7 +236,9 @@ def apply_rope_nd(xq: Tensor, xk: Tensor | None, ids: Tensor, axes_dim, theta: f
 def rope_table(ids: Tensor, axes_dim, theta: float = 10000.0) -> Tensor:
     """The fp32 rotation matrices that the blocks and apply_rope take, [B, 1, L, D/2, 2, 2] for ids [B, L, n] ([1, 1, ...] for [L, n]):
     one kernel for what EmbedND of the plain blocks computes; arguments as in apply_rope_nd."""
-    out = None if is_compiling() else nv.ops().rope_table(ids, axes_dim, theta)
+    if is_dynamo_compiling():
+        return torch.compiler.disable(rope_table)(ids, axes_dim, theta)
+    out = nv.ops().rope_table(ids, axes_dim, theta)
     if out is not None:
         return out
     dev = nv.require_gpu(ids)
