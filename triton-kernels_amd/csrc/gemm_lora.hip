@@ -291,30 +291,26 @@ void launch_lora_rect(int fm, int fn, const GemmSet& g, const LoraTail& tail, hi
     else launch_rect<7, 8>(g, tail, st);
 }
 
-// Row vectors: the loops over K of launch_gemv (gemm_bf16.hip) that fit any K; W keeps the non-temporal hint where it is large.
-template <int MM, bool LDS, int U, bool ONCE>
+// Row vectors: the loops over K of launch_gemv (gemm_bf16.hip) that fit any K. W always has the non-temporal hint, which leaves the caches to the
+// adapters, low and the rows. us of the whole operator at rank 16 with and without it, W from HBM (the same W again at once): 6 x 6144 x 1024 12.9 and 16.4 (10.7,
+// 12.5), 1 x 9216 x 3072 17.9 and 21.0 (15.1, 17.4), 4 x 9216 x 3072 25.0 and 28.6 (20.8, 23.2), 1 x 3072 x 12288 33.8 and 40.5 (28.3, 28.7), 6 x 12288 x 12288
+// 107 and 195 (105, 195). Where 216 MiB are read again at once beside one or three rows it loses 5 and 6 %, and gains 17 and 10 % from HBM: 1 x 18432 x 6144
+// 45.0 and 54.1 (43.9, 41.8), 3 x 36864 x 3072 50.6 and 56.3 (48.4, 45.5).
+template <int MM, bool LDS, int U>
 __global__ __launch_bounds__(256) void lora_rows_kernel(GemmParams p, LoraTail t) {
     extern __shared__ __attribute__((aligned(16))) char act_lds[];
     LoraRowTail<MM> tail;
     tail.t = t;
-    gemv_small_m<MM, LDS, U, false, ONCE>(p, static_cast<int>(blockIdx.x), act_lds, tail);
+    gemv_small_m<MM, LDS, U, false, true>(p, static_cast<int>(blockIdx.x), act_lds, tail);
 }
 
 template <int MM>
 static void launch_rows_of(const GemmParams& p, const LoraTail& tail, hipStream_t st) {
     const dim3 grid((unsigned)((p.N + 4 * kGemvCols - 1) / (4 * kGemvCols)));
     const size_t act_bytes = static_cast<size_t>(MM) * p.K * 2;
-    const bool once = static_cast<int64_t>(p.N) * p.K * 2 <= (int64_t{128} << 20);
     constexpr int U = MM <= 2 ? 6 : 3;
-#define CALL(LDS, ONCE, BYTES) hipLaunchKernelGGL((lora_rows_kernel<MM, LDS, U, ONCE>), grid, dim3(256), BYTES, st, p, tail)
-    if (act_bytes <= kGemvSiluLds) {
-        if (once) CALL(true, true, act_bytes);
-        else CALL(true, false, act_bytes);
-    } else {
-        if (once) CALL(false, true, 0);
-        else CALL(false, false, 0);
-    }
-#undef CALL
+    if (act_bytes <= kGemvSiluLds) hipLaunchKernelGGL((lora_rows_kernel<MM, true, U>), grid, dim3(256), act_bytes, st, p, tail);
+    else hipLaunchKernelGGL((lora_rows_kernel<MM, false, U>), grid, dim3(256), 0, st, p, tail);
 }
 
 void launch_lora_rows(const GemmParams& p, const LoraTail& tail, hipStream_t st) {
