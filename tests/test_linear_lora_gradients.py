@@ -42,3 +42,18 @@ def test_a_gradient_that_reaches_it_is_an_error(monkeypatch, native):
             assert torch.equal(tk.linear_lora(**mine, adapter=adapter), plain)
     empty = tk.linear_lora(**{**operands, "x": operands["x"][:0].requires_grad_(True)}, adapter=adapter[:0])
     assert empty.shape == (0, 20, 64)
+
+
+@pytest.mark.gpu
+def test_forward_mode_and_transforms_are_refused():
+    import torch.autograd.forward_ad as fwad
+
+    g = seeded(2)
+    x, w, a, b = randn(g, 3, 20, 64, dtype=BF).to(DEV), randn(g, 48, 64, dtype=BF).to(DEV), randn(g, 2, 8, 64, dtype=BF).to(DEV), randn(g, 2, 48, 8, dtype=BF).to(DEV)
+    adapter = torch.tensor([1, -1, 0], device=DEV)
+    for at in range(4):
+        with fwad.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+            operands = [fwad.make_dual(t, torch.ones_like(t)) if i == at else t for i, t in enumerate((x, w, a, b))]
+            tk.linear_lora(operands[0], operands[1], None, *operands[2:], adapter)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: tk.linear_lora(t, w, None, a, b, adapter))(x[None])

@@ -306,13 +306,11 @@ def linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, lora_b: 
         y = nv.ops().linear_lora(x, w, b, lora_a, lora_b, adapter, scaling, known)
         if y is not None:
             return y
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, b, lora_a, lora_b, scaling)):
-        return _linear_lora.apply(x, w, b, lora_a, lora_b, adapter, scaling, activation)
-    return _launch_linear_lora(x, w, b, lora_a, lora_b, adapter, scaling, activation)
+    return _linear_lora.apply(x, w, b, lora_a, lora_b, adapter, scaling, activation)
 
 
 class _linear_lora(torch.autograd.Function):
-    """What operands that require gradients have an edge to: an error, not nothing."""
+    """What operands that require gradients have an edge to: an error, not nothing. Forward-mode derivatives and function transforms are refused as well."""
 
     @staticmethod
     def forward(ctx, *args):
