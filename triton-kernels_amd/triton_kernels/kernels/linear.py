@@ -345,7 +345,7 @@ def _launch_linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, 
     if w.stride(1) != 1 or (N > 1 and w.stride(0) < K):
         w = w.contiguous()
     if b is not None:
-        assert b.shape[-1] == N
+        assert b.dim() >= 1 and b.shape[-1] == b.numel() == N, f"the bias is [{N}], not {tuple(b.shape)}"
         b = b.to(x.dtype).contiguous()
     y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
     if y.numel() == 0:
