@@ -18,7 +18,7 @@ int flux_tune_abi_version(void);
 /* ---------------------------------------------------------------------------------------------
  * Layer norm with weights.   h = (x - mean) * rstd,  y = h * w + b,  rounded once.
  * x is [batch, seq, n] with element strides (sb, sl, 1), y contiguous. w and b are [n] vectors: one for all rows (groups 1), or one for
- * each batch element (groups == batch), w_sb and b_sb elements apart. w null: the factor is 1, b null: nothing is added. plus_one != 0:
+ * each batch element (groups == batch, 65535 at most), w_sb and b_sb elements apart. w null: the factor is 1, b null: nothing is added. plus_one != 0:
  * the factor is 1 + w (adaLN's scale).
  * mean and rstd (both or neither null) receive the fp32 statistics of every row, for the backward pass.
  * w and b may be FLUX_F32 while x is FLUX_BF16. Statistics, factors and sums are fp32.
@@ -62,7 +62,8 @@ typedef struct flux_rope_ids {
 
 /* q_out = q and k_out = k with every pair turned by its angle ((x0 c - x1 s, x0 s + x1 c); inverse != 0: by the negative one, which is the
  * backward pass). q is [B, Hq, L, D] and k [B, Hk, L, D] with strides as in flux_src4, D = 2 P; the outputs are contiguous. Either may be
- * absent (null pointers and no heads). fp32 arithmetic, rounded once; sines and cosines are within 2^-23 of those of the 64-bit angle. */
+ * absent (null pointers and no heads), B is 65535 at most. fp32 arithmetic, rounded once; sines and cosines of an angle of a radians are within
+ * 2^-23 + |a| (3 |log2 theta| + d / 5 + 5) 2^-53 of the exact ones, d the values of its axis; the second term is the smaller one up to positions of ten million. */
 typedef struct flux_rope_nd_args {
     flux_src4 q, k;
     void* q_out; void* k_out;
