@@ -571,7 +571,7 @@ static LnBwdPlan ln_bwd_plan(const flux_layer_norm_bwd_args& a) {
     // 16 waves a workgroup and one workgroup a CU (us at 4608 x 3072 for one, two and five rows a workgroup: 46.3, 31.5 and 26.7), fewer waves
     // where that leaves CUs without one (512 x 768, four rows and 16: 6.9 and 8.4)
     int per_block = kLnMost / p.row.T;
-    while (per_block > 1 && per_block * p.row.T > 256 && (rows + per_block - 1) / per_block < most) per_block /= 2;  
+    while (per_block > 1 && per_block * p.row.T > 256 && (rows + per_block - 1) / per_block < most) per_block /= 2;
     p.threads = per_block * p.row.T;
     p.blocks = static_cast<int>(std::min<int64_t>((rows + per_block - 1) / per_block, most));
     // Up to 128 rows the waves of a workgroup request all of a column's values at once, and with no more such workgroups than CUs that is quicker. us of

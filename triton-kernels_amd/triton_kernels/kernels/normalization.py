@@ -281,7 +281,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     """layer_norm(x) * weight + bias over the last dimension, with gradients for all three; rounded once.
 
     weight, bias : [N], shared by all rows, or one for each element of x's first dimension, [B, N] or [B, 1, ..., N] (chunks of a wider modulation
-    tensor are read in place); either may be None. Their gradients are sums over the rows that share them, formed in fp32.
+    tensor are read in place), 65535 of them at most; either may be None. Their gradients are sums over the rows that share them, formed in fp32.
     plus_one : the factor is 1 + weight, adaLN's scale. layer_norm_modulation is that operator for inference, in the rounding order of
     PyTorch's bf16 operations and without gradients.
     x is bf16 or fp32, [..., N] with N up to 65536. weight and bias may be of other types than x, and each of its own: unless both are of x's they are taken

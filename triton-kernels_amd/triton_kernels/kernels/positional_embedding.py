@@ -212,7 +212,7 @@ class _apply_rope_nd_inverse(torch.autograd.Function):
 def apply_rope_nd(xq: Tensor, xk: Tensor | None, ids: Tensor, axes_dim, theta: float = 10000.0) -> tuple[Tensor, Tensor | None]:
     """q and k rotated by positions of several axes (time, height, width), with gradients for both.
 
-    xq, xk : [B, H, L, D] views with any strides; xk may have another number of heads or be None. bf16 or fp32.
+    xq, xk : [B, H, L, D] views with any strides, B 65535 at most; xk may have another number of heads or be None. bf16 or fp32.
     ids : the tokens' positions, [B, L, n] or [L, n] for all batch elements: float32, float64, int32 or int64 (others are converted).
     axes_dim : values of a row that belong to each of the n axes, in order; even, D in all, at most 512.
     Pair j of an axis of d values turns by ids[b, l, axis] * theta^(-2j/d), formed in 64 bits: apply_rope with EmbedND's table, without the
