@@ -84,8 +84,9 @@ int flux_rope_table(const flux_rope_ids* at, float* out, int64_t B, int64_t L, v
  * is FLUX_ACT_NONE or FLUX_ACT_GELU_TANH. lora_a is [adapters, rank, K], lora_b [adapters, N, rank], contiguous bf16, with rank up to
  * FLUX_LORA_MOST_RANK; scaling is fp32 [adapters] or null (1). adapter holds one number for each of `requests` groups of M / requests rows that
  * follow one another, int32 or (wide_ids) int64; a number outside [0, adapters) means no adapter, whatever lora_a and lora_b hold.
- * fp32 sums, y rounded once; s_i x a_i^T goes between the two products as a bf16 number and another one for what that leaves over, 2^-16 of its value off. What is not finite in an adapter reaches rows of its own requests only,
- * as the formula has it: +inf and -inf by the signs, NaN for NaN, for 0 * inf and for infinities of both signs, whatever else is in the call.
+ * fp32 sums, y rounded once; s_i x a_i^T goes between the two products as a bf16 number and another one for what that leaves over, 2^-16 of its
+ * value off. What is not finite in an adapter reaches rows of its own requests only, as the formula has it: +inf and -inf by the signs, NaN for
+ * NaN, for 0 * inf and for infinities of both signs, whatever else is in the call.
  * The workspace (flux_linear_lora_workspace_bytes; 256-byte aligned, the launch's own until it has run) holds s_i x a_i^T and, where K is cut
  * over workgroups, partial sums; flux_linear_lora_least_bytes is what the call cannot do without. Beyond rank 16 that may have no room for the second
  * numbers of s_i x a_i^T, which is then off by 2^-8 of its value; twice that many bytes have it.

@@ -9,10 +9,11 @@
 // ranks side by side or, beyond rank 16, both of 32 ranks one after the other onto the same columns of b. So y
 // is written once and rounded once, and the adapter costs a few times rank / K of the product's own time.
 //
-// Measured, us (the product with W by itself, then the first launch, then the second): 13008 x 12288 x 3072 rank 16 with GELU 738, 15.8 and 738; 4608 x 9216 x
-// 3072 rank 64 182, 15.5 and 195; 517 x 2048 x 2048 rank 32, two or three adapters in a tile of rows, 11.7, 4.9 and 14.3; six rows, 6144 x 1024 rank 16, 7.3,
-// 3.7 and 8.8. Bound by the matrix instructions, for few rows by W from HBM and two dependent launches. Adapters mixed by row cost a pass
-// over x and a step of the tail each: 517 rows of 16 mixed adapters 8.8 and 17.5.
+// Measured, medians in us (the product with W by itself, then the first launch, then the second): 13008 x 12288 x 3072 rank 16 with GELU 738, 20.6 and 745;
+// 4608 x 9216 x 3072 rank 64 182, 16.6 and 207 to 223 by the power limit; 517 x 2048 x 2048 rank 32, two or three adapters in a tile of rows, 12.0, 5.0
+// and 14 to 15; six rows, 6144 x 1024 rank 16, 7.3, 4.0 and 9.0. Bound by the matrix instructions, for few rows by W from HBM and two dependent launches.
+// Adapters mixed by row cost a pass over x and a step of the tail each: 517 rows of 16 mixed adapters 9.4 and 18.2. Operands without 16-byte rows take a
+// kernel for which speed was not sought: 517 x 2048 x 2047 19.0 and 6733 (the product by itself 7671).
 #pragma once
 
 #include "gemm_common.h"
