@@ -29,8 +29,9 @@ struct LoraPlace {
     int rank, width, planes;   // width: rank rounded up to whole steps of 32
 
     __host__ __device__ bool beside() const { return planes == 1 && rank <= 16; }
-    __host__ __device__ int pitch() const { return (rank + 15) / 16 * 16; }                                 // planes 0
-    __host__ __device__ int64_t block(int64_t block, int k) const { return (block * (width / 32) + k / 32) * planes * 512; }   // 16 rows, a step
+    __host__ __device__ int pitch() const { return (rank + 15) / 16 * 16; }   // planes 0: values from row to row
+    // Otherwise: where rows 16 n .. and the step of slot k begin.
+    __host__ __device__ int64_t block(int64_t n, int k) const { return (n * (width / 32) + k / 32) * planes * 512; }
     __host__ __device__ int64_t bytes(int64_t rows) const { return planes == 0 ? rows * pitch() * 4 : block((rows + 15) / 16, 0) * 2; }
 };
 
@@ -80,7 +81,8 @@ struct LoraTail {
             }
         }
     }
-    // Whether fragment rows without rows of a step's adapter are left out. Not in the tiles of more of them, whose registers do not allow the branches.
+    // Whether fragment rows without rows of a step's adapter are left out. us with and without: 8192 x 1024 x 1024, rank 64, runs of 12 rows, four
+    // fragment rows a wave 63 and 71; 4608 x 9216 x 3072, rank 64, one adapter, nine of them 230 and 226.
     template <int ROWS> static constexpr bool kSkip = ROWS > 1 && ROWS <= 4;
     // of: the fragment rows that are wanted. (Past M: the last rows' block again.)
     template <int ROWS, int FN>
@@ -222,8 +224,8 @@ struct LoraTail {
 
     // What is not finite in a step's columns of b, for the rows of adapter a, as low * b would have it: +inf and -inf by the signs, NaN where b is NaN or
     // low is zero. Both factors become 3.4e38 of their signs, whose product is infinite, and zero everywhere else; one combination of signs at a
-    // time, so that terms of one instruction do not cancel before they are rounded, and NaN and zero are of either sign: +inf - inf. b itself is left with 1 of its sign
-    // (which keeps an infinite or NaN low what it is, and second numbers without effect beside an infinity).
+    // time, so that terms of one instruction do not cancel before they are rounded, and NaN and zero are of either sign: +inf - inf. b itself is
+    // left with 1 of its sign (which keeps an infinite or NaN low what it is, and second numbers without effect beside an infinity).
     template <int ROWS, int FN>
     __device__ __forceinline__ void not_finite_terms(f32x4 (&acc)[ROWS][FN], Step<ROWS, FN>& s, const int (&own)[ROWS], int a, int k) const {
         const int rank = this->at.rank, at = k + (lane_again() >> 4) * 8;
