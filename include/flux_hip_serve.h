@@ -1,0 +1,50 @@
+/*
+ * flux_hip_serve.h — C ABI of libfluxhip.so, third part: serving a block with less to read and less to multiply. Products with weights held in 4
+ * bits, and attention over the blocks of keys that a cheap score selects. The conventions of flux_hip.h (device pointers, strides in elements,
+ * streams, return values, flux_last_error, dtype codes) hold here too. None of these calls stands for an interface of the reference.
+ */
+#ifndef FLUX_HIP_SERVE_H
+#define FLUX_HIP_SERVE_H
+
+#include "flux_hip.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define FLUX_SERVE_ABI_VERSION 1
+int flux_serve_abi_version(void);
+
+/* ---------------------------------------------------------------------------------------------
+ * Weights in 4 bits.  W[n, k] = (q[n, k] - z[n, k / group]) * s[n, k / group], q and z in 0 .. 15, s bf16, z null: 8 everywhere; group 32, 64 or 128,
+ * K a multiple of it. In memory (N up to a multiple of 16, K of 128, what is behind them q = z = s = 0):
+ *   q      tiles of 16 rows x 128 columns, [ceil(N / 16)][ceil(K / 128)][4][16][16 bytes]: 16 bytes at [g][r] are row r's columns 32 j + 8 g + e
+ *          (j 0 .. 3 the 32-bit word, e 0 .. 7), e at bits 4 (e / 2) + 16 (e mod 2) of its word
+ *   s, z   [ceil(N / 16)][ceil(K / 128)][16][128 / group], two bytes and one byte each
+ * ------------------------------------------------------------------------------------------- */
+typedef struct flux_w4 {
+    const void* q; const void* s; const void* z;
+    int64_t N, K;
+    int32_t group;
+} flux_w4;
+
+/* y[m] = act(f(x[m]) W^T + bias): x [M, K] bf16 (row stride ldx), bias [N] bf16 or null, y [M, N] bf16 (row stride ldy); act is FLUX_ACT_NONE or
+ * FLUX_ACT_GELU_TANH, in_act FLUX_ACT_NONE or (up to 8 rows) FLUX_ACT_SILU, f(x) = x sigmoid(x). fp32 sums, rounded once; f(x) is held to 2^-16 of its
+ * value. From some number of rows on the weights are laid out as bf16, each rounded once (2^-9 of it), in the workspace
+ * (flux_linear_w4_workspace_bytes, 0 below; 256-byte aligned, the launch's own until it has run) in front of flux_linear_bf16. */
+typedef struct flux_linear_w4_args {
+    const void* x; const void* bias; void* y;
+    flux_w4 w;
+    int64_t M, ldx, ldy;
+    int32_t act, in_act;
+} flux_linear_w4_args;
+int64_t flux_linear_w4_workspace_bytes(const flux_linear_w4_args* args);
+int flux_linear_w4_bf16(const flux_linear_w4_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The weights themselves, out [N, K] bf16, contiguous, rounded once. */
+int flux_w4_unpack(const flux_w4* w, void* out, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* FLUX_HIP_SERVE_H */

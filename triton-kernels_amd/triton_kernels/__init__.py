@@ -13,6 +13,7 @@ from triton_kernels.functional import (
     rms_norm_torch_compile,
 )
 from triton_kernels.kernels import (
+    W4,
     apply_rope,
     apply_rope_nd,
     attention_into,
@@ -21,7 +22,10 @@ from triton_kernels.kernels import (
     linear,
     linear_into,
     linear_lora,
+    linear_w4,
+    pack_w4,
     qkv_prep,
+    quantize_w4,
     rms_norm,
     rope_table,
     scaled_dot_product_attention,
@@ -32,6 +36,6 @@ __all__ = [
     "apply_rope_nd_torch", "apply_rope_torch", "apply_rope_torch_compile", "layer_norm_modulation_torch",
     "layer_norm_modulation_torch_compile", "layer_norm_torch", "linear_lora_torch", "rms_norm_torch", "rms_norm_torch_compile",
     "apply_rope", "apply_rope_nd", "layer_norm", "layer_norm_modulation", "linear", "rms_norm", "scaled_dot_product_attention",
-    "attention_into", "linear_into", "linear_lora", "qkv_prep", "rope_table",
+    "attention_into", "linear_into", "linear_lora", "linear_w4", "qkv_prep", "rope_table", "W4", "pack_w4", "quantize_w4",
     "DoubleStreamBlock", "EmbedND", "LayerNorm", "QKNorm", "RMSNorm", "SingleStreamBlock",
 ]

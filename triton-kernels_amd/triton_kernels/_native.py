@@ -140,6 +140,17 @@ class LinearLoraArgs(Structure):
     ]
 
 
+class W4(Structure):
+    _fields_ = [("q", c_void_p), ("s", c_void_p), ("z", c_void_p), ("N", c_int64), ("K", c_int64), ("group", c_int32)]
+
+
+class LinearW4Args(Structure):
+    _fields_ = [
+        ("x", c_void_p), ("bias", c_void_p), ("y", c_void_p), ("w", W4),
+        ("M", c_int64), ("ldx", c_int64), ("ldy", c_int64), ("act", c_int32), ("in_act", c_int32),
+    ]
+
+
 # name -> (restype, argtypes); also the list the symbol-export test walks.
 SIGNATURES = {
     "flux_abi_version": (c_int32, []),
@@ -190,6 +201,15 @@ TUNE_SIGNATURES = {
     "flux_linear_lora_bf16": (c_int32, [POINTER(LinearLoraArgs), c_void_p, c_int64, c_void_p]),
 }
 
+# The same for include/flux_hip_serve.h.
+SERVE_ABI_VERSION = 1
+SERVE_SIGNATURES = {
+    "flux_serve_abi_version": (c_int32, []),
+    "flux_linear_w4_workspace_bytes": (c_int64, [POINTER(LinearW4Args)]),
+    "flux_linear_w4_bf16": (c_int32, [POINTER(LinearW4Args), c_void_p, c_int64, c_void_p]),
+    "flux_w4_unpack": (c_int32, [POINTER(W4), c_void_p, c_void_p]),
+}
+
 
 def lib_path() -> str:
     return _LIB_PATH
@@ -207,11 +227,12 @@ def lib():
                 "(or `make -C triton-kernels_amd/csrc`). There is no fallback path."
             )
         handle = ctypes.CDLL(_LIB_PATH)
-        for name, (res, args) in {**SIGNATURES, **TUNE_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **TUNE_SIGNATURES, **SERVE_SIGNATURES}.items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
-        if handle.flux_abi_version() != ABI_VERSION or handle.flux_tune_abi_version() != TUNE_ABI_VERSION:
+        if handle.flux_abi_version() != ABI_VERSION or handle.flux_tune_abi_version() != TUNE_ABI_VERSION \
+                or handle.flux_serve_abi_version() != SERVE_ABI_VERSION:
             raise RuntimeError("libfluxhip.so: ABI version mismatch")
         _lib = handle
     return _lib
@@ -325,6 +346,6 @@ def src4(t: torch.Tensor | None) -> Src4:
 __all__ = [
     "lib", "lib_path", "check", "last_error", "dtype_code", "require_gpu", "stream_ptr", "on_device", "ptr", "src4",
     "Src4", "QkvPrepArgs", "LinearArgs", "LinearPairArgs", "LinearPlan", "RmsNormArgs", "LayerNormArgs", "AttnArgs", "LayerNormFwdArgs", "LayerNormBwdArgs", "RopeIds", "RopeNdArgs", "LinearLoraArgs",
-    "SIGNATURES", "TUNE_SIGNATURES", "byref",
+    "W4", "LinearW4Args", "SIGNATURES", "TUNE_SIGNATURES", "SERVE_SIGNATURES", "byref",
     "FLUX_BF16", "FLUX_F32", "ACT_NONE", "ACT_GELU_TANH", "ACT_SILU", "LINEAR_SHARED_GPU", "MAX_ROW",
 ]

@@ -1,6 +1,6 @@
 """linear: y = act(x @ w.T + b) on the bf16 matrix cores (kernels/linear.py:104-151 of the reference),
 with the extra epilogues the fused Flux blocks use; linear_lora, which the reference does not have, is the same with
-a low-rank adapter of each request's own."""
+a low-rank adapter of each request's own, and linear_w4 with a weight held in 4 bits."""
 from __future__ import annotations
 
 import ctypes
@@ -10,6 +10,7 @@ from torch import Tensor
 from torch.compiler import is_dynamo_compiling
 
 from triton_kernels import _native as nv
+from triton_kernels.kernels.quantization import W4
 
 _ACTIVATIONS = {"": nv.ACT_NONE, "GELU": nv.ACT_GELU_TANH}
 # Tile plan per dtype; like the reference's table it has a single entry, so any other dtype is a KeyError.
@@ -361,4 +362,61 @@ def _launch_linear_lora(x: Tensor, w: Tensor, b: Tensor | None, lora_a: Tensor, 
         ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
         rc = nv.lib().flux_linear_lora_bf16(nv.byref(a), nv.ptr(ws), need, nv.stream_ptr(dev))
     nv.check(rc, "flux_linear_lora_bf16")
+    return y
+
+
+def linear_w4(x: Tensor, w: W4, b: Tensor | None = None, *, activation: str = "", in_activation: str = "") -> Tensor:
+    """y = act(f(x) w^T + b) with a weight in 4 bits.
+
+    x             : bf16 [..., K], b : [N] or None, result bf16 [..., N]
+    activation    : "" or "GELU", as in linear
+    in_activation : "SiLU" applies x * sigmoid(x) to x on the way in; at most 8 rows
+
+    Sums are fp32 and y is rounded once; up to 64 rows the weights are what the numbers stand for, beyond them they are laid out as bf16 first, each rounded
+    once. x * sigmoid(x) keeps 16 bits. What is not finite in x goes as in the formula. It is not differentiated: a gradient that reaches it raises NotImplementedError.
+    """
+    if is_dynamo_compiling():
+        return torch.compiler.disable(linear_w4)(x, w, b, activation=activation, in_activation=in_activation)
+    return _linear_w4.apply(x, b, w, activation, in_activation)
+
+
+class _linear_w4(torch.autograd.Function):
+    """What operands that require gradients have an edge to: an error, not nothing. Forward-mode derivatives and function transforms are refused as well."""
+
+    @staticmethod
+    def forward(ctx, x, b, w, activation, in_activation):
+        return _launch_linear_w4(x, w, b, activation, in_activation)
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise NotImplementedError("linear_w4 is not differentiated")
+
+
+def _launch_linear_w4(x: Tensor, w: W4, b: Tensor | None, activation: str, in_activation: str) -> Tensor:
+    n, k = w.shape
+    assert x.dim() >= 1 and x.shape[-1] == k, "Incompatible dimensions"
+    if x.dtype != torch.bfloat16:
+        raise TypeError(f"unsupported dtype {x.dtype}: linear_w4 takes bfloat16")
+    act, in_act = _ACTIVATIONS[activation], _IN_ACTIVATIONS[in_activation]
+    dev = nv.require_gpu(x, w.packed, w.scale, w.zero, b)
+    y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=dev)
+    if b is not None:
+        assert b.dim() == 1 and b.numel() == n, f"the bias is [{n}], not {tuple(b.shape)}"
+        b = b.to(x.dtype).contiguous()
+    if y.numel() == 0:
+        return y
+    x2 = _rows_2d(x, k)
+    m = x2.shape[0]
+    if x2.data_ptr() % 16 or (m > 1 and x2.stride(0) % 8):
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    a = nv.LinearW4Args(x2.data_ptr(), nv.ptr(b), y.data_ptr(), w._args(), m, x2.stride(0) if m > 1 else k, n, act, in_act)
+    if launch_hook is not None:
+        note = linear_launch_metadata(m, n, k, x.element_size(), "+".join(p for p in (activation, in_activation and f"in:{in_activation}", f"4 bits by {w.group}") if p))
+        note["bytes"] -= 1.5 * n * k
+        launch_hook(note)
+    with nv.on_device(dev):
+        need = nv.lib().flux_linear_w4_workspace_bytes(nv.byref(a))
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        rc = nv.lib().flux_linear_w4_bf16(nv.byref(a), nv.ptr(ws), need, nv.stream_ptr(dev))
+    nv.check(rc, "flux_linear_w4_bf16")
     return y
