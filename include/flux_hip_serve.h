@@ -44,6 +44,40 @@ int flux_linear_w4_bf16(const flux_linear_w4_args* args, void* workspace, int64_
 /* The weights themselves, out [N, K] bf16, contiguous, rounded once. */
 int flux_w4_unpack(const flux_w4* w, void* out, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Which blocks of keys a block of queries attends to.
+ * q [B, Hq, Lq, D] and k [B, Hk, Lk, D] bf16 with strides as in flux_src4, Hq a multiple of Hk (query head h reads key head h / (Hq / Hk)), D 64 or 128. For each
+ * block of FLUX_QUERY_BLOCK queries (the last may be shorter) the scores of the blocks of FLUX_KEY_BLOCK keys are mean(q) . mean(k), formed in 64 bits;
+ * the `keep` largest (or all, where there are no more) are chosen, the lower number among equals, a NaN below everything, the first `always` blocks in any case.
+ * lengths (int32 [B], or null): keys from lengths[b] on are not there; below 0 counts as 0, beyond Lk as Lk.
+ * blocks receives int32 [B, Hq, ceil(Lq / 128), min(keep, ceil(Lk / 64))]: the chosen numbers in ascending order, -1 behind them.
+ * The workspace (flux_select_blocks_workspace_bytes; 256-byte aligned) holds the means and scores.
+ * ------------------------------------------------------------------------------------------- */
+enum { FLUX_QUERY_BLOCK = 128, FLUX_KEY_BLOCK = 64, FLUX_SELECT_MOST_BLOCKS = 16384 };
+typedef struct flux_select_blocks_args {
+    flux_src4 q, k;
+    const int32_t* lengths; int32_t* blocks;
+    int64_t B, Hq, Hk, Lq, Lk, keep, always;
+    int32_t D;
+} flux_select_blocks_args;
+int64_t flux_select_blocks_workspace_bytes(const flux_select_blocks_args* args);
+int flux_select_blocks(const flux_select_blocks_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention of every block of queries over the blocks of keys that its list names:
+ *   o[i] = sum_j p_j v[j],  p = softmax(sm_scale q[i] . k[j]) over the tokens j of those blocks, j < min(lengths[b], Lk).
+ * q, o [B, Hq, Lq, D], k, v [B, Hk, Lk, D] bf16. blocks is int32 [B, Hq, ceil(Lq / 128), count], contiguous; numbers that are no block of the sequence
+ * name nothing, a number that stands there twice counts twice. Rows that see no token at all are 0. sm_scale is finite.
+ * The workspace (flux_sparse_attention_workspace_bytes, 0 where lists are not cut; 256-byte aligned) holds partial results. */
+typedef struct flux_sparse_attention_args {
+    flux_src4 q, k, v;
+    void* o; int64_t o_sb, o_sh, o_sl;
+    const int32_t* blocks; const int32_t* lengths;
+    int64_t B, Hq, Hk, Lq, Lk, count;
+    int32_t D; float sm_scale;
+} flux_sparse_attention_args;
+int64_t flux_sparse_attention_workspace_bytes(const flux_sparse_attention_args* args);
+int flux_sparse_attention_bf16(const flux_sparse_attention_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

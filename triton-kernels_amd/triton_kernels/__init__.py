@@ -17,6 +17,7 @@ from triton_kernels.kernels import (
     apply_rope,
     apply_rope_nd,
     attention_into,
+    block_sparse_attention,
     layer_norm,
     layer_norm_modulation,
     linear,
@@ -29,6 +30,7 @@ from triton_kernels.kernels import (
     rms_norm,
     rope_table,
     scaled_dot_product_attention,
+    select_blocks,
 )
 from triton_kernels.modules import DoubleStreamBlock, EmbedND, LayerNorm, QKNorm, RMSNorm, SingleStreamBlock
 
@@ -36,6 +38,6 @@ __all__ = [
     "apply_rope_nd_torch", "apply_rope_torch", "apply_rope_torch_compile", "layer_norm_modulation_torch",
     "layer_norm_modulation_torch_compile", "layer_norm_torch", "linear_lora_torch", "rms_norm_torch", "rms_norm_torch_compile",
     "apply_rope", "apply_rope_nd", "layer_norm", "layer_norm_modulation", "linear", "rms_norm", "scaled_dot_product_attention",
-    "attention_into", "linear_into", "linear_lora", "linear_w4", "qkv_prep", "rope_table", "W4", "pack_w4", "quantize_w4",
+    "attention_into", "linear_into", "linear_lora", "linear_w4", "qkv_prep", "rope_table", "W4", "pack_w4", "quantize_w4", "block_sparse_attention", "select_blocks",
     "DoubleStreamBlock", "EmbedND", "LayerNorm", "QKNorm", "RMSNorm", "SingleStreamBlock",
 ]

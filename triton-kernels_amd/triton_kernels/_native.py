@@ -151,6 +151,21 @@ class LinearW4Args(Structure):
     ]
 
 
+class SelectBlocksArgs(Structure):
+    _fields_ = [
+        ("q", Src4), ("k", Src4), ("lengths", c_void_p), ("blocks", c_void_p),
+        ("B", c_int64), ("Hq", c_int64), ("Hk", c_int64), ("Lq", c_int64), ("Lk", c_int64), ("keep", c_int64), ("always", c_int64), ("D", c_int32),
+    ]
+
+
+class SparseAttentionArgs(Structure):
+    _fields_ = [
+        ("q", Src4), ("k", Src4), ("v", Src4), ("o", c_void_p), ("o_sb", c_int64), ("o_sh", c_int64), ("o_sl", c_int64),
+        ("blocks", c_void_p), ("lengths", c_void_p),
+        ("B", c_int64), ("Hq", c_int64), ("Hk", c_int64), ("Lq", c_int64), ("Lk", c_int64), ("count", c_int64), ("D", c_int32), ("sm_scale", c_float),
+    ]
+
+
 # name -> (restype, argtypes); also the list the symbol-export test walks.
 SIGNATURES = {
     "flux_abi_version": (c_int32, []),
@@ -208,6 +223,10 @@ SERVE_SIGNATURES = {
     "flux_linear_w4_workspace_bytes": (c_int64, [POINTER(LinearW4Args)]),
     "flux_linear_w4_bf16": (c_int32, [POINTER(LinearW4Args), c_void_p, c_int64, c_void_p]),
     "flux_w4_unpack": (c_int32, [POINTER(W4), c_void_p, c_void_p]),
+    "flux_select_blocks_workspace_bytes": (c_int64, [POINTER(SelectBlocksArgs)]),
+    "flux_select_blocks": (c_int32, [POINTER(SelectBlocksArgs), c_void_p, c_int64, c_void_p]),
+    "flux_sparse_attention_workspace_bytes": (c_int64, [POINTER(SparseAttentionArgs)]),
+    "flux_sparse_attention_bf16": (c_int32, [POINTER(SparseAttentionArgs), c_void_p, c_int64, c_void_p]),
 }
 
 
@@ -346,6 +365,6 @@ def src4(t: torch.Tensor | None) -> Src4:
 __all__ = [
     "lib", "lib_path", "check", "last_error", "dtype_code", "require_gpu", "stream_ptr", "on_device", "ptr", "src4",
     "Src4", "QkvPrepArgs", "LinearArgs", "LinearPairArgs", "LinearPlan", "RmsNormArgs", "LayerNormArgs", "AttnArgs", "LayerNormFwdArgs", "LayerNormBwdArgs", "RopeIds", "RopeNdArgs", "LinearLoraArgs",
-    "W4", "LinearW4Args", "SIGNATURES", "TUNE_SIGNATURES", "SERVE_SIGNATURES", "byref",
+    "W4", "LinearW4Args", "SelectBlocksArgs", "SparseAttentionArgs", "SIGNATURES", "TUNE_SIGNATURES", "SERVE_SIGNATURES", "byref",
     "FLUX_BF16", "FLUX_F32", "ACT_NONE", "ACT_GELU_TANH", "ACT_SILU", "LINEAR_SHARED_GPU", "MAX_ROW",
 ]

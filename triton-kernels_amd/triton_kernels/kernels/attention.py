@@ -1,5 +1,6 @@
 """scaled_dot_product_attention: non-causal flash-attention forward (kernels/attention.py:173-221 of
-the reference) on the HIP kernel flux_attention_fwd_bf16."""
+the reference) on the HIP kernel flux_attention_fwd_bf16. select_blocks and block_sparse_attention, which the reference does not
+have, are attention over the blocks of keys that a cheap score selects for each block of queries."""
 from __future__ import annotations
 
 import math
@@ -82,3 +83,122 @@ def scaled_dot_product_attention(q: Tensor, k: Tensor, v: Tensor, sm_scale: floa
         return o
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     return attention_into(q, k, v, o, sm_scale)
+
+
+QUERY_BLOCK, KEY_BLOCK = 128, 64
+
+
+def _lengths(lengths: Tensor | None, batch: int, dev: torch.device, most: int) -> Tensor | None:
+    if lengths is None:
+        return None
+    if lengths.is_floating_point() or lengths.is_complex() or lengths.dtype == torch.bool:
+        raise TypeError(f"unsupported dtype {lengths.dtype} of lengths")
+    assert lengths.shape == (batch,), f"lengths are [{batch}], not {tuple(lengths.shape)}"
+    if lengths.dtype != torch.int32:
+        lengths = lengths.clamp(0, most).to(torch.int32)   # (a number beyond 32 bits is a long sequence, not what is left of it)
+    return lengths.contiguous()
+
+
+def _sparse_shapes(name: str, q: Tensor, k: Tensor) -> tuple[int, int, int, int, int, int]:
+    assert q.dim() == 4 and k.dim() == 4 and q.shape[0] == k.shape[0] and q.shape[3] == k.shape[3], f"{name}: q is [B, Hq, Lq, D] and k [B, Hk, Lk, D], not {tuple(q.shape)} and {tuple(k.shape)}"
+    B, Hq, Lq, D = q.shape
+    Hk, Lk = k.shape[1:3]
+    assert Hk > 0 and Hq > 0 and Hq % Hk == 0, f"{name}: {Hq} heads of q are no multiple of {Hk} heads of k"
+    assert D in (64, 128), f"{name}: heads of 64 or 128, not {D}"
+    return B, Hq, Hk, Lq, Lk, D
+
+
+def select_blocks(q: Tensor, k: Tensor, keep: int, *, always: int = 0, lengths: Tensor | None = None) -> Tensor:
+    """The blocks of 64 keys that each block of 128 queries attends to: int32 [B, Hq, ceil(Lq / 128), min(keep, ceil(Lk / 64))].
+
+    q, k    : bf16 [B, Hq, Lq, D] and [B, Hk, Lk, D] views, heads of 64 or 128; Hq is a multiple of Hk, query head h reads key head h // (Hq // Hk).
+              Up to 16384 blocks of keys
+    keep    : how many blocks; all of them where there are no more
+    always  : the first `always` blocks are among them in any case (the text in front of an image)
+    lengths : whole numbers [B] on the GPU, or None: keys from lengths[b] on are not there
+
+    A block's score is the product of the queries' mean and the mean of its keys, both formed in 64 bits, so that the choice does not go with rounding; the
+    lower number goes first among equals, a NaN comes last. The numbers ascend; where a sequence has fewer blocks, -1 stands behind them. Not differentiated.
+    """
+    if is_dynamo_compiling():
+        return torch.compiler.disable(select_blocks)(q, k, keep, always=always, lengths=lengths)
+    B, Hq, Hk, Lq, Lk, D = _sparse_shapes("select_blocks", q, k)
+    if q.dtype != torch.bfloat16 or k.dtype != q.dtype:
+        raise TypeError("select_blocks: the HIP kernel takes bfloat16 q, k")
+    keep, always = int(keep), int(always)
+    assert keep >= 0 and always >= 0, f"select_blocks: keep and always are counts, not {keep} and {always}"
+    dev = nv.require_gpu(q, k, lengths)
+    lengths = _lengths(lengths, B, dev, Lk)
+    q, k = _bhld_view(q.detach()), _bhld_view(k.detach())
+    blocks = torch.empty((B, Hq, -(-Lq // QUERY_BLOCK), min(keep, -(-Lk // KEY_BLOCK))), dtype=torch.int32, device=dev)
+    if blocks.numel() == 0:
+        return blocks
+    a = nv.SelectBlocksArgs(nv.src4(q), nv.src4(k), nv.ptr(lengths), blocks.data_ptr(), B, Hq, Hk, Lq, Lk, keep, always, D)
+    with nv.on_device(dev):
+        need = nv.lib().flux_select_blocks_workspace_bytes(nv.byref(a))
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        rc = nv.lib().flux_select_blocks(nv.byref(a), nv.ptr(ws), need, nv.stream_ptr(dev))
+    nv.check(rc, "flux_select_blocks")
+    return blocks
+
+
+class _block_sparse_attention(torch.autograd.Function):
+    """What operands that require gradients have an edge to: an error, not nothing. Forward-mode derivatives and function transforms are refused as well."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _launch_sparse(*args)
+
+    @staticmethod
+    def backward(ctx, do):
+        raise NotImplementedError("block_sparse_attention is not differentiated")
+
+
+def _launch_sparse(q: Tensor, k: Tensor, v: Tensor, blocks: Tensor, sm_scale: float | None, lengths: Tensor | None, out: Tensor | None) -> Tensor:
+    B, Hq, Hk, Lq, Lk, D = _sparse_shapes("block_sparse_attention", q, k)
+    assert v.shape == k.shape, f"block_sparse_attention: k and v are of one shape, not {tuple(k.shape)} and {tuple(v.shape)}"
+    if q.dtype != torch.bfloat16 or k.dtype != q.dtype or v.dtype != q.dtype or (out is not None and out.dtype != q.dtype):
+        raise TypeError("block_sparse_attention: the HIP kernel takes bfloat16 q, k, v")
+    if blocks.is_floating_point() or blocks.is_complex() or blocks.dtype == torch.bool:
+        raise TypeError(f"unsupported dtype {blocks.dtype} of block numbers")
+    assert blocks.dim() == 4 and blocks.shape[:3] == (B, Hq, -(-Lq // QUERY_BLOCK)), \
+        f"block_sparse_attention: blocks are [{B}, {Hq}, {-(-Lq // QUERY_BLOCK)}, count], not {tuple(blocks.shape)}"
+    dev = nv.require_gpu(q, k, v, blocks, lengths, out)
+    lengths = _lengths(lengths, B, dev, Lk)
+    if blocks.dtype != torch.int32:
+        blocks = blocks.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    blocks = blocks.contiguous()
+    o = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
+    assert o.shape == q.shape and (o.numel() == 0 or o.stride(3) == 1), f"block_sparse_attention: out is {tuple(q.shape)} with contiguous heads"
+    if o.numel() == 0:
+        return o
+    q, k, v = _bhld_view(q), _bhld_view(k), _bhld_view(v)
+    a = nv.SparseAttentionArgs(nv.src4(q), nv.src4(k), nv.src4(v), o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), blocks.data_ptr(), nv.ptr(lengths),
+                               B, Hq, Hk, Lq, Lk, blocks.shape[3], D, 1 / math.sqrt(D) if sm_scale is None else float(sm_scale))
+    with nv.on_device(dev):
+        need = nv.lib().flux_sparse_attention_workspace_bytes(nv.byref(a))
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        rc = nv.lib().flux_sparse_attention_bf16(nv.byref(a), nv.ptr(ws), need, nv.stream_ptr(dev))
+    nv.check(rc, "flux_sparse_attention_bf16")
+    return o
+
+
+def block_sparse_attention(q: Tensor, k: Tensor, v: Tensor, blocks: Tensor, sm_scale: float | None = None, *, lengths: Tensor | None = None, out: Tensor | None = None) -> Tensor:
+    """Attention of each block of 128 queries over the blocks of 64 keys that its list names, [B, Hq, Lq, D] bf16.
+
+    q, k, v  : bf16 [B, Hq, Lq, D] and [B, Hk, Lk, D] views, heads of 64 or 128; Hq is a multiple of Hk, query head h reads key head h // (Hq // Hk)
+    blocks   : whole numbers [B, Hq, ceil(Lq / 128), count], as select_blocks gives them or any others, in any order. A number that is no block of
+               the sequence, -1 for one, names nothing, a number that stands there twice counts twice
+    sm_scale : factor of the scores, 1 / sqrt(D) if None
+    lengths  : whole numbers [B], or None: keys from lengths[b] on are not there
+    out      : where the result goes, a [B, Hq, Lq, D] view with contiguous heads, 16-byte aligned rows and memory of its own
+
+    Rows that see no key are 0. Scores and sums are fp32; q times the scale, and the probabilities, are rounded to bf16 for the matrix cores, as in
+    scaled_dot_product_attention. It is not differentiated: a gradient that reaches it raises NotImplementedError.
+    """
+    if is_dynamo_compiling():
+        return torch.compiler.disable(block_sparse_attention)(q, k, v, blocks, sm_scale, lengths=lengths, out=out)
+    if out is not None:
+        assert not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, out))), "block_sparse_attention: a result that goes to `out` is not differentiated"
+        return _launch_sparse(q, k, v, blocks, sm_scale, lengths, out)
+    return _block_sparse_attention.apply(q, k, v, blocks, sm_scale, lengths, None)
