@@ -30,7 +30,7 @@ typedef struct flux_w4 {
 
 /* y[m] = act(f(x[m]) W^T + bias): x [M, K] bf16 (row stride ldx), bias [N] bf16 or null, y [M, N] bf16 (row stride ldy); act is FLUX_ACT_NONE or
  * FLUX_ACT_GELU_TANH, in_act FLUX_ACT_NONE or (up to 8 rows) FLUX_ACT_SILU, f(x) = x sigmoid(x). fp32 sums, rounded once; f(x) is held to 2^-16 of its
- * value. From some number of rows on the weights are laid out as bf16, each rounded once (2^-9 of it), in the workspace
+ * value. Beyond 128 rows the weights are laid out as bf16, each rounded once (2^-9 of it), in the workspace
  * (flux_linear_w4_workspace_bytes, 0 below; 256-byte aligned, the launch's own until it has run) in front of flux_linear_bf16. */
 typedef struct flux_linear_w4_args {
     const void* x; const void* bias; void* y;

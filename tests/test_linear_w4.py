@@ -61,17 +61,17 @@ def check(got, x, b, q, scale, zero, activation="", in_activation="", rounded=Fa
 @pytest.mark.gpu
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("group,rows,n,k", [(32, 1, 1, 32), (64, 1, 17, 64), (128, 1, 16, 128), (32, 2, 100, 160), (64, 3, 257, 448), (128, 5, 48, 3072), (64, 8, 33, 8256), (32, 9, 130, 96), (128, 15, 31, 640),
-                                            (64, 16, 96, 2048), (32, 17, 64, 4096), (64, 33, 40, 192), (128, 63, 144, 384), (64, 64, 20, 3072), (64, 65, 80, 320), (32, 130, 264, 1056), (128, 257, 128, 1024)])
+                                            (64, 16, 96, 2048), (32, 17, 64, 4096), (64, 33, 40, 192), (128, 63, 144, 384), (64, 64, 20, 3072), (64, 65, 80, 320), (32, 32, 48, 8224), (64, 40, 100, 8256), (128, 128, 2100, 1152), (64, 12, 4200, 1088), (64, 24, 9000, 64), (32, 4, 300, 8192), (64, 100, 9300, 128), (128, 129, 64, 256), (32, 130, 264, 1056), (128, 257, 128, 1024)])
 def test_against_float64(group, rows, n, k, zeros):
     g = seeded(rows * n + k)
     w, q, scale, zero = weights(g, n, k, group, zeros)
     x, b = randn(g, rows, k, dtype=torch.bfloat16), randn(g, n, dtype=torch.bfloat16)
-    check(tk.linear_w4(x.to(DEV), w, b.to(DEV)), x, b, q, scale, zero, rounded=rows > 64)
-    check(tk.linear_w4(x.to(DEV), w, activation="GELU"), x, None, q, scale, zero, "GELU", rounded=rows > 64)
+    check(tk.linear_w4(x.to(DEV), w, b.to(DEV)), x, b, q, scale, zero, rounded=rows > 128)
+    check(tk.linear_w4(x.to(DEV), w, activation="GELU"), x, None, q, scale, zero, "GELU", rounded=rows > 128)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("group,rows,n,k,zeros", [(64, 1, 512, 3072, False), (128, 3, 100, 1024, True), (32, 8, 65, 2080, True), (64, 8, 16, 8256, False), (32, 5, 1, 32, False), (64, 2, 48, 64, True)])
+@pytest.mark.parametrize("group,rows,n,k,zeros", [(64, 1, 512, 3072, False), (128, 3, 100, 1024, True), (32, 8, 65, 2080, True), (64, 8, 16, 8256, False), (32, 5, 1, 32, False), (64, 2, 48, 64, True), (64, 5, 4200, 320, True), (32, 3, 5000, 96, False), (128, 4, 100, 8192, True)])
 def test_silu_on_the_way_in(group, rows, n, k, zeros):
     g = seeded(rows + n + k)
     w, q, scale, zero = weights(g, n, k, group, zeros)
@@ -81,7 +81,7 @@ def test_silu_on_the_way_in(group, rows, n, k, zeros):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [1, 8, 20, 70])
+@pytest.mark.parametrize("rows", [1, 8, 20, 70, 140])
 @pytest.mark.parametrize("silu", [False, True])
 def test_what_is_not_finite_goes_as_in_the_formula(rows, silu):
     if silu and rows > 8:
@@ -137,22 +137,22 @@ def test_rows_are_the_same_whoever_stands_beside_them():
 def test_streams_and_replayed_graphs():
     g = seeded(12)
     w, q, scale, zero = weights(g, 96, 256, 64, False)
-    x = randn(g, 70, 256, dtype=torch.bfloat16).to(DEV)
-    want = [tk.linear_w4(x[:r], w) for r in (1, 40, 70)]
+    x = randn(g, 140, 256, dtype=torch.bfloat16).to(DEV)
+    want = [tk.linear_w4(x[:r], w) for r in (1, 40, 140)]
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
-        other = [tk.linear_w4(x[:r], w) for r in (1, 40, 70)]
+        other = [tk.linear_w4(x[:r], w) for r in (1, 40, 140)]
     stream.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, other))
     graph, again = torch.cuda.CUDAGraph(), x.clone()
     with torch.cuda.graph(graph):
-        out = [tk.linear_w4(again[:r], w) for r in (1, 40, 70)]
+        out = [tk.linear_w4(again[:r], w) for r in (1, 40, 140)]
     for i in range(3):
         again.copy_(x * (i + 1))
         graph.replay()
         torch.cuda.synchronize()
-        assert all(torch.equal(a, tk.linear_w4((x * (i + 1))[:r], w)) for a, r in zip(out, (1, 40, 70)))
+        assert all(torch.equal(a, tk.linear_w4((x * (i + 1))[:r], w)) for a, r in zip(out, (1, 40, 140)))
 
 
 @pytest.mark.gpu
@@ -255,7 +255,7 @@ def test_refusals_of_a_layout():
 
 
 @pytest.mark.parametrize("change,rc", [(dict(x=None), -1), (dict(y=None), -1), (dict(M=-1), -2), (dict(act=2), -6), (dict(in_act=1), -6), (dict(in_act=2, M=9), -6), (dict(M=0, x=None), 0), (dict(x=24), -4),
-                                       (dict(M=2, ldx=65), -4), (dict(M=2, ldy=3), -2), (dict(M=65), -2)])
+                                       (dict(M=2, ldx=65), -4), (dict(M=2, ldy=3), -2), (dict(M=129), -2)])
 def test_refusals_of_the_library(change, rc):
     import ctypes
 

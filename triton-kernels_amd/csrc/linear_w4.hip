@@ -5,12 +5,16 @@
 // Half a byte a weight and two operations a row: up to some dozens of rows bound by the bytes of the weights. A multiplication on the VALU would cost more
 // than they do: 57 M weights are 28 MB, 5.6 us at a copy's rate, and at three instructions a weight (take it out, convert, multiply) 4.4 us of all VALUs for one
 // row. So a weight becomes a bf16 number in one instruction, 16 + q = (q << 3) | 0x4180 for two of them at once, and the matrix cores multiply (16x16x32,
-// x the rows and W the columns of the result, whose 16 rows cost one row's time): the sum that is too much, (16 + z) sum x, is where a group's sum
-// starts. Sums of x by group are formed once, as x goes to LDS. A group's sum takes its scale behind the product, in fp32: nothing is rounded but y.
+// x the rows and W the columns of the result, whose 16 rows cost one row's time). What is too much, (16 + z) times the sum of x, comes from the matrix cores as well,
+// as a product with ones. A group's sum takes its scale behind the product, in fp32: nothing is rounded but y.
+//
+// us among others of its kind: 1 x 18432 x 3072 8.4, with SiLU 10.1 (floor 5.6), 3 x 9216 x 3072 with SiLU 9.6, 1 x 1000 x 1024 3.0 (a launch), 16 x 9216 x 3072 9.0, 24 x 12288
+// x 3072 13.5, 128 x 9216 x 3072 29, 512 x 9216 x 3072 47 (17 of them for laying the weights out).
 #include "common.h"
 #include "../../include/flux_hip_serve.h"
 #include <algorithm>
 #include <math.h>
+#include <type_traits>
 
 namespace flux {
 
@@ -47,113 +51,317 @@ __device__ __forceinline__ w4_bf16x8 w4_unpack_exact(uint32_t w, float z) {
     return r;
 }
 
-// A workgroup of four waves takes 16 outputs of up to 16 rows of x (8 with SPLIT: f(x) as a bf16 number and another one for what that leaves over, in
-// rows 8 beneath). The waves take every fourth chunk of K and add their sums in order.
-// GPC: groups of a chunk.
-template <int GPC, bool ZERO, bool SPLIT>
-__global__ __launch_bounds__(256) void w4_rows_kernel(W4Params p) {
-    constexpr int RB = SPLIT ? 8 : 16, U = 6;
+// The scales (or zero points) of a lane's row in one chunk, as one load.
+template <int BYTES> struct W4Word;
+template <> struct W4Word<1> { typedef uint8_t type; };
+template <> struct W4Word<2> { typedef uint16_t type; };
+template <> struct W4Word<4> { typedef uint32_t type; };
+template <> struct W4Word<8> { typedef uint64_t type; };
+
+// What a wave holds of 16 outputs x 128 columns.
+template <int GPC, bool ZERO> struct W4Piece {
+    w4_u32x4 q;
+    typename W4Word<2 * GPC>::type s;
+    typename W4Word<GPC>::type z;
+    __device__ __forceinline__ float scale(int i) const { return bf2f(static_cast<bf16_t>(s >> (16 * i))); }
+    __device__ __forceinline__ float zero(int i) const { return ZERO ? static_cast<float>(static_cast<uint8_t>(z >> (8 * i))) : 8.0f; }
+};
+// A row tile of W: q at the lane's 16 bytes, s and z at its row.
+template <int GPC, bool ZERO> struct W4Tile {
+    const w4_u32x4* q; const typename W4Word<2 * GPC>::type* s; const typename W4Word<GPC>::type* z;
+    __device__ __forceinline__ W4Tile(const W4Params& p, int tile, int lane) {
+        const int64_t at = static_cast<int64_t>(tile) * p.chunks;
+        q = p.q + at * 64 + lane;
+        s = reinterpret_cast<const typename W4Word<2 * GPC>::type*>(p.s) + at * 16 + (lane & 15);
+        z = ZERO ? reinterpret_cast<const typename W4Word<GPC>::type*>(p.z) + at * 16 + (lane & 15) : nullptr;
+    }
+    template <bool ONCE> __device__ __forceinline__ void request(W4Piece<GPC, ZERO>& to, int c) const {
+        to.q = ONCE ? __builtin_nontemporal_load(q + static_cast<int64_t>(c) * 64) : q[static_cast<int64_t>(c) * 64];
+        to.s = s[c * 16];
+        if (ZERO) to.z = z[c * 16];
+    }
+};
+
+// f(x) = x sigmoid(x) as a bf16 number in x and what it leaves over in lo.
+__device__ __forceinline__ void w4_silu(Vec16<bf16_t>& x, Vec16<bf16_t>& lo) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float f = bf2f(x.v[e]);
+        f = f * __builtin_amdgcn_rcpf(1.0f + __expf(-f));
+        x.v[e] = f2bf(f);
+        lo.v[e] = f2bf(fabsf(f) < INFINITY ? f - bf2f(x.v[e]) : 0.0f);
+    }
+}
+
+// acc += s (q - z) x over one chunk, for MT times 16 rows of x, the lane's `row` bytes behind `a`: the sum of (16 + q) x without (16 + z) times the sum of x, which the
+// matrix cores form beside it. `peak` takes the largest of these sums: what goes with it is lost to 2^-23 of it, and where x is not finite it leaves a NaN or an infinity.
+template <int GPC, bool ZERO, int MT>
+__device__ __forceinline__ void w4_chunk(w4_f32x4 (&acc)[MT], const W4Piece<GPC, ZERO>& w, const char* a, const int (&row)[MT], float& peak) {
+    const w4_f32x4 none = {0.f, 0.f, 0.f, 0.f};
+    const w4_bf16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+#pragma unroll
+    for (int i = 0; i < GPC; ++i) {
+        const float zero = w.zero(i), scale = w.scale(i);
+        w4_f32x4 t[MT], u[MT];
+#pragma unroll
+        for (int j = i * 4 / GPC; j < (i + 1) * 4 / GPC; ++j) {
+            const bool first = j == i * 4 / GPC;
+            const w4_bf16x8 b = w4_unpack(w.q[j]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const w4_bf16x8 x = *reinterpret_cast<const w4_bf16x8*>(a + row[m] + j * 64);
+                t[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, b, first ? none : t[m], 0, 0, 0);
+                u[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, ones, first ? none : u[m], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            peak = fmaxf(fmaxf(peak, fabsf(u[m][0])), fabsf(u[m][1]));
+            peak = fmaxf(fmaxf(peak, fabsf(u[m][2])), fabsf(u[m][3]));
+            acc[m] += (t[m] - u[m] * (16.0f + zero)) * scale;
+        }
+    }
+}
+
+// Whether a lane of the wave holds a sum that is not finite, or had one beyond 2^100 on its way.
+template <int N, int MT> __device__ __forceinline__ bool w4_lost(const w4_f32x4 (&acc)[N][MT], float peak) {
+    bool lost = !(peak < 0x1p100f);
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lost |= !(fabsf(acc[t][m][i]) < INFINITY);
+    return __builtin_amdgcn_ballot_w64(lost) != 0;
+}
+
+// The wave's sums once more, with q - z as it is and x from memory: for rows that are not finite.
+// part, parts: which chunks of K; a row of x: row(m) of the wave's 16 MT, with SPLIT f(x) as in LDS.
+template <bool SPLIT, int GPC, bool ZERO, int MT>
+__device__ __forceinline__ void w4_again(w4_f32x4 (&acc)[MT], const W4Params& p, int tile, int m0, int rows, int part, int parts) {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+    const W4Tile<GPC, ZERO> w(p, tile, lane);
+#pragma unroll 1
+    for (int c = part; c < p.chunks; c += parts) {
+        W4Piece<GPC, ZERO> piece;
+        w.template request<false>(piece, c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = j * GPC / 4, k = c * kW4Chunk + j * 32 + g * 8;
+            const w4_bf16x8 b = w4_unpack_exact(piece.q[j], piece.zero(i));
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const int row = SPLIT ? l16 & 7 : m * 16 + l16;
+                Vec16<bf16_t> x, lo;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x.v[e] = 0;
+                if (k < p.K && row < rows) x = ld16(p.x + static_cast<int64_t>(m0 + row) * p.ldx + k);
+                if (SPLIT) {
+                    w4_silu(x, lo);
+                    if (l16 >= 8) x = lo;
+                }
+                const w4_f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(w4_bf16x8, x), b, w4_f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                acc[m] += t * piece.scale(i);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ bf16_t w4_result(const W4Params& p, float y, float bias) {
+    y += bias;
+    return f2bf(p.act == FLUX_ACT_GELU_TANH ? gelu_tanh_f32(y) : y);
+}
+
+// A workgroup takes 16 NW outputs of up to 16 rows of x (8 with SPLIT: f(x) as a bf16 number and another one for what that leaves over, in
+// rows 8 beneath). KS waves share 16 of them; they take every KS-th chunk of K and add their sums in order. The first vectors of x are asked for in front of the weights: loads
+// return in order, and the weights of a wave can wait in registers while x is on its way through LDS.
+template <int GPC, bool ZERO, bool SPLIT, int NW, int KS>
+__global__ __launch_bounds__(64 * NW * KS, 4) void w4_rows_kernel(W4Params p) {
+    constexpr int RB = SPLIT ? 8 : 16, U = 6, PRE = 2, T = 64 * NW * KS;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
-    const int tile = blockIdx.x, m0 = blockIdx.y * RB, rows = min(RB, p.M - m0), held = SPLIT ? 2 * rows : rows;
+    const int tiles = (p.N + kW4Tile - 1) / kW4Tile, part = wave / NW, tile = min(static_cast<int>(blockIdx.x) * NW + wave % NW, tiles - 1), m0 = blockIdx.y * RB, rows = min(RB, p.M - m0), held = SPLIT ? 2 * rows : rows;
     const int stride = p.slab * (kW4Chunk * 2) + 16;                  // bytes of a row of x in LDS, 16 more against conflicts
-    float* const sums = reinterpret_cast<float*>(lds + held * stride);  // [group of the slab][16]: -sum x
-    int* const odd = reinterpret_cast<int*>(sums + p.slab * GPC * 16);
     // rows of the product without a row of x read the first one; what they sum up is not stored
     const int my_row = l16 < rows ? l16 : (SPLIT && l16 >= 8 && l16 - 8 < rows) ? rows + l16 - 8 : 0;
-    const char* const xrow = lds + my_row * stride + g * 16;
-    const w4_u32x4* const q = p.q + static_cast<int64_t>(tile) * p.chunks * 64 + lane;
-    const bf16_t* const s = p.s + (static_cast<int64_t>(tile) * p.chunks * 16 + l16) * GPC;
-    const uint8_t* const z = ZERO ? p.z + (static_cast<int64_t>(tile) * p.chunks * 16 + l16) * GPC : nullptr;
-    if (tid == 0) *odd = 0;
-    w4_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    w4_u32x4 wq[U];
-    bf16_t ws[U][GPC];
-    uint8_t wz[U][GPC];
+    const int xrow[1] = {my_row * stride + g * 16};
+    const W4Tile<GPC, ZERO> w(p, tile, lane);
+    const int out_n = (blockIdx.x * NW + (tid >> 8)) * kW4Tile + (tid & 15);   // (of the thread's result)
+    const float bias = p.bias != nullptr ? bf2f(p.bias[min(out_n, p.N - 1)]) : 0.0f;
+    w4_f32x4 acc[1][1] = {{{0.f, 0.f, 0.f, 0.f}}};
+    float peak = 0.0f;
+    W4Piece<GPC, ZERO> piece[U];
     for (int c0 = 0; c0 < p.chunks; c0 += p.slab) {
-        const int n = min(p.slab, p.chunks - c0);
-        auto request = [&](int u, int c) {   // (past the end: the slab's first chunk again, not used)
-            const int64_t at = c0 + (c < n ? c : 0);
-            wq[u] = __builtin_nontemporal_load(q + at * 64);
+        const int n = min(p.slab, p.chunks - c0), vectors = rows * n * 16;   // vectors of 8 values of x, 16 a chunk
+        auto load = [&](int i) {
+            const int m = rows == 1 ? 0 : i / (n * 16), v = i - m * (n * 16), k = (c0 * 16 + v) * 8;
+            Vec16<bf16_t> x;
 #pragma unroll
-            for (int i = 0; i < GPC; ++i) {
-                ws[u][i] = s[at * 16 * GPC + i];
-                if (ZERO) wz[u][i] = z[at * 16 * GPC + i];
-            }
+            for (int e = 0; e < 8; ++e) x.v[e] = 0;
+            if (i < vectors && k < p.K) x = ld16(p.x + (m0 + m) * p.ldx + k);
+            return x;
         };
-#pragma unroll
-        for (int u = 0; u < U; ++u) request(u, wave + 4 * u);
-        __syncthreads();   // the slab before is read
-        for (int i = tid; i < rows * n * 16; i += 256) {   // 8 values each; 16 threads a chunk
-            const int m = i / (n * 16), v = i - m * (n * 16), k = (c0 * 16 + v) * 8;
-            Vec16<bf16_t> hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) hi.v[e] = 0;
-            if (k < p.K) hi = ld16(p.x + (m0 + m) * p.ldx + k);
-            float sh = 0.0f, sl = 0.0f;
-            bool far = false;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float f = bf2f(hi.v[e]);
-                if (SPLIT) {
-                    f = f * __builtin_amdgcn_rcpf(1.0f + __expf(-f));
-                    hi.v[e] = f2bf(f);
-                    lo.v[e] = f2bf(fabsf(f) < INFINITY ? f - bf2f(hi.v[e]) : 0.0f);
-                    sl += bf2f(lo.v[e]);
-                }
-                sh += bf2f(hi.v[e]);
-                far |= !(fabsf(f) < 0x1p100f);   // (16 + z) x would leave fp32's range, or is not a number
-            }
-            if (far) *odd = 1;
-            sh = group_sum<16 / GPC>(sh);
+        auto stage = [&](int i, Vec16<bf16_t> hi) {
+            const int m = rows == 1 ? 0 : i / (n * 16), v = i - m * (n * 16);
+            Vec16<bf16_t> lo;
+            if (SPLIT) w4_silu(hi, lo);
             *reinterpret_cast<Vec16<bf16_t>*>(lds + m * stride + v * 16) = hi;
-            if (v % (16 / GPC) == 0) sums[v / (16 / GPC) * 16 + m] = -sh;
-            if (SPLIT) {
-                sl = group_sum<16 / GPC>(sl);
-                *reinterpret_cast<Vec16<bf16_t>*>(lds + (rows + m) * stride + v * 16) = lo;
-                if (v % (16 / GPC) == 0) sums[v / (16 / GPC) * 16 + 8 + m] = -sl;
-            }
-        }
+            if (SPLIT) *reinterpret_cast<Vec16<bf16_t>*>(lds + (rows + m) * stride + v * 16) = lo;
+        };
+        Vec16<bf16_t> x[PRE];
+#pragma unroll
+        for (int j = 0; j < PRE; ++j) x[j] = load(tid + j * T);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) w.template request<true>(piece[u], c0 + min(part + KS * u, n - 1));   // (past the end: not used)
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();   // the slab before is read
+#pragma unroll
+        for (int j = 0; j < PRE; ++j)
+            if (tid + j * T < vectors) stage(tid + j * T, x[j]);
+        for (int i = tid + PRE * T; i < vectors; i += T) stage(i, load(i));
         __syncthreads();
-        const bool exact = *odd != 0;
-        for (int base = wave; base < n; base += 4 * U) {
+        for (int base = part; base < n; base += KS * U)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int c = base + 4 * u;
-                if (c < n) {
+                const int c = base + KS * u;
+                if (c >= n) break;
+                w4_chunk<GPC, ZERO, 1>(acc[0], piece[u], lds + c * (kW4Chunk * 2), xrow, peak);
+                if (c + KS * U < n) w.template request<true>(piece[u], c0 + c + KS * U);
+            }
+    }
+    if (__builtin_expect(w4_lost(acc, peak), 0)) w4_again<SPLIT, GPC, ZERO, 1>(acc[0], p, tile, m0, rows, part, KS);
+    __syncthreads();
+    float* const parts = reinterpret_cast<float*>(lds);   // [wave][lane][4]
+    *reinterpret_cast<w4_f32x4*>(parts + tid * 4) = acc[0][0];
+    __syncthreads();
+    const int m = (tid >> 4) & 15;
+    if (tid >= NW * 256 || m >= rows || out_n >= p.N) return;
+    float y = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < GPC; ++i) {
-                        const float zero = ZERO ? static_cast<float>(wz[u][i]) : 8.0f;
-                        w4_f32x4 t = *reinterpret_cast<const w4_f32x4*>(sums + (c * GPC + i) * 16 + g * 4) * (16.0f + zero);
-                        if (exact) t = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < KS; ++i) {
+        y += parts[((i * NW + (tid >> 8)) * 64 + (m >> 2) * 16 + (tid & 15)) * 4 + (m & 3)];
+        if (SPLIT) y += parts[((i * NW + (tid >> 8)) * 64 + ((m + 8) >> 2) * 16 + (tid & 15)) * 4 + (m & 3)];
+    }
+    p.y[(m0 + m) * p.ldy + out_n] = w4_result(p, y, bias);
+}
+
+// x straight to LDS, 64 x 16 bytes, asked for behind the compiler's back: it would wait for every such load in front of every read of LDS. The kernel waits for
+// them itself. What lies past the descriptor's end arrives as zeros.
+__device__ __forceinline__ void w4_load_lds(w4_u32x4 rsrc, uint32_t lds_addr, uint32_t voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds_addr), "v"(voff), "s"(rsrc) : "memory", "m0");
+}
+
+// More rows: up to 16 MT of them a workgroup, whose waves are NW groups of 16 NTW outputs times KS parts of K. A wave keeps CW chunks of weights on
+// their way. x goes through LDS, all of K at once where it fits, or in slabs of p.slab chunks, the next one on its way while one is multiplied.
+template <int GPC, bool ZERO, int MT, int NTW, int NW, int KS, int CW>
+__global__ __launch_bounds__(64 * NW * KS) void w4_tiles_kernel(W4Params p) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    constexpr int RB = 16 * MT, WAVES = NW * KS;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
+    const int nw = wave % NW, part = wave / NW, m0 = blockIdx.y * RB, rows = min(RB, p.M - m0);
+    const int tiles = (p.N + kW4Tile - 1) / kW4Tile, tile0 = (blockIdx.x * NW + nw) * NTW;
+    const int stride = p.slab * (kW4Chunk * 2) + 16, buffer = rows * stride, pieces = p.slab / 4;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)lds));
+    auto load_x = [&](int slab) {
+        for (int i = wave; i < rows * pieces; i += WAVES) {
+            const int m = i / pieces, piece = i - m * pieces;
+            const uint64_t at = reinterpret_cast<uint64_t>(p.x + static_cast<int64_t>(m0 + m) * p.ldx);
+            w4_u32x4 r;
+            r.x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
+            r.y = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32) & 0xffffu);
+            r.z = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(p.K) * 2u);
+            r.w = 0x00020000u;
+            w4_load_lds(r, __builtin_amdgcn_readfirstlane(lds0 + (slab & 1) * buffer + m * stride + piece * 1024), static_cast<uint32_t>(slab * p.slab * (kW4Chunk * 2) + piece * 1024 + lane * 16));
+        }
+    };
+    w4_f32x4 acc[NTW][MT];
 #pragma unroll
-                        for (int j = i * 4 / GPC; j < (i + 1) * 4 / GPC; ++j) {
-                            const w4_bf16x8 a = *reinterpret_cast<const w4_bf16x8*>(xrow + c * (kW4Chunk * 2) + j * 64);
-                            const w4_bf16x8 b = exact ? w4_unpack_exact(wq[u][j], zero) : w4_unpack(wq[u][j]);
-                            t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, t, 0, 0, 0);
-                        }
-                        acc += t * bf2f(ws[u][i]);
-                    }
+    for (int t = 0; t < NTW; ++t)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[t][m] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+    float peak = 0.0f;
+    W4Piece<GPC, ZERO> piece[NTW][CW];
+    auto load_w = [&](W4Piece<GPC, ZERO>& to, int t, int chunk) {   // (past the end: not used)
+        W4Tile<GPC, ZERO>(p, min(tile0 + t, tiles - 1), lane).template request<false>(to, min(chunk, p.chunks - 1));
+    };
+    load_x(0);
+#pragma unroll
+    for (int c = 0; c < CW; ++c)
+#pragma unroll
+        for (int t = 0; t < NTW; ++t) load_w(piece[t][c], t, c * KS + part);
+    // rows of the product without a row of x read the first one; what they sum up is not stored
+    int row[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) row[m] = (m * 16 + l16 < rows ? m * 16 + l16 : 0) * stride + g * 16;
+    const int per = p.slab / KS, steps = (p.chunks + KS - 1) / KS;   // a wave's chunks of a slab, and of all
+    const char* x = lds;
+    auto open = [&](int slab) {   // what was asked for has landed, and the slab before is read
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if ((slab + 1) * p.slab < p.chunks) load_x(slab + 1);
+        x = lds + (slab & 1) * buffer;
+    };
+    int next = 0;   // the step at which a slab begins
+    for (int base = 0; base < steps; base += CW) {
+#pragma unroll
+        for (int c = 0; c < CW; ++c) {
+            const int step = base + c;
+            if (step < steps) {
+                if (step == next) {
+                    open(step / per);
+                    next += per;
                 }
-                request(u, c + 4 * U);
+                const int chunk = step * KS + part, at = chunk % p.slab;
+                if (chunk < p.chunks) {
+#pragma unroll
+                    for (int t = 0; t < NTW; ++t) w4_chunk<GPC, ZERO, MT>(acc[t], piece[t][c], x + at * (kW4Chunk * 2), row, peak);
+                }
+#pragma unroll
+                for (int t = 0; t < NTW; ++t) load_w(piece[t][c], t, (step + CW) * KS + part);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
-    __syncthreads();
-    float* const parts = reinterpret_cast<float*>(lds);   // [wave][lane][4]
-    *reinterpret_cast<w4_f32x4*>(parts + tid * 4) = acc;
-    __syncthreads();
-    const int m = tid >> 4, col = tid & 15, nn = tile * kW4Tile + col;
-    if (m >= rows || nn >= p.N) return;
-    float y = 0.0f;
+    if (__builtin_expect(w4_lost(acc, peak), 0))
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        y += parts[(w * 64 + (m >> 2) * 16 + col) * 4 + (m & 3)];
-        if (SPLIT) y += parts[(w * 64 + ((m + 8) >> 2) * 16 + col) * 4 + (m & 3)];
+        for (int t = 0; t < NTW; ++t) w4_again<false, GPC, ZERO, MT>(acc[t], p, min(tile0 + t, tiles - 1), m0, rows, part, KS);
+    if constexpr (KS > 1) {   // the parts' sums, in order
+        __syncthreads();
+        float* const parts = reinterpret_cast<float*>(lds);
+        auto at = [&](int from, int t, int m) { return reinterpret_cast<w4_f32x4*>(parts + ((((from - 1) * NW + nw) * NTW + t) * MT + m) * 256 + lane * 4); };
+        if (part > 0)
+#pragma unroll
+            for (int t = 0; t < NTW; ++t)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) *at(part, t, m) = acc[t][m];
+        __syncthreads();
+        if (part > 0) return;
+#pragma unroll
+        for (int t = 0; t < NTW; ++t)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 1; i < KS; ++i) acc[t][m] += *at(i, t, m);
     }
-    if (p.bias != nullptr) y += bf2f(p.bias[nn]);
-    if (p.act == FLUX_ACT_GELU_TANH) y = gelu_tanh_f32(y);
-    p.y[(m0 + m) * p.ldy + nn] = f2bf(y);
+#pragma unroll
+    for (int t = 0; t < NTW; ++t) {
+        const int n = (tile0 + t) * kW4Tile + l16;
+        const float bias = p.bias != nullptr && n < p.N ? bf2f(p.bias[n]) : 0.0f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = m * 16 + g * 4 + i;
+                if (r < rows && n < p.N) p.y[static_cast<int64_t>(m0 + r) * p.ldy + n] = w4_result(p, acc[t][m][i], bias);
+            }
+    }
+}
+// bytes of LDS: x, one slab or two, or the parts' sums
+static int w4_tiles_lds(const W4Params& p, int held, int parts_kb) {
+    const int slabs = (p.chunks + p.slab - 1) / p.slab;
+    return std::max((slabs > 1 ? 2 : 1) * held * (p.slab * kW4Chunk * 2 + 16), parts_kb * 1024);
 }
 
 // W as bf16 [N, K], (q - z) s rounded once. A wave takes a tile; a lane's row is written as four pieces of 16 bytes.
@@ -215,20 +423,59 @@ static void w4_unpack_any(const flux_w4& w, void* out, hipStream_t st) {
     else w4_unpack_launch<1>(w, out, st);
 }
 
-template <int GPC>
+template <int GPC, bool ZERO>
 static void w4_rows_launch(W4Params p, hipStream_t st) {
-    const int rb = p.silu ? 8 : 16, held = std::min(p.M, rb) * (p.silu ? 2 : 1);
-    // up to 48 KB of x, so that three workgroups share a CU
-    p.slab = std::min({p.chunks, 64, 48 * 1024 / (held * kW4Chunk * 2) / 4 * 4});
-    const int bytes = std::max(held * (p.slab * kW4Chunk * 2 + 16) + p.slab * GPC * 64 + 16, 4096);
-    const dim3 grid(static_cast<unsigned>((p.N + kW4Tile - 1) / kW4Tile), static_cast<unsigned>((p.M + rb - 1) / rb));
-#define CALL(ZERO, SPLIT) hipLaunchKernelGGL((w4_rows_kernel<GPC, ZERO, SPLIT>), grid, dim3(256), bytes, st, p)
-    if (p.z) { if (p.silu) CALL(true, true); else CALL(true, false); }
-    else { if (p.silu) CALL(false, true); else CALL(false, false); }
+    const int tiles = (p.N + kW4Tile - 1) / kW4Tile;
+    const bool few = tiles <= 256;   // no more than a row tile a CU
+    // Up to 4 rows, f(x), and up to 8 rows of few outputs: x through registers. Two row tiles a wave group or more make the work on x less (3 x 9216 x 3072 with SiLU
+    // 10.0 -> 9.5 us, 4 rows 11.8 -> 9.9) and the launch longer (1 x 18432 x 3072 10.1 -> 15.9, 1 x 9216 7.5 -> 9.1); eight parts of K pay where there are few
+    // outputs and many chunks (2 x 4096 x 8192 10.8 -> 7.7, 8 x 3072 x 3072 6.8 -> 5.6; 1 x 18432 x 3072 10.1 -> 13.7) or many rows.
+    if (p.M <= 4 || p.silu || (p.M <= 8 && few)) {
+        const int rb = p.silu ? 8 : 16, held = std::min(p.M, rb) * (p.silu ? 2 : 1);
+        p.slab = std::min({p.chunks, 64, 48 * 1024 / (held * kW4Chunk * 2) / 4 * 4});   // up to 48 KB of x, so that three workgroups share a CU
+        auto call = [&](auto kernel, int nw, int ks) {
+            const int bytes = std::max(held * (p.slab * kW4Chunk * 2 + 16), 1024 * nw * ks);
+            hipLaunchKernelGGL(kernel, dim3((tiles + nw - 1) / nw, (p.M + rb - 1) / rb), dim3(64 * nw * ks), bytes, st, p);
+        };
+#define CALL(NW, KS) if (p.silu) call(w4_rows_kernel<GPC, ZERO, true, NW, KS>, NW, KS); else call(w4_rows_kernel<GPC, ZERO, false, NW, KS>, NW, KS)
+        if (few && (p.chunks >= 32 || p.M > 4)) { CALL(1, 8); }
+        else if (p.silu && p.M >= 3 && !few) call(w4_rows_kernel<GPC, ZERO, true, 4, 4>, 4, 4);
+        else { CALL(1, 4); }
+#undef CALL
+        return;
+    }
+    // More: x fills the LDS of a CU at K = 3072, so workgroups run in rounds of 256. What a round takes there, us, by the rows and row tiles of a workgroup; the form
+    // whose rounds take least: 16 x 9216 9.3 (16 rows, 4 tiles), 24 x 3072 8.5 (32 rows, 2 tiles), 24 x 12288 13.4 (32, 4), 64 x 12288 21.2 (64, 4; 24.8 with
+    // 32, 4), 128 x 12288 29.2 (64, 8; 33.9 with 32, 4), 128 x 3072 12.4 (32, 4).
+    struct Form { int rows, tiles; float us; };
+    static const Form forms[] = {{16, 2, 6.5f}, {16, 4, 9.0f}, {32, 2, 8.5f}, {32, 4, 12.4f}, {64, 4, 19.5f}, {64, 8, 28.5f}};
+    int best = 0;
+    float best_us = 0.0f;
+    for (int i = 0; i < 6; ++i) {
+        const int64_t groups = static_cast<int64_t>((tiles + forms[i].tiles - 1) / forms[i].tiles) * ((p.M + forms[i].rows - 1) / forms[i].rows);
+        const float us = static_cast<float>((groups + 255) / 256) * forms[i].us;
+        if (i == 0 || us < best_us) { best = i; best_us = us; }
+    }
+    auto call = [&](auto kernel, int mt, int ntw, int nw, int ks) {
+        const int held = std::min(p.M, 16 * mt), most = 152 * 1024;
+        const int unit = std::max(4, ks);   // chunks: whole loads of 1 KB of a row, and as many for each part
+        p.slab = (p.chunks + unit - 1) / unit * unit;
+        if (held * (p.slab * kW4Chunk * 2 + 16) > most) p.slab = (most / 2 / held - 16) / (kW4Chunk * 2) / unit * unit;
+        hipLaunchKernelGGL(kernel, dim3((tiles + nw * ntw - 1) / (nw * ntw), (p.M + 16 * mt - 1) / (16 * mt)), dim3(64 * nw * ks), w4_tiles_lds(p, held, (ks - 1) * nw * ntw * mt), st, p);
+    };
+#define CALL(MT, NTW, NW, KS, CW) call(w4_tiles_kernel<GPC, ZERO, MT, NTW, NW, KS, CW>, MT, NTW, NW, KS)
+    switch (best) {
+        case 0: CALL(1, 1, 2, 4, 6); break;
+        case 1: CALL(1, 1, 4, 4, 6); break;
+        case 2: CALL(2, 1, 2, 4, 6); break;
+        case 3: CALL(2, 1, 4, 4, 6); break;
+        case 4: CALL(4, 2, 2, 4, 3); break;
+        default: CALL(4, 2, 4, 2, 3); break;
+    }
 #undef CALL
 }
 
-constexpr int kW4MostRows = 64;   // beyond them the weights are laid out first
+constexpr int kW4MostRows = 128;   // beyond them the weights are laid out first
 
 static flux_linear_args w4_linear(const flux_linear_w4_args& a, const void* w) {
     flux_linear_args l = {};
@@ -292,8 +539,10 @@ extern "C" int flux_linear_w4_bf16(const flux_linear_w4_args* a, void* ws, int64
     W4Params p = {static_cast<const bf16_t*>(a->x), static_cast<const w4_u32x4*>(a->w.q), static_cast<const bf16_t*>(a->w.s), static_cast<const uint8_t*>(a->w.z),
                   static_cast<const bf16_t*>(a->bias), static_cast<bf16_t*>(a->y), a->M > 1 ? a->ldx : 0, a->M > 1 ? a->ldy : 0,
                   static_cast<int>(a->M), static_cast<int>(a->w.N), static_cast<int>(a->w.K), static_cast<int>((a->w.K + kW4Chunk - 1) / kW4Chunk), 0, a->act, a->in_act == FLUX_ACT_SILU};
-    if (a->w.group == 32) w4_rows_launch<4>(p, st);
-    else if (a->w.group == 64) w4_rows_launch<2>(p, st);
-    else w4_rows_launch<1>(p, st);
+#define CALL(GPC) if (p.z) w4_rows_launch<GPC, true>(p, st); else w4_rows_launch<GPC, false>(p, st)
+    if (a->w.group == 32) { CALL(4); }
+    else if (a->w.group == 64) { CALL(2); }
+    else { CALL(1); }
+#undef CALL
     return check_launch(what);
 }
