@@ -29,10 +29,12 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <optional>
 #include <string>
 
 #include "../../include/flux_hip.h"
+#include "../../include/flux_hip_serve.h"
 #include "../../include/flux_hip_tune.h"
 
 namespace {
@@ -1103,9 +1105,123 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- serving with less to read and to multiply -------------------------------------------------
+// (calls that are recorded for a backward pass, and lengths and lists of other types, are the launchers')
+
+bool recorded(std::initializer_list<const Tensor*> operands) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : operands)
+        if (t && t->requires_grad()) return true;
+    return false;
+}
+
+// int32 numbers beside `beside`, or none
+bool numbers(const Tensor* t, const Tensor& beside) { return !t || (t->scalar_type() == at::kInt && t->device() == beside.device() && t->is_contiguous()); }
+
+// linear_w4(x, packed, scale, zero or None, b or None, N, K, group, activation, in_activation)
+PyObject* py_linear_w4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(nargs == 10, "linear_w4 takes 10 arguments");
+    const Tensor *x = tensor_of(args[0]), *q = tensor_of(args[1]), *s = tensor_of(args[2]), *z, *b;
+    int64_t N, K, group, act, in_act, M, ld;
+    if (!x || !q || !s || !optional_tensor(args[3], z) || !optional_tensor(args[4], b) || !whole_number(args[5], N) || !whole_number(args[6], K) || !whole_number(args[7], group) ||
+        !whole_number(args[8], act) || !whole_number(args[9], in_act) || !quiet() || recorded({x, b}) || x->scalar_type() != at::kBFloat16 || !flat_rows(*x, K, M, ld) ||
+        q->device() != x->device() || s->device() != x->device() || (z && z->device() != x->device()) || (b && (!is_bf16(*b, *x) || b->dim() != 1 || b->numel() != N || b->stride(0) != 1)))
+        Py_RETURN_NONE;
+    Tensor y;
+    int rc;
+    {
+        const Tensor xa = *x, qa = *q, sa = *s, za = z ? *z : Tensor(), ba = b ? *b : Tensor();
+        const WithoutInterpreter free;
+        const c10::DeviceGuard guard(xa.device());
+        at::DimVector sizes(xa.sizes().begin(), xa.sizes().end());
+        sizes.back() = N;
+        y = empty(sizes, at::kBFloat16, xa);
+        const flux_linear_w4_args a = {xa.data_ptr(), ba.defined() ? ba.data_ptr() : nullptr, y.data_ptr(),
+                                       {qa.data_ptr(), sa.data_ptr(), za.defined() ? za.data_ptr() : nullptr, N, K, static_cast<int32_t>(group)},
+                                       M, M > 1 ? ld : K, N, static_cast<int32_t>(act), static_cast<int32_t>(in_act)};
+        const int64_t need = flux_linear_w4_workspace_bytes(&a);
+        const Tensor ws = need ? empty({need}, at::kByte, xa) : Tensor();
+        rc = flux_linear_w4_bf16(&a, need ? ws.data_ptr() : nullptr, need, stream_of(xa));
+    }
+    if (rc < 0) Py_RETURN_NONE;   // (a refusal: its kind of error is the launcher's)
+    check(rc, "flux_linear_w4_bf16");
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// [B, H, L, D] views of one batch and head dim in 16-byte rows, whole groups of query heads a head of keys
+bool sparse_views(const Tensor& q, const Tensor& k) {
+    return q.dim() == 4 && k.dim() == 4 && q.scalar_type() == at::kBFloat16 && same_kind(q, k) && q.size(0) == k.size(0) && q.size(3) == k.size(3) && q.size(1) % k.size(1) == 0 && q.stride(3) == 1 &&
+           k.stride(3) == 1 && vector_rows(q) && vector_rows(k);
+}
+constexpr int64_t blocks_of(int64_t n, int64_t size) { return (n + size - 1) / size; }
+
+// select_blocks(q, k, keep, always, lengths or None)
+PyObject* py_select_blocks(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(nargs == 5, "select_blocks takes 5 arguments");
+    const Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *lengths;
+    int64_t keep, always;
+    if (!q || !k || !whole_number(args[2], keep) || !whole_number(args[3], always) || !optional_tensor(args[4], lengths) || !quiet() || !sparse_views(*q, *k) || keep <= 0 ||
+        !numbers(lengths, *q) || (lengths && (lengths->dim() != 1 || lengths->numel() != q->size(0))))
+        Py_RETURN_NONE;
+    Tensor blocks;
+    int rc;
+    {
+        const Tensor qa = *q, ka = *k, la = lengths ? *lengths : Tensor();
+        const WithoutInterpreter free;
+        const c10::DeviceGuard guard(qa.device());
+        blocks = empty({qa.size(0), qa.size(1), blocks_of(qa.size(2), FLUX_QUERY_BLOCK), std::min(keep, blocks_of(ka.size(2), FLUX_KEY_BLOCK))}, at::kInt, qa);
+        const flux_select_blocks_args a = {source(qa), source(ka), la.defined() ? static_cast<const int32_t*>(la.data_ptr()) : nullptr, static_cast<int32_t*>(blocks.data_ptr()),
+                                           qa.size(0), qa.size(1), ka.size(1), qa.size(2), ka.size(2), keep, always, static_cast<int32_t>(qa.size(3))};
+        const int64_t need = flux_select_blocks_workspace_bytes(&a);
+        const Tensor ws = need ? empty({need}, at::kByte, qa) : Tensor();
+        rc = flux_select_blocks(&a, need ? ws.data_ptr() : nullptr, need, stream_of(qa));
+    }
+    if (rc < 0) Py_RETURN_NONE;
+    check(rc, "flux_select_blocks");
+    return THPVariable_Wrap(blocks);
+    END_HANDLE_TH_ERRORS
+}
+
+// block_sparse_attention(q, k, v, blocks, scale or None, lengths or None, out or None)
+PyObject* py_block_sparse_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(nargs == 7, "block_sparse_attention takes 7 arguments");
+    const Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *v = tensor_of(args[2]), *blocks = tensor_of(args[3]), *lengths, *out;
+    if (!q || !k || !v || !blocks || !optional_tensor(args[5], lengths) || !optional_tensor(args[6], out) || !quiet() || recorded({q, k, v, out}) || !sparse_views(*q, *k) || !sparse_views(*q, *v) ||
+        k->sizes() != v->sizes() || !numbers(blocks, *q) || blocks->dim() != 4 || blocks->size(0) != q->size(0) || blocks->size(1) != q->size(1) ||
+        blocks->size(2) != blocks_of(q->size(2), FLUX_QUERY_BLOCK) || !numbers(lengths, *q) || (lengths && (lengths->dim() != 1 || lengths->numel() != q->size(0))) ||
+        (out && (out->sizes() != q->sizes() || !same_kind(*q, *out) || out->stride(3) != 1)))
+        Py_RETURN_NONE;
+    double scale = 1.0 / std::sqrt(static_cast<double>(q->size(3)));
+    if (args[4] != Py_None && !number(args[4], scale)) Py_RETURN_NONE;
+    Tensor o;
+    int rc;
+    {
+        const Tensor qa = *q, ka = *k, va = *v, ba = *blocks, la = lengths ? *lengths : Tensor();
+        if (out) o = *out;
+        const WithoutInterpreter free;
+        const c10::DeviceGuard guard(qa.device());
+        if (!out) o = empty(qa.sizes(), at::kBFloat16, qa);
+        const flux_sparse_attention_args a = {source(qa), source(ka), source(va), o.data_ptr(), o.stride(0), o.stride(1), o.stride(2), static_cast<const int32_t*>(ba.data_ptr()),
+                                              la.defined() ? static_cast<const int32_t*>(la.data_ptr()) : nullptr, qa.size(0), qa.size(1), ka.size(1), qa.size(2), ka.size(2), ba.size(3),
+                                              static_cast<int32_t>(qa.size(3)), static_cast<float>(scale)};
+        const int64_t need = flux_sparse_attention_workspace_bytes(&a);
+        const Tensor ws = need ? empty({need}, at::kByte, qa) : Tensor();
+        rc = flux_sparse_attention_bf16(&a, need ? ws.data_ptr() : nullptr, need, stream_of(qa));
+    }
+    if (rc < 0) Py_RETURN_NONE;
+    check(rc, "flux_sparse_attention_bf16");
+    return THPVariable_Wrap(o);
+    END_HANDLE_TH_ERRORS
+}
+
 #define FLUX_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FLUX_METHOD(rms_norm), FLUX_METHOD(rms_norm_pair), FLUX_METHOD(layer_norm), FLUX_METHOD(layer_norm_modulation), FLUX_METHOD(layer_norm_modulation_pair), FLUX_METHOD(apply_rope), FLUX_METHOD(apply_rope_nd), FLUX_METHOD(rope_table),
-                         FLUX_METHOD(qkv_prep), FLUX_METHOD(linear), FLUX_METHOD(linear_into), FLUX_METHOD(linear_pair_into), FLUX_METHOD(linear_lora), FLUX_METHOD(attention), {nullptr, nullptr, 0, nullptr}};
+                         FLUX_METHOD(qkv_prep), FLUX_METHOD(linear), FLUX_METHOD(linear_into), FLUX_METHOD(linear_pair_into), FLUX_METHOD(linear_lora), FLUX_METHOD(attention),
+                         FLUX_METHOD(linear_w4), FLUX_METHOD(select_blocks), FLUX_METHOD(block_sparse_attention), {nullptr, nullptr, 0, nullptr}};
 #undef FLUX_METHOD
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -122,6 +122,9 @@ def select_blocks(q: Tensor, k: Tensor, keep: int, *, always: int = 0, lengths: 
     """
     if is_dynamo_compiling():
         return torch.compiler.disable(select_blocks)(q, k, keep, always=always, lengths=lengths)
+    blocks = nv.ops().select_blocks(q, k, keep, always, lengths)
+    if blocks is not None:
+        return blocks
     B, Hq, Hk, Lq, Lk, D = _sparse_shapes("select_blocks", q, k)
     if q.dtype != torch.bfloat16 or k.dtype != q.dtype:
         raise TypeError("select_blocks: the HIP kernel takes bfloat16 q, k")
@@ -198,6 +201,9 @@ def block_sparse_attention(q: Tensor, k: Tensor, v: Tensor, blocks: Tensor, sm_s
     """
     if is_dynamo_compiling():
         return torch.compiler.disable(block_sparse_attention)(q, k, v, blocks, sm_scale, lengths=lengths, out=out)
+    o = nv.ops().block_sparse_attention(q, k, v, blocks, sm_scale, lengths, out)
+    if o is not None:
+        return o
     if out is not None:
         assert not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, out))), "block_sparse_attention: a result that goes to `out` is not differentiated"
         return _launch_sparse(q, k, v, blocks, sm_scale, lengths, out)

@@ -372,11 +372,16 @@ def linear_w4(x: Tensor, w: W4, b: Tensor | None = None, *, activation: str = ""
     activation    : "" or "GELU", as in linear
     in_activation : "SiLU" applies x * sigmoid(x) to x on the way in; at most 8 rows
 
-    Sums are fp32 and y is rounded once; up to 64 rows the weights are what the numbers stand for, beyond them they are laid out as bf16 first, each rounded
+    Sums are fp32 and y is rounded once; up to 128 rows the weights are what the numbers stand for, beyond them they are laid out as bf16 first, each rounded
     once. x * sigmoid(x) keeps 16 bits. What is not finite in x goes as in the formula. It is not differentiated: a gradient that reaches it raises NotImplementedError.
     """
     if is_dynamo_compiling():
         return torch.compiler.disable(linear_w4)(x, w, b, activation=activation, in_activation=in_activation)
+    act, in_act = _ACTIVATIONS.get(activation), _IN_ACTIVATIONS.get(in_activation)
+    if act is not None and in_act is not None and launch_hook is None:
+        y = nv.ops().linear_w4(x, w.packed, w.scale, w.zero, b, *w.shape, w.group, act, in_act)
+        if y is not None:
+            return y
     return _linear_w4.apply(x, b, w, activation, in_activation)
 
 
