@@ -8,6 +8,7 @@
 #include "common.h"
 #include "../../include/flux_hip_serve.h"
 #include <algorithm>
+#include <math.h>
 
 namespace flux {
 
@@ -68,81 +69,150 @@ __device__ __forceinline__ uint64_t select_rank(double s) {
     return (u >> 63) ? ~u : u | (uint64_t{1} << 63);
 }
 
-// The numbers of the `keep` largest of key[0 .. n) in ascending order, the lower number among equals, by one wave. The keep-th largest is found bit by bit: the
-// count of keys at or above a candidate says whether that bit is one of its own. Most rows are done once as many keys as are wanted are left.
-template <typename Keys>
-__device__ __forceinline__ void select_largest(const Keys key, int n, int keep, int lane, int32_t* out, int width) {
-    uint64_t floor_ = 0;
-    bool exact = n <= keep;   // whether the keys at or above floor_ are what is wanted
-    for (int bit = 63; bit >= 0 && !exact; --bit) {
-        const uint64_t candidate = floor_ | (uint64_t{1} << bit);
-        int count = 0;
-        for (int i = 0; i < n; i += 64) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i + lane < n && key[i + lane] >= candidate));
-        if (count >= keep) floor_ = candidate;
-        exact = count == keep;
-    }
-    int ties = 0x7fffffff;   // how many of the keys equal to floor_
-    if (!exact) {
-        ties = keep;
-        for (int i = 0; i < n; i += 64) ties -= __builtin_popcountll(__builtin_amdgcn_ballot_w64(i + lane < n && key[i + lane] > floor_));
-    }
+// The numbers of the first `always` scores and of the largest of the others, `keep` in all, of score[0 .. n) in ascending order to `out`, -1 behind them, by one wave.
+struct SelectRow {
+    int32_t* out;
+    int n, keep, always, width, lane;
     int written = 0;
-    const uint64_t below = (uint64_t{1} << lane) - 1;
-    for (int i = 0; i < n; i += 64) {
-        const uint64_t k = i + lane < n ? key[i + lane] : 0;
-        const uint64_t equal = __builtin_amdgcn_ballot_w64(i + lane < n && k == floor_);
-        const bool mine = i + lane < n && (k > floor_ || (k == floor_ && __builtin_popcountll(equal & below) < ties));
-        ties -= ties == 0x7fffffff ? 0 : min(ties, __builtin_popcountll(equal));
+    __device__ __forceinline__ void take(int i, bool mine) {   // of the 64 scores from i on
         const uint64_t chosen = __builtin_amdgcn_ballot_w64(mine);
-        if (mine) out[written + __builtin_popcountll(chosen & below)] = i + lane;
+        if (mine) out[written + __builtin_popcountll(chosen & ((uint64_t{1} << lane) - 1))] = i + lane;
         written += __builtin_popcountll(chosen);
     }
-    for (int i = written + lane; i < width; i += 64) out[i] = -1;
+    __device__ __forceinline__ void rest() const {
+        for (int i = written + lane; i < width; i += 64) out[i] = -1;
+    }
+};
+
+// Among equals the lower number. The rest-th largest score is found bit by bit: the count of scores at or above a candidate says whether that bit is one of its own.
+__device__ __forceinline__ void select_by_bits(SelectRow row, const double* score) {
+    const int rest = row.keep - row.always, lane = row.lane;
+    auto rank = [&](int i) { return i + lane >= row.always && i + lane < row.n ? select_rank(score[i + lane]) : 0; };
+    auto there = [&](int i) { return i + lane >= row.always && i + lane < row.n; };
+    uint64_t floor_ = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+        const uint64_t candidate = floor_ | (uint64_t{1} << bit);
+        int count = 0;
+        for (int i = 0; i < row.n; i += 64) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there(i) && rank(i) >= candidate));
+        if (count >= rest) floor_ = candidate;
+    }
+    int ties = rest;   // how many of those equal to floor_
+    for (int i = 0; i < row.n; i += 64) ties -= __builtin_popcountll(__builtin_amdgcn_ballot_w64(there(i) && rank(i) > floor_));
+    for (int i = 0; i < row.n; i += 64) {
+        const uint64_t equal = __builtin_amdgcn_ballot_w64(there(i) && rank(i) == floor_);
+        const bool tied = (equal >> lane & 1) && __builtin_popcountll(equal & ((uint64_t{1} << lane) - 1)) < ties;
+        row.take(i, i + lane < row.always || (there(i) && rank(i) > floor_) || tied);
+        ties -= min(ties, __builtin_popcountll(equal));
+    }
+    row.rest();
+}
+
+// The same for up to 64 V scores, which a lane holds rounded to fp32. Rounding keeps their order, so a bound that as many of them reach as are wanted parts the
+// scores themselves, and halving the range finds one in a dozen steps (512 scores: 64 bits one by one took 5 us a row). Where two scores on either side of the border
+// are one number in fp32, or something is not finite, there is no such bound.
+template <int V>
+__device__ __forceinline__ void select_by_bound(SelectRow row, const double* score) {
+    const int rest = row.keep - row.always, lane = row.lane;
+    float f[V];
+    float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int i = v * 64 + lane;
+        const bool there = i >= row.always && i < row.n;
+        f[v] = there ? static_cast<float>(score[there ? i : 0]) : -INFINITY;
+        if (there) {
+            lo = fminf(lo, f[v]);
+            hi = fmaxf(hi, f[v]);
+        }
+    }
+    auto across = [&](auto permuted) {
+        lo = fminf(lo, permuted(lo));
+        hi = fmaxf(hi, permuted(hi));
+    };
+    across([](float v) { return dpp_f32<0xB1>(v); });
+    across([](float v) { return dpp_f32<0x4E>(v); });
+    across([](float v) { return dpp_f32<0x141>(v); });
+    across([](float v) { return dpp_f32<0x140>(v); });
+    across([](float v) { return __shfl_xor(v, 16, 64); });
+    across([](float v) { return __shfl_xor(v, 32, 64); });
+    bool found = false;
+    float bound = lo;
+    for (int step = 0; step < 40 && !found; ++step) {
+        bound = lo + (hi - lo) * 0.5f;
+        if (!(bound > lo)) break;   // (nothing between them, or no number)
+        int count = 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(f[v] >= bound));
+        found = count == rest;
+        if (count > rest) lo = bound;
+        else hi = bound;
+    }
+    if (!found) {
+        select_by_bits(row, score);
+        return;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+        if (v * 64 < row.n) row.take(v * 64, v * 64 + lane < row.always || f[v] >= bound);
+    row.rest();
 }
 
 // A workgroup of eight waves takes 16 query blocks of a (batch, head): their scores against all blocks of keys, 16 blocks a wave at a time, then the lists, two rows a
-// wave. The scores stay in LDS as whole numbers, or beyond 1024 blocks in memory of the workgroup's own.
-// The contraction is taken in an order of its own, so that a lane reads whole stretches of a mean: step s of lane group g is column g D/4 + s.
+// wave. The scores stay in LDS, or beyond 1024 blocks in memory of the workgroup's own.
+// The contraction is taken in an order of its own, so that the four lanes of a mean read 64 bytes of it that lie together: steps 2 s and 2 s + 1 of lane group g are columns
+// 8 s + 2 g and the next (with a stretch of a mean for each lane a load was 64 pieces of 16 bytes: 512 x 256 blocks of 24 heads 71 us).
 // MOST: blocks of keys that there is room for in LDS, 0: none.
 template <int D, int MOST>
 __global__ __launch_bounds__(512) void select_rows_kernel(SelectParams p) {
-    __shared__ uint64_t lds[16 * MOST + 1];
+    __shared__ double lds[16 * MOST + 1];
     constexpr int S = D / 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
     const int per_head = (p.nq + 15) / 16, padded = (p.nk + 15) / 16 * 16;
-    uint64_t* const keys = MOST == 0 ? reinterpret_cast<uint64_t*>(p.scores) + static_cast<int64_t>(blockIdx.x) * 16 * padded : lds;
+    double* const scores = MOST == 0 ? p.scores + static_cast<int64_t>(blockIdx.x) * 16 * padded : lds;
     for (int64_t at = blockIdx.x; at < p.groups; at += gridDim.x) {
         const int64_t bh = at / per_head;
         const int i0 = static_cast<int>(at % per_head) * 16, b = static_cast<int>(bh / p.Hq), h = static_cast<int>(bh % p.Hq);
         const int have = (select_length(p, b) + FLUX_KEY_BLOCK - 1) / FLUX_KEY_BLOCK;
-        const double* const mq = p.mq + (bh * p.nq + min(i0 + l16, p.nq - 1)) * D + g * S;
-        const double* const mk = p.mk + (static_cast<int64_t>(b) * p.Hk + h / (p.Hq / p.Hk)) * p.nk * D + g * S;
-        f64x2 a[S / 2];
+        const double* const mq = p.mq + (bh * p.nq + min(i0 + l16, p.nq - 1)) * D + g * 2;
+        const double* const mk = p.mk + (static_cast<int64_t>(b) * p.Hk + h / (p.Hq / p.Hk)) * p.nk * D + g * 2;
+        const int always = min(p.always, min(p.keep, have));
+        const bool all = have <= p.keep || always == p.keep;   // the first ones, whatever their scores are
+        if (!all) {
+            f64x2 a[S / 2];
 #pragma unroll
-        for (int s = 0; s < S / 2; ++s) a[s] = *reinterpret_cast<const f64x2*>(mq + 2 * s);
-        for (int j0 = wave * 16; j0 < have; j0 += 128) {
-            const double* const row = mk + static_cast<int64_t>(min(j0 + l16, have - 1)) * D;
-            f64x4 t = {0.0, 0.0, 0.0, 0.0};
+            for (int s = 0; s < S / 2; ++s) a[s] = *reinterpret_cast<const f64x2*>(mq + 8 * s);
+            for (int j0 = wave * 16; j0 < have; j0 += 128) {
+                const double* const row = mk + static_cast<int64_t>(min(j0 + l16, have - 1)) * D;
+                f64x4 t = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-            for (int s = 0; s < S / 2; ++s) {
-                const f64x2 v = *reinterpret_cast<const f64x2*>(row + 2 * s);
-                t = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s].x, v.x, t, 0, 0, 0);
-                t = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s].y, v.y, t, 0, 0, 0);
+                for (int s = 0; s < S / 2; ++s) {
+                    const f64x2 v = *reinterpret_cast<const f64x2*>(row + 8 * s);
+                    t = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s].x, v.x, t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s].y, v.y, t, 0, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) scores[(4 * r + g) * padded + j0 + l16] = t[r];   // (the lane's rows are g, 4 + g, 8 + g and 12 + g)
             }
-            const int j = j0 + l16;   // the lane's column; its rows are g, 4 + g, 8 + g and 12 + g
-#pragma unroll
-            for (int r = 0; r < 4; ++r) keys[(4 * r + g) * padded + j] = j < p.always ? ~uint64_t{0} : select_rank(t[r]);
         }
         __syncthreads();
-        for (int r = wave; r < 16 && i0 + r < p.nq; r += 8)
-            select_largest(keys + r * padded, have, p.keep, lane, p.blocks + (bh * p.nq + i0 + r) * p.width, p.width);
+        for (int r = wave; r < 16 && i0 + r < p.nq; r += 8) {
+            SelectRow row = {p.blocks + (bh * p.nq + i0 + r) * p.width, have, p.keep, always, p.width, lane};
+            if (all) {
+                for (int i = 0; i < min(have, p.keep); i += 64) row.take(i, i + lane < min(have, p.keep));
+                row.rest();
+            } else if constexpr (MOST == 0) {
+                select_by_bits(row, scores + r * padded);
+            } else {
+                select_by_bound<MOST / 64>(row, scores + r * padded);
+            }
+        }
         __syncthreads();
     }
 }
 
 constexpr int kSelectNear = 1024, kSelectFarGroups = 512;
 
-static int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+static int64_t mean_bytes(int64_t blocks, int D) { return (blocks * D * 8 + 255) / 256 * 256; }
 
 // Checks a call and turns it into the kernels' parameters; `nothing`: there are no lists. `need`: bytes of the workspace.
 static int read_select_args(const flux_select_blocks_args* a, SelectParams& p, bool& nothing, int64_t& need) {
@@ -162,7 +232,7 @@ static int read_select_args(const flux_select_blocks_args* a, SelectParams& p, b
     if (a->B > 0x7fffffff / 64 || a->Hq > 0x7fffffff / 64 / a->B || a->B * a->Hq > 0x7fffffff / 512 / (nq + nk)) return fail(FLUX_E_SHAPE, "%s: problem too large", what);
     p = {a->q, a->k, a->lengths, a->blocks, nullptr, nullptr, nullptr, (int)a->B, (int)a->Hq, (int)a->Hk, (int)a->Lq, (int)a->Lk, (int)nq, (int)nk, (int)width, (int)width,
          (int)std::min(a->always, nk), a->B * a->Hq * ((nq + 15) / 16)};
-    need = round256(a->B * a->Hq * nq * a->D * 8) + round256(a->B * a->Hk * nk * a->D * 8);
+    need = mean_bytes(a->B * a->Hq * nq, a->D) + mean_bytes(a->B * a->Hk * nk, a->D);
     if (nk > kSelectNear) need += std::min<int64_t>(p.groups, kSelectFarGroups) * 16 * ((nk + 15) / 16 * 16) * 8;
     return FLUX_OK;
 }
@@ -170,14 +240,15 @@ static int read_select_args(const flux_select_blocks_args* a, SelectParams& p, b
 template <int D>
 static void select_launch(SelectParams p, char* ws, hipStream_t st) {
     p.mq = reinterpret_cast<double*>(ws);
-    ws += round256(static_cast<int64_t>(p.B) * p.Hq * p.nq * D * 8);
+    ws += mean_bytes(static_cast<int64_t>(p.B) * p.Hq * p.nq, D);
     p.mk = reinterpret_cast<double*>(ws);
-    ws += round256(static_cast<int64_t>(p.B) * p.Hk * p.nk * D * 8);
+    ws += mean_bytes(static_cast<int64_t>(p.B) * p.Hk * p.nk, D);
     p.scores = reinterpret_cast<double*>(ws);
     const int64_t blocks = static_cast<int64_t>(p.B) * (static_cast<int64_t>(p.Hq) * p.nq + static_cast<int64_t>(p.Hk) * p.nk);
     hipLaunchKernelGGL(block_means_kernel<D>, dim3((unsigned)blocks), dim3(256), 0, st, p);
     const dim3 groups((unsigned)p.groups), far_groups((unsigned)std::min<int64_t>(p.groups, kSelectFarGroups));
-    if (p.nk <= 256) hipLaunchKernelGGL((select_rows_kernel<D, 256>), groups, dim3(512), 0, st, p);
+    if (p.nk <= 128) hipLaunchKernelGGL((select_rows_kernel<D, 128>), groups, dim3(512), 0, st, p);
+    else if (p.nk <= 256) hipLaunchKernelGGL((select_rows_kernel<D, 256>), groups, dim3(512), 0, st, p);
     else if (p.nk <= 512) hipLaunchKernelGGL((select_rows_kernel<D, 512>), groups, dim3(512), 0, st, p);   // (two workgroups a CU)
     else if (p.nk <= kSelectNear) hipLaunchKernelGGL((select_rows_kernel<D, kSelectNear>), groups, dim3(512), 0, st, p);
     else hipLaunchKernelGGL((select_rows_kernel<D, 0>), far_groups, dim3(512), 0, st, p);
