@@ -272,3 +272,47 @@ def test_refusals_of_the_library(change, rc):
     a = nv.SparseAttentionArgs(**{**dict(q=s, k=s, v=s, o=p, o_sb=64, o_sh=64, o_sl=64, blocks=p, B=1, Hq=2, Hk=2, Lq=128, Lk=128, count=1, D=64, sm_scale=1.0), **change})
     assert nv.lib().flux_sparse_attention_bf16(ctypes.byref(a), None, 0, None) == rc
     assert nv.lib().flux_sparse_attention_bf16(None, None, 0, None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_lists_cut_in_parts(D):
+    """Few query blocks with long lists: parts without a key, with scores of -inf, and one workspace for two captured graphs."""
+    g = seeded(15)
+    q, k, v = inputs(g, 1, 2, 1, 70, 64 * 40, D)
+    blocks = lists(g, 1, 2, 70, 64 * 40, 40)
+    blocks[0, 0, 0, 8:] = -1                      # the parts behind the first ones name nothing
+    blocks[0, 1, 0, :32] = -1                     # ... in front of the last ones
+    want = tk.block_sparse_attention(q.to(DEV), k.to(DEV), v.to(DEV), blocks.to(DEV))
+    a = nv.SparseAttentionArgs(B=1, Hq=2, Hk=1, Lq=70, Lk=64 * 40, count=40, D=D)
+    assert nv.lib().flux_sparse_attention_workspace_bytes(ctypes.byref(a)) > 0
+    check(want, q, k, v, blocks)
+    none = torch.full_like(blocks, -1)
+    none[0, 1] = blocks[0, 1]
+    got = tk.block_sparse_attention(q.to(DEV), k.to(DEV), v.to(DEV), none.to(DEV))
+    assert bool((got[0, 0] == 0).all()) and torch.equal(got[0, 1], want[0, 1])
+    # keys whose scores are -inf beside others add nothing; where there are no others the formula is no number
+    k2, q2 = k.clone(), q.clone()
+    q2[..., 0] = q2[..., 0].abs() + 0.1
+    first = int(blocks[0, 0, 0, 0])
+    k2[0, 0, first * 64:first * 64 + 64, 0] = -math.inf
+    some = blocks.clone()
+    some[0, 1, 0, :], some[0, 1, 0, 3] = -1, first
+    got = tk.block_sparse_attention(q2.to(DEV), k2.to(DEV), v.to(DEV), some.to(DEV)).cpu()
+    rest = some.clone()
+    rest[0, 0, 0, 0] = -1
+    check(got[:, :1], q2[:, :1], k2, v, rest[:, :1])
+    assert bool(got[0, 1].isnan().all())
+    graphs, outs, args = [], [], [(q.to(DEV), blocks.to(DEV)), ((q * 2).to(DEV), some.to(DEV))]
+    k, v = k.to(DEV), v.to(DEV)
+    pool = None
+    for qd, bd in args:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(tk.block_sparse_attention(qd, k, v, bd))
+        pool = graph.pool()
+        graphs.append(graph)
+    for _ in range(3):
+        for graph, out, (qd, bd) in zip(graphs, outs, args):
+            graph.replay()
+            assert torch.equal(out, tk.block_sparse_attention(qd, k, v, bd))

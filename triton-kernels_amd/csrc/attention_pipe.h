@@ -555,6 +555,7 @@ __device__ __forceinline__ void attn_pipe(const AttnParams& p, char* lds, int nb
         const float inv = LIST && ntiles == 0 ? 0.0f : 1.0f / l_tot;   // (a list without a block: O is 0)
         const int row = q0 + qb * 32 + frow;
         if constexpr (SPLIT) {
+            if (LIST && q0 >= p.L) return;   // (no rows, nothing to add up)
             // in the order the lanes hold it (1 KB per store, rows past L included): block = 32 rows of a (batch, head)
             const int64_t blocks = static_cast<int64_t>(p.total_tiles / splits) * (4 * QB);
             const int64_t at = part * blocks + (static_cast<int64_t>(bh) * p.n_qtiles + qt) * (4 * QB) + wave * QB + qb;
@@ -565,7 +566,9 @@ __device__ __forceinline__ void attn_pipe(const AttnParams& p, char* lds, int nb
                 for (int g = 0; g < 4; ++g)
                     wblk[(db * 4 + g) * 64] = u32x4{__float_as_uint(acc[qb][db][g * 4 + 0]), __float_as_uint(acc[qb][db][g * 4 + 1]),
                                                     __float_as_uint(acc[qb][db][g * 4 + 2]), __float_as_uint(acc[qb][db][g * 4 + 3])};
-            if (fhalf == 0) *reinterpret_cast<f32x2*>(ws + splits * blocks * (32 * D) + (at * 32 + frow) * 2) = f32x2{m_run[qb] * c, l_tot};
+            // (a list's part whose scores are all -inf has a sum of -1, which tells it from one without a key)
+            const float l_out = LIST && ntiles > 0 && m_run[qb] == -INFINITY ? -1.0f : l_tot;
+            if (fhalf == 0) *reinterpret_cast<f32x2*>(ws + splits * blocks * (32 * D) + (at * 32 + frow) * 2) = f32x2{m_run[qb] * c, l_out};
         } else if constexpr (DIRECT) {
             if (row < p.L) {
                 bf16_t* const orow = p.o + b * p.o_sb + h * p.o_sh + static_cast<int64_t>(row) * p.o_sl;
