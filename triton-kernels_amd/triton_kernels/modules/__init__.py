@@ -3,6 +3,7 @@ from triton_kernels.modules.blocks import (
     DoubleStreamBlock,
     Linear,
     LinearGELU,
+    LinearW4,
     Modulation,
     ModulationOut,
     SelfAttention,
@@ -13,6 +14,6 @@ from triton_kernels.modules.normalization import LayerNorm, QKNorm, RMSNorm
 from triton_kernels.modules.positional_embedding import EmbedND
 
 __all__ = [
-    "MLP", "DoubleStreamBlock", "Linear", "LinearGELU", "Modulation", "ModulationOut", "SelfAttention",
+    "MLP", "DoubleStreamBlock", "Linear", "LinearGELU", "LinearW4", "Modulation", "ModulationOut", "SelfAttention",
     "SingleStreamBlock", "attention", "EmbedND", "LayerNorm", "QKNorm", "RMSNorm",
 ]

@@ -25,10 +25,11 @@ import torch.nn as nn
 from torch import Tensor
 
 from triton_kernels import _native as nv
-from triton_kernels.kernels.attention import attention_into, scaled_dot_product_attention, takes_rows
-from triton_kernels.kernels.linear import linear, linear_into, linear_pair_into, qk_fusable, qk_pays
+from triton_kernels.kernels.attention import attention_into, block_sparse_attention, scaled_dot_product_attention, select_blocks, takes_rows
+from triton_kernels.kernels.linear import linear, linear_into, linear_pair_into, linear_w4, qk_fusable, qk_pays
 from triton_kernels.kernels.normalization import layer_norm_modulation, layer_norm_modulation_pair
 from triton_kernels.kernels.positional_embedding import apply_rope, qkv_prep
+from triton_kernels.kernels.quantization import W4, quantize_w4
 from triton_kernels.modules.normalization import QKNorm, plain
 
 
@@ -87,9 +88,12 @@ def _gated_residual(x: Tensor, gate: Tensor, y: Tensor) -> Tensor:
     return out
 
 
-def attention(q: Tensor, k: Tensor, v: Tensor, pe: Tensor) -> Tensor:
+def attention(q: Tensor, k: Tensor, v: Tensor, pe: Tensor, keep: int | None = None, always: int = 0) -> Tensor:
+    """keep: each block of 128 queries attends to that many blocks of 64 keys, as select_blocks chooses them, the first `always` among them; None: to all."""
     q, k = apply_rope(q, k, pe)
-    return _merge_heads(scaled_dot_product_attention(q, k, v))
+    if keep is None:
+        return _merge_heads(scaled_dot_product_attention(q, k, v))
+    return _merge_heads(block_sparse_attention(q, k, v, select_blocks(q, k, keep, always=always)))
 
 
 class Linear(nn.Linear):
@@ -100,6 +104,36 @@ class Linear(nn.Linear):
 class LinearGELU(nn.Linear):
     def forward(self, input: Tensor) -> Tensor:
         return linear(input, self.weight, self.bias, activation="GELU")
+
+
+class LinearW4(nn.Module):
+    """A projection whose weight is held in 4 bits (linear_w4), for serving: its weight is no parameter. zero_points: whether groups have one."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, group: int = 64, zero_points: bool = False, device=None):
+        super().__init__()
+        self.in_features, self.out_features, self.group = in_features, out_features, group
+        w = quantize_w4(torch.zeros(out_features, in_features, device=device), group, zero_points)
+        self.register_buffer("packed", w.packed)
+        self.register_buffer("scale", w.scale)
+        self.register_buffer("zero", w.zero)
+        self.bias = nn.Parameter(torch.zeros(out_features, dtype=torch.bfloat16, device=device), requires_grad=False) if bias else None
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, group: int = 64, zero_points: bool = False) -> "LinearW4":
+        """The projection `linear` with its weight in 4 bits, where that lies."""
+        out = cls(linear.in_features, linear.out_features, linear.bias is not None, group, zero_points, linear.weight.device)
+        w = quantize_w4(linear.weight, group, zero_points)
+        out.packed, out.scale, out.zero = w.packed, w.scale, w.zero
+        if linear.bias is not None:
+            out.bias.data = linear.bias.detach().to(torch.bfloat16, copy=True)
+        return out
+
+    @property
+    def weight(self) -> W4:
+        return W4(self.packed, self.scale, self.zero, (self.out_features, self.in_features), self.group)
+
+    def forward(self, input: Tensor) -> Tensor:
+        return linear_w4(input, self.weight, self.bias)
 
 
 class SelfAttention(nn.Module):
@@ -133,12 +167,22 @@ class Modulation(nn.Module):
         self.lin = Linear(dim, self.multiplier * dim, bias=True)
 
     def forward(self, vec: Tensor) -> tuple[ModulationOut, ModulationOut | None]:
-        if self.takes_fused_silu(vec):
+        if isinstance(self.lin, LinearW4):
+            if self.takes_fused_silu(vec):
+                out = linear_w4(vec, self.lin.weight, self.lin.bias, in_activation="SiLU")
+            else:
+                out = self.lin(_silu(vec))
+        elif self.takes_fused_silu(vec):
             # one launch: the row-vector kernel applies SiLU to vec as it reads it
             out = linear_into(vec, self.lin.weight, self.lin.bias, in_activation="SiLU").reshape(*vec.shape[:-1], -1)
         else:
             out = self.lin(_silu(vec))
         return self.chunks(out)
+
+    def quantize(self, group: int = 64, zero_points: bool = False) -> "Modulation":
+        """Holds the projection's weight in 4 bits from here on: a quarter of a block's weights, which a pass reads for one row a batch element."""
+        self.lin = LinearW4.from_linear(self.lin, group, zero_points)
+        return self
 
     def takes_fused_silu(self, vec: Tensor) -> bool:
         return self.fused_silu and vec.is_cuda and vec.dtype == torch.bfloat16 and vec.numel() // vec.shape[-1] <= 8
@@ -174,6 +218,10 @@ class SingleStreamBlock(nn.Module):
     # fused forward, "linear1", "attention", "linear2". Benchmarks set it to record stream events
     # around a kernel inside real block passes.
     stage_hook = None
+    # How many blocks of 64 keys each block of 128 queries attends to, as select_blocks chooses them (heads of 64 or 128), and how many of
+    # them are the first ones in any case, for the text in front of an image; None: attention over all keys.
+    sparse_keep: int | None = None
+    sparse_always = 0
 
     def __init__(self, hidden_size: int, num_heads: int, mlp_ratio: float = 4.0, qk_scale: float | None = None):
         super().__init__()
@@ -203,7 +251,7 @@ class SingleStreamBlock(nn.Module):
         y1 = self.linear1(x_mod)
         q, k, v = _heads(y1[..., : 3 * hid], self.num_heads)
         q, k = self.norm(q, k, v)
-        attn = attention(q, k, v, pe=pe)
+        attn = attention(q, k, v, pe, self.sparse_keep, self.sparse_always)
         both = torch.cat((attn, _gelu_tanh(y1[..., 3 * hid:])), 2)
         return _gated_residual(x, mod.gate, self.linear2(both))
 
@@ -238,7 +286,10 @@ class SingleStreamBlock(nn.Module):
         # attention output lands in both[:, :hid] in "B L (H D)" order
         attn_out = both[..., :hid].view(B, L, H, D).permute(0, 2, 1, 3)
         hook("attention", "begin")
-        attention_into(q, k, v_src, attn_out)
+        if self.sparse_keep is None:
+            attention_into(q, k, v_src, attn_out)
+        else:
+            block_sparse_attention(q, k, v_src, select_blocks(q, k, self.sparse_keep, always=self.sparse_always), out=attn_out)
         hook("attention", "end")
         out = torch.empty_like(x)
         hook("linear2", "begin")
@@ -250,6 +301,9 @@ class SingleStreamBlock(nn.Module):
 
 class DoubleStreamBlock(nn.Module):
     fused = True
+    # As in SingleStreamBlock; the text's blocks come first.
+    sparse_keep: int | None = None
+    sparse_always = 0
 
     def __init__(self, hidden_size: int, num_heads: int, mlp_ratio: float, qkv_bias: bool = False):
         super().__init__()
@@ -283,7 +337,7 @@ class DoubleStreamBlock(nn.Module):
         img_q, img_k = self.img_attn.norm(img_q, img_k, img_v)
         txt_q, txt_k = self.txt_attn.norm(txt_q, txt_k, txt_v)
         q, k, v = qkv_prep(img_q, img_k, img_v, txt_q, txt_k, txt_v)   # torch.cat(dim=2) of the three pairs
-        attn = attention(q, k, v, pe=pe)
+        attn = attention(q, k, v, pe, self.sparse_keep, self.sparse_always)
         img = self._stream_tail(img, attn[:, Lt:], img_mod1, img_mod2, self.img_attn.proj, self.img_mlp)
         txt = self._stream_tail(txt, attn[:, :Lt], txt_mod1, txt_mod2, self.txt_attn.proj, self.txt_mlp)
         return img, txt
@@ -299,7 +353,7 @@ class DoubleStreamBlock(nn.Module):
         B, Li, hid = img.shape
         Lt = txt.shape[1]
         img, txt = img.contiguous(), txt.contiguous()
-        img_mod1, img_mod2, txt_mod1, txt_mod2, beside = self._modulations(vec, takes_rows(B * H, Lt + Li, hid // H, 2 * B, hid))
+        img_mod1, img_mod2, txt_mod1, txt_mod2, beside = self._modulations(vec, self.sparse_keep is None and takes_rows(B * H, Lt + Li, hid // H, 2 * B, hid))
         img_qkv_lin, txt_qkv_lin = self.img_attn.qkv, self.txt_attn.qkv
         img_m, txt_m = layer_norm_modulation_pair((img, img_mod1.scale, img_mod1.shift), (txt, txt_mod1.scale, txt_mod1.shift))
         qkv = None
@@ -323,7 +377,11 @@ class DoubleStreamBlock(nn.Module):
         if qkv is not None:
             v = _heads(qkv.unsqueeze(0), H)[2]
         attn = torch.empty((B, Lt + Li, hid), dtype=img.dtype, device=img.device)
-        attention_into(q, k, v, attn.view(B, Lt + Li, H, hid // H).permute(0, 2, 1, 3), beside=beside)
+        attn_out = attn.view(B, Lt + Li, H, hid // H).permute(0, 2, 1, 3)
+        if self.sparse_keep is None:
+            attention_into(q, k, v, attn_out, beside=beside)
+        else:
+            block_sparse_attention(q, k, v, select_blocks(q, k, self.sparse_keep, always=self.sparse_always), out=attn_out)
 
         def gated(x, lin, resid, gate):
             return dict(x=x, w=lin.weight, b=lin.bias, resid=resid, gate=gate)
@@ -343,7 +401,7 @@ class DoubleStreamBlock(nn.Module):
         with them, for the attention to run beside it: 226 MB of weights are 35 us of a pass otherwise, now the first third of it.
         Passes at 1024 + 256 tokens 365.9 -> 359.5 us; at 4096 + 512 the attention leaves no room beside it."""
         mods = (self.img_mod, self.txt_mod)
-        if not (all(plain(m, Modulation) and m.takes_fused_silu(vec) for m in mods) and mods[0].multiplier == mods[1].multiplier):
+        if not (all(plain(m, Modulation) and not isinstance(m.lin, LinearW4) and m.takes_fused_silu(vec) for m in mods) and mods[0].multiplier == mods[1].multiplier):
             return (*self.img_mod(vec), *self.txt_mod(vec), ())
         rows = vec.reshape(-1, vec.shape[-1])
         outs = [torch.empty((rows.shape[0], m.lin.weight.shape[0]), dtype=vec.dtype, device=vec.device) for m in mods]
