@@ -144,3 +144,32 @@ def test_refusals_of_the_library(change, rc):
     assert (need > 0) == (rc in (-1, -4) or not change)
     assert nv.lib().flux_select_blocks(ctypes.byref(a), p, need - 1 if not change else 1 << 30, None) == rc
     assert nv.lib().flux_select_blocks(None, None, 0, None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,L", [(64, 64 * 100), (128, 64 * 300), (64, 64 * 700)])
+@pytest.mark.parametrize("close", [2.0 ** -7, 2.0 ** -16, 0.0])
+def test_scores_that_lie_close_together(D, L, close):
+    """Blocks of keys that are nearly alike, of a few kinds: neighbours differ by one bf16 step of one value, or by a large common value that all share, or not at all."""
+    g = seeded(D)
+    q = randn(g, 1, 1, 140, D, dtype=torch.bfloat16)
+    kinds = randn(g, 5, 64, D, dtype=torch.bfloat16)
+    k = kinds[torch.randint(0, 5, (L // 64,), generator=g)].reshape(1, 1, L, D).clone()
+    at = torch.arange(0, L, 64) + torch.randint(0, 64, (L // 64,), generator=g)
+    column = torch.randint(0, D, (L // 64,), generator=g)
+    k[0, 0, at, column] += (k[0, 0, at, column].float() * close * torch.randint(-3, 4, (L // 64,), generator=g)).to(torch.bfloat16)
+    k[..., 0] += 200.0   # scores are the same to 2^-10 of them and more
+    q[..., 0] += 50.0
+    for keep in (1, 7, L // 64 // 3, L // 64 - 1):
+        assert torch.equal(tk.select_blocks(q.to(DEV), k.to(DEV), keep, always=1).cpu(), expected(q, k, keep, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-38, 1e-30, 1e-19, 1e12, 1e30])
+def test_scores_of_other_sizes(size):
+    g = seeded(7)
+    q, k = inputs(g, 1, 2, 1, 300, 64 * 150, 128)
+    q, k = (q.float() * size).bfloat16(), (k.float() * size).bfloat16()
+    assert torch.equal(tk.select_blocks(q.to(DEV), k.to(DEV), 20).cpu(), expected(q, k, 20))
+    k[:, :, ::3] = (k[:, :, ::3].float() / max(size, 1e-20) * 1e-3).bfloat16()   # among others of ordinary size
+    assert torch.equal(tk.select_blocks(q.to(DEV), k.to(DEV), 20).cpu(), expected(q, k, 20))

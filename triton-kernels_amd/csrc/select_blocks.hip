@@ -157,19 +157,21 @@ __device__ __forceinline__ void select_by_bound(SelectRow row, const double* sco
     row.rest();
 }
 
-// A workgroup of eight waves takes 16 query blocks of a (batch, head): their scores against all blocks of keys, 16 blocks a wave at a time, then the lists, two rows a
+// A workgroup takes 16 query blocks of a (batch, head): their scores against all blocks of keys, 16 blocks a wave at a time, then the lists, one or two rows a
 // wave. The scores stay in LDS, or beyond 1024 blocks in memory of the workgroup's own.
 // The contraction is taken in an order of its own, so that the four lanes of a mean read 64 bytes of it that lie together: steps 2 s and 2 s + 1 of lane group g are columns
 // 8 s + 2 g and the next (with a stretch of a mean for each lane a load was 64 pieces of 16 bytes: 512 x 256 blocks of 24 heads 71 us).
 // MOST: blocks of keys that there is room for in LDS, 0: none.
-template <int D, int MOST>
-__global__ __launch_bounds__(512) void select_rows_kernel(SelectParams p) {
+template <int D, int MOST, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, MOST > 512 ? 2 : 4) void select_rows_kernel(SelectParams p) {
     __shared__ double lds[16 * MOST + 1];
     constexpr int S = D / 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
     const int per_head = (p.nq + 15) / 16, padded = (p.nk + 15) / 16 * 16;
     double* const scores = MOST == 0 ? p.scores + static_cast<int64_t>(blockIdx.x) * 16 * padded : lds;
-    for (int64_t at = blockIdx.x; at < p.groups; at += gridDim.x) {
+    // (the groups of a head of keys share an XCD, whose L2 keeps its means)
+    const int64_t per_xcd = gridDim.x / 8;
+    for (int64_t at = blockIdx.x % 8 * per_xcd + blockIdx.x / 8; at < p.groups; at += gridDim.x) {
         const int64_t bh = at / per_head;
         const int i0 = static_cast<int>(at % per_head) * 16, b = static_cast<int>(bh / p.Hq), h = static_cast<int>(bh % p.Hq);
         const int have = (select_length(p, b) + FLUX_KEY_BLOCK - 1) / FLUX_KEY_BLOCK;
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(512) void select_rows_kernel(SelectParams p) {
             f64x2 a[S / 2];
 #pragma unroll
             for (int s = 0; s < S / 2; ++s) a[s] = *reinterpret_cast<const f64x2*>(mq + 8 * s);
-            for (int j0 = wave * 16; j0 < have; j0 += 128) {
+            for (int j0 = wave * 16; j0 < have; j0 += 16 * WAVES) {
                 const double* const row = mk + static_cast<int64_t>(min(j0 + l16, have - 1)) * D;
                 f64x4 t = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(512) void select_rows_kernel(SelectParams p) {
             }
         }
         __syncthreads();
-        for (int r = wave; r < 16 && i0 + r < p.nq; r += 8) {
+        for (int r = wave; r < 16 && i0 + r < p.nq; r += WAVES) {
             SelectRow row = {p.blocks + (bh * p.nq + i0 + r) * p.width, have, p.keep, always, p.width, lane};
             if (all) {
                 for (int i = 0; i < min(have, p.keep); i += 64) row.take(i, i + lane < min(have, p.keep));
@@ -233,7 +235,7 @@ static int read_select_args(const flux_select_blocks_args* a, SelectParams& p, b
     p = {a->q, a->k, a->lengths, a->blocks, nullptr, nullptr, nullptr, (int)a->B, (int)a->Hq, (int)a->Hk, (int)a->Lq, (int)a->Lk, (int)nq, (int)nk, (int)width, (int)width,
          (int)std::min(a->always, nk), a->B * a->Hq * ((nq + 15) / 16)};
     need = mean_bytes(a->B * a->Hq * nq, a->D) + mean_bytes(a->B * a->Hk * nk, a->D);
-    if (nk > kSelectNear) need += std::min<int64_t>(p.groups, kSelectFarGroups) * 16 * ((nk + 15) / 16 * 16) * 8;
+    if (nk > kSelectNear) need += std::min<int64_t>((p.groups + 7) / 8 * 8, kSelectFarGroups) * 16 * ((nk + 15) / 16 * 16) * 8;
     return FLUX_OK;
 }
 
@@ -246,12 +248,15 @@ static void select_launch(SelectParams p, char* ws, hipStream_t st) {
     p.scores = reinterpret_cast<double*>(ws);
     const int64_t blocks = static_cast<int64_t>(p.B) * (static_cast<int64_t>(p.Hq) * p.nq + static_cast<int64_t>(p.Hk) * p.nk);
     hipLaunchKernelGGL(block_means_kernel<D>, dim3((unsigned)blocks), dim3(256), 0, st, p);
-    const dim3 groups((unsigned)p.groups), far_groups((unsigned)std::min<int64_t>(p.groups, kSelectFarGroups));
-    if (p.nk <= 128) hipLaunchKernelGGL((select_rows_kernel<D, 128>), groups, dim3(512), 0, st, p);
-    else if (p.nk <= 256) hipLaunchKernelGGL((select_rows_kernel<D, 256>), groups, dim3(512), 0, st, p);
-    else if (p.nk <= 512) hipLaunchKernelGGL((select_rows_kernel<D, 512>), groups, dim3(512), 0, st, p);   // (two workgroups a CU)
-    else if (p.nk <= kSelectNear) hipLaunchKernelGGL((select_rows_kernel<D, kSelectNear>), groups, dim3(512), 0, st, p);
-    else hipLaunchKernelGGL((select_rows_kernel<D, 0>), far_groups, dim3(512), 0, st, p);
+    const dim3 groups((unsigned)((p.groups + 7) / 8 * 8)), far_groups((unsigned)std::min<int64_t>((p.groups + 7) / 8 * 8, kSelectFarGroups));
+    // (sixteen waves, a row each, where there are few workgroups: 72 x 36 blocks of 24 heads 10.7 -> 9.9 us; eight where two workgroups fit a CU)
+#define CALL(MOST, WAVES, GROUPS) hipLaunchKernelGGL((select_rows_kernel<D, MOST, WAVES>), GROUPS, dim3(64 * WAVES), 0, st, p)
+    if (p.nk <= 128) CALL(128, 16, groups);
+    else if (p.nk <= 256) CALL(256, 16, groups);
+    else if (p.nk <= 512) CALL(512, 8, groups);
+    else if (p.nk <= kSelectNear) CALL(kSelectNear, 8, groups);
+    else CALL(0, 8, far_groups);
+#undef CALL
 }
 
 }  // namespace flux
