@@ -33,9 +33,15 @@ struct W4Params {
     int act, silu;
 };
 
+// Two times 16 in bf16, in a vector register: v_and_or_b32 takes one scalar constant, and with two of them it was two instructions.
+__device__ __forceinline__ uint32_t w4_sixteens() {
+    uint32_t one = 0x41804180u;
+    asm volatile("" : "+v"(one));
+    return one;
+}
 // Eight weights, 16 + q each.
-__device__ __forceinline__ w4_bf16x8 w4_unpack(uint32_t w) {
-    const uint32_t mask = 0x00780078u, one = 0x41804180u;
+__device__ __forceinline__ w4_bf16x8 w4_unpack(uint32_t w, uint32_t one) {
+    const uint32_t mask = 0x00780078u;
     w4_u32x4 r;
     r.x = ((w << 3) & mask) | one;
     r.y = ((w >> 1) & mask) | one;
@@ -96,7 +102,7 @@ __device__ __forceinline__ void w4_silu(Vec16<bf16_t>& x, Vec16<bf16_t>& lo) {
 // acc += s (q - z) x over one chunk, for MT times 16 rows of x, the lane's `row` bytes behind `a`: the sum of (16 + q) x without (16 + z) times the sum of x, which the
 // matrix cores form beside it. `peak` takes the largest of these sums: what goes with it is lost to 2^-23 of it, and where x is not finite it leaves a NaN or an infinity.
 template <int GPC, bool ZERO, int MT>
-__device__ __forceinline__ void w4_chunk(w4_f32x4 (&acc)[MT], const W4Piece<GPC, ZERO>& w, const char* a, const int (&row)[MT], float& peak) {
+__device__ __forceinline__ void w4_chunk(w4_f32x4 (&acc)[MT], const W4Piece<GPC, ZERO>& w, const char* a, const int (&row)[MT], uint32_t sixteens, float& peak) {
     const w4_f32x4 none = {0.f, 0.f, 0.f, 0.f};
     const w4_bf16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
@@ -106,7 +112,7 @@ __device__ __forceinline__ void w4_chunk(w4_f32x4 (&acc)[MT], const W4Piece<GPC,
 #pragma unroll
         for (int j = i * 4 / GPC; j < (i + 1) * 4 / GPC; ++j) {
             const bool first = j == i * 4 / GPC;
-            const w4_bf16x8 b = w4_unpack(w.q[j]);
+            const w4_bf16x8 b = w4_unpack(w.q[j], sixteens);
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 const w4_bf16x8 x = *reinterpret_cast<const w4_bf16x8*>(a + row[m] + j * 64);
@@ -192,6 +198,7 @@ __global__ __launch_bounds__(64 * NW * KS, 4) void w4_rows_kernel(W4Params p) {
     const float bias = p.bias != nullptr ? bf2f(p.bias[min(out_n, p.N - 1)]) : 0.0f;
     w4_f32x4 acc[1][1] = {{{0.f, 0.f, 0.f, 0.f}}};
     float peak = 0.0f;
+    const uint32_t sixteens = w4_sixteens();
     W4Piece<GPC, ZERO> piece[U];
     for (int c0 = 0; c0 < p.chunks; c0 += p.slab) {
         const int n = min(p.slab, p.chunks - c0), vectors = rows * n * 16;   // vectors of 8 values of x, 16 a chunk
@@ -228,7 +235,7 @@ __global__ __launch_bounds__(64 * NW * KS, 4) void w4_rows_kernel(W4Params p) {
             for (int u = 0; u < U; ++u) {
                 const int c = base + KS * u;
                 if (c >= n) break;
-                w4_chunk<GPC, ZERO, 1>(acc[0], piece[u], lds + c * (kW4Chunk * 2), xrow, peak);
+                w4_chunk<GPC, ZERO, 1>(acc[0], piece[u], lds + c * (kW4Chunk * 2), xrow, sixteens, peak);
                 if (c + KS * U < n) w.template request<true>(piece[u], c0 + c + KS * U);
             }
     }
@@ -283,6 +290,7 @@ __global__ __launch_bounds__(64 * NW * KS) void w4_tiles_kernel(W4Params p) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[t][m] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
     float peak = 0.0f;
+    const uint32_t sixteens = w4_sixteens();
     W4Piece<GPC, ZERO> piece[NTW][CW];
     auto load_w = [&](W4Piece<GPC, ZERO>& to, int t, int chunk) {   // (past the end: not used)
         W4Tile<GPC, ZERO>(p, min(tile0 + t, tiles - 1), lane).template request<false>(to, min(chunk, p.chunks - 1));
@@ -316,10 +324,11 @@ __global__ __launch_bounds__(64 * NW * KS) void w4_tiles_kernel(W4Params p) {
                 const int chunk = step * KS + part, at = chunk % p.slab;
                 if (chunk < p.chunks) {
 #pragma unroll
-                    for (int t = 0; t < NTW; ++t) w4_chunk<GPC, ZERO, MT>(acc[t], piece[t][c], x + at * (kW4Chunk * 2), row, peak);
+                    for (int t = 0; t < NTW; ++t) w4_chunk<GPC, ZERO, MT>(acc[t], piece[t][c], x + at * (kW4Chunk * 2), row, sixteens, peak);
                 }
+                if (step + CW < steps)
 #pragma unroll
-                for (int t = 0; t < NTW; ++t) load_w(piece[t][c], t, (step + CW) * KS + part);
+                    for (int t = 0; t < NTW; ++t) load_w(piece[t][c], t, (step + CW) * KS + part);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
