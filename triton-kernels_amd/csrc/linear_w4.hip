@@ -443,9 +443,10 @@ template <int GPC, bool ZERO>
 static void w4_rows_launch(W4Params p, hipStream_t st) {
     const int tiles = (p.N + kW4Tile - 1) / kW4Tile;
     const bool few = tiles <= 256;   // no more than a row tile a CU
-    // Up to 4 rows, f(x), and up to 8 rows of few outputs: x through registers. Two row tiles a wave group or more make the work on x less (3 x 9216 x 3072 with SiLU
-    // 10.0 -> 9.5 us, 4 rows 11.8 -> 9.9) and the launch longer (1 x 18432 x 3072 10.1 -> 15.9, 1 x 9216 7.5 -> 9.1); eight parts of K pay where there are few
-    // outputs and many chunks (2 x 4096 x 8192 10.8 -> 7.7, 8 x 3072 x 3072 6.8 -> 5.6; 1 x 18432 x 3072 10.1 -> 13.7) or many rows.
+    // Up to 4 rows, f(x), and up to 8 rows of few outputs: x through registers. More row tiles a workgroup share the work on x, and leave CUs idle: us for one, two, three and four
+    // of them at 3 x 9216 x 3072 with SiLU 10.0, 9.7, 8.1 and 9.2, 4 x 9216 11.8, 10.9, 8.6 and 10.2, 6 x 6144 (two are a workgroup a CU) 8.8 with two and 10.2 with three,
+    // 1 x 18432 10.1, 11.8 and 15.9 with four. Eight parts of K pay where there are few outputs and many chunks (2 x 4096 x 8192 10.8 -> 7.7, 8 x 3072 x 3072 6.8 -> 5.6; 1 x
+    // 18432 x 3072 10.1 -> 13.7) or many rows.
     if (p.M <= 4 || p.silu || (p.M <= 8 && few)) {
         const int rb = p.silu ? 8 : 16, held = std::min(p.M, rb) * (p.silu ? 2 : 1);
         p.slab = std::min({p.chunks, 64, 48 * 1024 / (held * kW4Chunk * 2) / 4 * 4});   // up to 48 KB of x, so that three workgroups share a CU
@@ -455,7 +456,8 @@ static void w4_rows_launch(W4Params p, hipStream_t st) {
         };
 #define CALL(NW, KS) if (p.silu) call(w4_rows_kernel<GPC, ZERO, true, NW, KS>, NW, KS); else call(w4_rows_kernel<GPC, ZERO, false, NW, KS>, NW, KS)
         if (few && (p.chunks >= 32 || p.M > 4)) { CALL(1, 8); }
-        else if (p.silu && p.M >= 3 && !few) call(w4_rows_kernel<GPC, ZERO, true, 4, 4>, 4, 4);
+        else if (p.silu && p.M >= 3 && tiles > 512) call(w4_rows_kernel<GPC, ZERO, true, 3, 4>, 3, 4);
+        else if (p.silu && p.M >= 3 && !few) call(w4_rows_kernel<GPC, ZERO, true, 2, 4>, 2, 4);
         else { CALL(1, 4); }
 #undef CALL
         return;
