@@ -95,7 +95,7 @@ def _lengths(lengths: Tensor | None, batch: int, dev: torch.device, most: int) -
         raise TypeError(f"unsupported dtype {lengths.dtype} of lengths")
     assert lengths.shape == (batch,), f"lengths are [{batch}], not {tuple(lengths.shape)}"
     if lengths.dtype != torch.int32:
-        lengths = lengths.clamp(0, most).to(torch.int32)   # (a number beyond 32 bits is a long sequence, not what is left of it)
+        lengths = lengths.long().clamp(0, most).to(torch.int32)   # (a number beyond 32 bits is a long sequence, not what is left of it)
     return lengths.contiguous()
 
 
@@ -169,7 +169,7 @@ def _launch_sparse(q: Tensor, k: Tensor, v: Tensor, blocks: Tensor, sm_scale: fl
     dev = nv.require_gpu(q, k, v, blocks, lengths, out)
     lengths = _lengths(lengths, B, dev, Lk)
     if blocks.dtype != torch.int32:
-        blocks = blocks.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+        blocks = blocks.long().clamp(-1, 2 ** 31 - 1).to(torch.int32)
     blocks = blocks.contiguous()
     o = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
     assert o.shape == q.shape and (o.numel() == 0 or o.stride(3) == 1), f"block_sparse_attention: out is {tuple(q.shape)} with contiguous heads"
