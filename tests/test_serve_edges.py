@@ -28,3 +28,13 @@ def test_lists_and_lengths_of_every_whole_type(dtype):
     want = tk.block_sparse_attention(q, k, v, blocks.int(), lengths=lengths.int()), tk.select_blocks(q, k, 2, lengths=lengths.int())
     assert torch.equal(tk.block_sparse_attention(q, k, v, blocks.to(dtype), lengths=lengths.to(dtype)), want[0])
     assert torch.equal(tk.select_blocks(q, k, 2, lengths=lengths.to(dtype)), want[1])
+
+
+@pytest.mark.gpu
+def test_counts_beyond_64_bits():
+    g = seeded(2)
+    q, k = (randn(g, 1, 2, 300, 64, dtype=BF).to(DEV) for _ in range(2))
+    every = torch.arange(5, dtype=torch.int32, device=DEV).expand(1, 2, 3, 5)
+    for keep in (2 ** 64, 2 ** 65 + 1, 2 ** 62, 5):
+        assert torch.equal(tk.select_blocks(q, k, keep), every)
+        assert torch.equal(tk.select_blocks(q, k, 3, always=keep), every[..., :3])

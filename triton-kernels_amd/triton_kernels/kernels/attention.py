@@ -114,7 +114,7 @@ def select_blocks(q: Tensor, k: Tensor, keep: int, *, always: int = 0, lengths: 
     q, k    : bf16 [B, Hq, Lq, D] and [B, Hk, Lk, D] views, heads of 64 or 128; Hq is a multiple of Hk, query head h reads key head h // (Hq // Hk).
               Up to 16384 blocks of keys
     keep    : how many blocks; all of them where there are no more
-    always  : the first `always` blocks are among them in any case (the text in front of an image)
+    always  : the first `always` blocks (as many of them as `keep` has room for) are among them in any case: the text in front of an image
     lengths : whole numbers [B] on the GPU, or None: keys from lengths[b] on are not there
 
     A block's score is the product of the queries' mean and the mean of its keys, both formed in 64 bits, so that the choice does not go with rounding; the
@@ -133,7 +133,8 @@ def select_blocks(q: Tensor, k: Tensor, keep: int, *, always: int = 0, lengths: 
     dev = nv.require_gpu(q, k, lengths)
     lengths = _lengths(lengths, B, dev, Lk)
     q, k = _bhld_view(q.detach()), _bhld_view(k.detach())
-    blocks = torch.empty((B, Hq, -(-Lq // QUERY_BLOCK), min(keep, -(-Lk // KEY_BLOCK))), dtype=torch.int32, device=dev)
+    keep, always = (min(n, -(-Lk // KEY_BLOCK)) for n in (keep, always))   # (a count may be beyond what the library's arguments hold)
+    blocks = torch.empty((B, Hq, -(-Lq // QUERY_BLOCK), keep), dtype=torch.int32, device=dev)
     if blocks.numel() == 0:
         return blocks
     a = nv.SelectBlocksArgs(nv.src4(q), nv.src4(k), nv.ptr(lengths), blocks.data_ptr(), B, Hq, Hk, Lq, Lk, keep, always, D)
