@@ -4,6 +4,7 @@ import torch
 
 import triton_kernels as tk
 from triton_kernels.kernels import attention as attention_calls
+from triton_kernels.modules import LinearW4, Modulation
 from util import DEV, randn, seeded
 
 BF = torch.bfloat16
@@ -38,3 +39,13 @@ def test_counts_beyond_64_bits():
     for keep in (2 ** 64, 2 ** 65 + 1, 2 ** 62, 5):
         assert torch.equal(tk.select_blocks(q, k, keep), every)
         assert torch.equal(tk.select_blocks(q, k, 3, always=keep), every[..., :3])
+
+
+def test_quantised_weights_of_the_whole_range():
+    w = torch.tensor([[-3e38, 3e38, 0.0, 1e38] * 8, [1e-30, -1e-30, 0.0, 5e-31] * 8, [3e38] * 32])
+    for zeros in (False, True):
+        q, scale, zero = tk.quantize_w4(w, 32, zeros).unpack()
+        assert bool(scale.isfinite().all()) and bool((scale > 0).all())
+        back = (q.double() - (8.0 if zero is None else zero.double().repeat_interleave(32, 1))) * scale.double().repeat_interleave(32, 1)
+        # half a step each for the value and the zero point, and half a bf16 step of the scale for 15 of them
+        assert bool(((back - w.double()).abs() <= scale.double().repeat_interleave(32, 1) * (1.0 + 15 * 2.0 ** -8)).all())

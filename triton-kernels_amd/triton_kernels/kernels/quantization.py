@@ -112,7 +112,7 @@ def quantize_w4(w: Tensor, group: int = 64, zero_points: bool = False) -> W4:
         raise ValueError("quantize_w4: the weight holds values that are not finite")
     if zero_points:
         low, high = wf.amin(-1).clamp(max=0), wf.amax(-1).clamp(min=0)
-        scale = ((high - low) / 15).to(torch.bfloat16)
+        scale = (high / 15 - low / 15).to(torch.bfloat16)   # (their difference may be beyond fp32)
     else:
         scale = (wf.abs().amax(-1) / 7.5).to(torch.bfloat16)
     step = torch.where(scale == 0, 1.0, scale.float())
