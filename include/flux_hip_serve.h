@@ -30,8 +30,9 @@ typedef struct flux_w4 {
 
 /* y[m] = act(f(x[m]) W^T + bias): x [M, K] bf16 (row stride ldx), bias [N] bf16 or null, y [M, N] bf16 (row stride ldy); act is FLUX_ACT_NONE or
  * FLUX_ACT_GELU_TANH, in_act FLUX_ACT_NONE or (up to 8 rows) FLUX_ACT_SILU, f(x) = x sigmoid(x). fp32 sums, rounded once; f(x) is held to 2^-16 of its
- * value. Beyond 128 rows the weights are laid out as bf16, each rounded once (2^-9 of it), in the workspace
- * (flux_linear_w4_workspace_bytes, 0 below; 256-byte aligned, the launch's own until it has run) in front of flux_linear_bf16. */
+ * value. Up to 128 rows a group's sum is that of (q + 16) x without that of (z + 16) x, which keeps what is above 2^-18 of the group's largest |x| s. Beyond
+ * them the weights are laid out as bf16, each rounded once (2^-8 of it), in the workspace (flux_linear_w4_workspace_bytes, 0 below; 256-byte aligned, the
+ * launch's own until it has run) in front of flux_linear_bf16, and ldx is at least K. */
 typedef struct flux_linear_w4_args {
     const void* x; const void* bias; void* y;
     flux_w4 w;
@@ -48,7 +49,7 @@ int flux_w4_unpack(const flux_w4* w, void* out, void* stream);
  * Which blocks of keys a block of queries attends to.
  * q [B, Hq, Lq, D] and k [B, Hk, Lk, D] bf16 with strides as in flux_src4, Hq a multiple of Hk (query head h reads key head h / (Hq / Hk)), D 64 or 128. For each
  * block of FLUX_QUERY_BLOCK queries (the last may be shorter) the scores of the blocks of FLUX_KEY_BLOCK keys are mean(q) . mean(k), formed in 64 bits;
- * the `keep` largest (or all, where there are no more) are chosen, the lower number among equals, a NaN below everything, the first `always` blocks in any case.
+ * the `keep` largest (or all, where there are no more) are chosen, the lower number among equals, a NaN below everything, the first `always` blocks (up to `keep` of them) in any case.
  * lengths (int32 [B], or null): keys from lengths[b] on are not there; below 0 counts as 0, beyond Lk as Lk.
  * blocks receives int32 [B, Hq, ceil(Lq / 128), min(keep, ceil(Lk / 64))]: the chosen numbers in ascending order, -1 behind them.
  * The workspace (flux_select_blocks_workspace_bytes; 256-byte aligned) holds the means and scores.
@@ -67,7 +68,7 @@ int flux_select_blocks(const flux_select_blocks_args* args, void* workspace, int
  *   o[i] = sum_j p_j v[j],  p = softmax(sm_scale q[i] . k[j]) over the tokens j of those blocks, j < min(lengths[b], Lk).
  * q, o [B, Hq, Lq, D], k, v [B, Hk, Lk, D] bf16. blocks is int32 [B, Hq, ceil(Lq / 128), count], contiguous; numbers that are no block of the sequence
  * name nothing, a number that stands there twice counts twice. Rows that see no token at all are 0. sm_scale is finite.
- * The workspace (flux_sparse_attention_workspace_bytes, 0 where lists are not cut; 256-byte aligned) holds partial results. */
+ * The workspace (flux_sparse_attention_workspace_bytes, 0 where lists are not cut; 256-byte aligned) holds partial results; without it lists stay whole. */
 typedef struct flux_sparse_attention_args {
     flux_src4 q, k, v;
     void* o; int64_t o_sb, o_sh, o_sl;

@@ -1,4 +1,6 @@
 """Calls of linear_w4, select_blocks and block_sparse_attention at the edges of what they take."""
+import sys
+
 import pytest
 import torch
 
@@ -49,3 +51,80 @@ def test_quantised_weights_of_the_whole_range():
         back = (q.double() - (8.0 if zero is None else zero.double().repeat_interleave(32, 1))) * scale.double().repeat_interleave(32, 1)
         # half a step each for the value and the zero point, and half a bf16 step of the scale for 15 of them
         assert bool(((back - w.double()).abs() <= scale.double().repeat_interleave(32, 1) * (1.0 + 15 * 2.0 ** -8)).all())
+
+
+def test_a_weight_is_quantised_once():
+    m = Modulation(64, double=False).quantize(32, True)
+    before = m.lin.weight.unpack()
+    with pytest.raises(AssertionError, match="LinearW4"):
+        m.quantize()
+    assert isinstance(m.lin, LinearW4) and all(torch.equal(a, b) for a, b in zip(before, m.lin.weight.unpack()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 9, 129])
+def test_a_hook_hears_of_the_product(monkeypatch, rows):
+    module, heard = sys.modules["triton_kernels.kernels.linear"], []   # (the package's attribute of that name is the function)
+    g = seeded(rows)
+    w, x = tk.quantize_w4(randn(g, 17, 96), 32).to(DEV), randn(g, rows, 96, dtype=BF).to(DEV)
+    want = tk.linear_w4(x, w)
+    monkeypatch.setattr(module, "launch_hook", heard.append)
+    assert torch.equal(tk.linear_w4(x, w, in_activation="SiLU" if rows == 1 else ""), want) == (rows > 1)
+    assert len(heard) == 1 and heard[0]["flops16"] == 2 * rows * 17 * 96 and heard[0]["bytes"] > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40, 128, 129, 300])
+def test_rows_that_are_one_row(rows):
+    """An expanded row, odd numbers of outputs and the shortest rows there are, also where the weights are laid out first."""
+    g = seeded(rows)
+    w, x = tk.quantize_w4(randn(g, 17, 32), 32).to(DEV), randn(g, 1, 32, dtype=BF).to(DEV)
+    y = tk.linear_w4(x.expand(rows, 32), w)
+    assert torch.equal(y, tk.linear_w4(x.repeat(rows, 1), w)) and torch.equal(y, y[:1].expand(rows, 17))
+    # weights rounded to bf16 beyond 128 rows, the result to bf16; fp32 sums of 32 terms of up to 31 |x| s, with and without the weight
+    q, scale, _ = w.to("cpu").unpack()
+    wf = (q.double() - 8) * scale.double().repeat_interleave(32, 1)
+    want, size = x.double().cpu() @ wf.T, x.double().abs().cpu() @ wf.abs().T
+    sums = x.double().abs().cpu().sum() * scale.double().T * 31 * 2 * 32 * 2.0 ** -24
+    off = (want.abs() * 2.0 ** -8 + size * (2.0 ** -8 if rows > 128 else 0.0) + sums) * 1.01
+    assert bool(((y[:1].double().cpu() - want).abs() <= off).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_calls_from_code_that_is_traced(backend):
+    torch._dynamo.reset()
+    g = seeded(3)
+    w, x = tk.quantize_w4(randn(g, 40, 64), 64).to(DEV), randn(g, 3, 64, dtype=BF).to(DEV)
+    q, k = randn(g, 1, 2, 300, 64, dtype=BF).to(DEV), randn(g, 1, 2, 300, 64, dtype=BF).to(DEV)
+    blocks = tk.select_blocks(q, k, 2)
+    for fn, args in ((lambda x: tk.linear_w4(x * 1.0, w, activation="GELU") * 2.0, (x,)), (lambda q, k: tk.select_blocks(q * 1.0, k, 2, always=1) + 0, (q, k)),
+                     (lambda q, k: tk.block_sparse_attention(q * 1.0, k, k, blocks, 0.1) * 1.0, (q, k)), (lambda q, k: tk.block_sparse_attention(q, k, k, tk.select_blocks(q, k, 3)) * 1.0, (q, k))):
+        assert torch.equal(torch.compile(fn, backend=backend)(*args), fn(*args))
+        torch._dynamo.reset()   # (what was compiled for it before serves a second call too)
+        with pytest.raises(Exception):
+            torch.compile(fn, backend=backend, fullgraph=True)(*args)
+    torch._dynamo.reset()
+
+
+@pytest.mark.gpu
+def test_two_operators_at_once_on_two_streams():
+    """The same operands on two streams, each call with a workspace of its own."""
+    g = seeded(4)
+    w, x = tk.quantize_w4(randn(g, 256, 512), 128).to(DEV), randn(g, 200, 512, dtype=BF).to(DEV)
+    q, k = randn(g, 1, 2, 70, 128, dtype=BF).to(DEV), randn(g, 1, 2, 64 * 40, 128, dtype=BF).to(DEV)
+    far, far_k = q[..., :64].contiguous(), randn(g, 1, 2, 64 * 1030, 64, dtype=BF).to(DEV)
+
+    def calls():
+        blocks = tk.select_blocks(q, k, 30)
+        return tk.linear_w4(x, w), blocks, tk.block_sparse_attention(q, k, k, blocks), tk.select_blocks(far, far_k, 9)
+
+    want, streams = calls(), [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(calls())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for each in got for a, b in zip(each, want))

@@ -197,7 +197,7 @@ def block_sparse_attention(q: Tensor, k: Tensor, v: Tensor, blocks: Tensor, sm_s
     lengths  : whole numbers [B], or None: keys from lengths[b] on are not there
     out      : where the result goes, a [B, Hq, Lq, D] view with contiguous heads, 16-byte aligned rows and memory of its own
 
-    Rows that see no key are 0. Scores and sums are fp32; q times the scale, and the probabilities, are rounded to bf16 for the matrix cores, as in
+    Rows that see no key are 0. Scores and sums are fp32; the probabilities are rounded to bf16 for the matrix cores, as in
     scaled_dot_product_attention. It is not differentiated: a gradient that reaches it raises NotImplementedError.
     """
     if is_dynamo_compiling():

@@ -373,7 +373,8 @@ def linear_w4(x: Tensor, w: W4, b: Tensor | None = None, *, activation: str = ""
     in_activation : "SiLU" applies x * sigmoid(x) to x on the way in; at most 8 rows
 
     Sums are fp32 and y is rounded once; up to 128 rows the weights are what the numbers stand for, beyond them they are laid out as bf16 first, each rounded
-    once. x * sigmoid(x) keeps 16 bits. What is not finite in x goes as in the formula. It is not differentiated: a gradient that reaches it raises NotImplementedError.
+    once. Up to 128 rows a group's sum is that of (q + 16) x without that of (zero + 16) x, which keeps what is above 2^-18 of the group's largest |x| times its
+    scale. x * sigmoid(x) keeps 16 bits. What is not finite in x goes as in the formula. It is not differentiated: a gradient that reaches it raises NotImplementedError.
     """
     if is_dynamo_compiling():
         return torch.compiler.disable(linear_w4)(x, w, b, activation=activation, in_activation=in_activation)
@@ -417,6 +418,7 @@ def _launch_linear_w4(x: Tensor, w: W4, b: Tensor | None, activation: str, in_ac
     a = nv.LinearW4Args(x2.data_ptr(), nv.ptr(b), y.data_ptr(), w._args(), m, x2.stride(0) if m > 1 else k, n, act, in_act)
     if launch_hook is not None:
         note = linear_launch_metadata(m, n, k, x.element_size(), "+".join(p for p in (activation, in_activation and f"in:{in_activation}", f"4 bits by {w.group}") if p))
+        note["name"] = note["name"].replace("flux_linear_bf16", "flux_linear_w4_bf16")
         note["bytes"] -= 1.5 * n * k
         launch_hook(note)
     with nv.on_device(dev):

@@ -121,6 +121,7 @@ class LinearW4(nn.Module):
     @classmethod
     def from_linear(cls, linear: nn.Linear, group: int = 64, zero_points: bool = False) -> "LinearW4":
         """The projection `linear` with its weight in 4 bits, where that lies."""
+        assert isinstance(linear, nn.Linear), f"a projection with a weight to hold in 4 bits, not {type(linear).__name__}"
         out = cls(linear.in_features, linear.out_features, linear.bias is not None, group, zero_points, linear.weight.device)
         w = quantize_w4(linear.weight, group, zero_points)
         out.packed, out.scale, out.zero = w.packed, w.scale, w.zero
