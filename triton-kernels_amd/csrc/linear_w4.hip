@@ -8,8 +8,8 @@
 // x the rows and W the columns of the result, whose 16 rows cost one row's time). What is too much, (16 + z) times the sum of x, comes from the matrix cores as well,
 // as a product with ones. A group's sum takes its scale behind the product, in fp32: nothing is rounded but y.
 //
-// us among others of its kind: 1 x 18432 x 3072 8.4, with SiLU 10.1 (floor 5.6), 3 x 9216 x 3072 with SiLU 9.6, 1 x 1000 x 1024 3.0 (a launch), 16 x 9216 x 3072 9.0, 24 x 12288
-// x 3072 13.5, 128 x 9216 x 3072 29, 512 x 9216 x 3072 47 (17 of them for laying the weights out).
+// us among others of its kind: 1 x 18432 x 3072 8.4, with SiLU 8.8 to 10.3 by the box (floor 5.7), 3 x 9216 x 3072 with SiLU 7.5 to 8.2, 1 x 1000 x 1024 3.1 (a launch), 16 x
+// 9216 x 3072 9.0, 24 x 12288 x 3072 12.4 to 12.9, 128 x 9216 x 3072 29, 512 x 9216 x 3072 47.5 (15 of them for laying the weights out).
 #include "common.h"
 #include "../../include/flux_hip_serve.h"
 #include <algorithm>
@@ -373,7 +373,7 @@ static int w4_tiles_lds(const W4Params& p, int held, int parts_kb) {
     return std::max((slabs > 1 ? 2 : 1) * held * (p.slab * kW4Chunk * 2 + 16), parts_kb * 1024);
 }
 
-// W as bf16 [N, K], (q - z) s rounded once. A wave takes a tile, whose rows pass through LDS so that they leave 256 bytes at a time (9216 x 3072: 17.1 us for
+// W as bf16 [N, K], (q - z) s rounded once. A wave takes a tile, whose rows pass through LDS so that they leave 256 bytes at a time (9216 x 3072: 14.4 us, 17.1 in
 // pieces of 64 bytes of 16 rows).
 template <int GPC, bool ZERO>
 __global__ __launch_bounds__(256) void w4_unpack_kernel(const w4_u32x4* q, const bf16_t* s, const uint8_t* z, bf16_t* out, int N, int K, int chunks, int64_t tiles) {
