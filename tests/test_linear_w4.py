@@ -271,3 +271,59 @@ def test_refusals_of_the_library(change, rc):
         b = nv.LinearW4Args(p, None, p, bad, 1, 64, 16, 0, 0)
         assert nv.lib().flux_linear_w4_bf16(ctypes.byref(b), None, 0, None) == code
         assert nv.lib().flux_w4_unpack(ctypes.byref(bad), p, None) == code
+
+
+# Beyond 128 rows, thousands of outputs: weights unpacked between the products. Fewer columns than a slab of 128, ends of slabs, more than the ring of four holds; last workgroups of one row
+# and of a few outputs, two and three tiles a wave.
+@pytest.mark.gpu
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group,rows,n,k", [(32, 129, 9301, 96), (64, 256, 9216, 192), (128, 200, 12300, 640), (64, 385, 6200, 1088), (32, 512, 9217, 32), (64, 513, 7000, 320), (128, 640, 9000, 1152), (32, 1000, 4616, 160)])
+def test_hundreds_of_rows_of_thousands_of_outputs(group, rows, n, k, zeros):
+    g = seeded(rows + n + k)
+    w, q, scale, zero = weights(g, n, k, group, zeros)
+    wide = randn(g, rows, k + 24, dtype=torch.bfloat16)
+    wide[:, k:], wide[:, :8] = math.nan, math.inf   # (what lies beside a row is not its own)
+    x, b = wide[:, 8:k + 8].clone(), randn(g, n, dtype=torch.bfloat16)
+    wide[:, 8:k + 8] = x[:] = randn(g, rows, k, dtype=torch.bfloat16)
+    moved = wide.to(DEV)
+    check(tk.linear_w4(moved[:, 8:k + 8], w, b.to(DEV)), x, b, q, scale, zero, rounded=True)
+    check(tk.linear_w4(x.to(DEV), w, activation="GELU"), x, None, q, scale, zero, "GELU", rounded=True)
+
+
+@pytest.mark.gpu
+def test_hundreds_of_rows_that_are_not_finite():
+    g = seeded(31)
+    w, q, scale, zero = weights(g, 9216, 256, 64, True)
+    x = randn(g, 200, 256, dtype=torch.bfloat16)
+    x[0, 3], x[199, 255], x[130, 17], x[131, 100] = math.inf, -math.inf, math.nan, 1e36
+    got = tk.linear_w4(x.to(DEV), w).double().cpu()
+    want = expected(x, None, q, scale, zero, "", "", True)[0]
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf() & (got > 0), want.isinf() & (want > 0)) and torch.equal(got.isinf() & (got < 0), want.isinf() & (want < 0))
+    rest = [i for i in range(200) if i not in (0, 130, 131, 199)]
+    # scales from the smallest to nearly the largest, whose products with q - z are numbers
+    for size in (2.0 ** -133, 2.0 ** -126, 2.0 ** 123):
+        most = tk.pack_w4(q, torch.full_like(scale, size), zero).to(DEV)
+        assert torch.equal(tk.linear_w4(torch.eye(256, dtype=torch.bfloat16, device=DEV), most).t(), most.dequantize())
+    check(tk.linear_w4(x.to(DEV), w)[rest], x[rest], None, q, scale, zero, rounded=True)
+
+
+@pytest.mark.gpu
+def test_hundreds_of_rows_in_a_graph_and_on_a_stream():
+    g = seeded(32)
+    w, *_ = weights(g, 9216, 384, 64, False)
+    x = randn(g, 300, 384, dtype=torch.bfloat16).to(DEV)
+    stream = torch.cuda.Stream()
+    want = [tk.linear_w4(x * i, w) for i in (1, 2, 3)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        other = tk.linear_w4(x, w)
+    stream.synchronize()
+    assert torch.equal(other, want[0])
+    graph, mine = torch.cuda.CUDAGraph(), x.clone()
+    with torch.cuda.graph(graph):
+        out = tk.linear_w4(mine, w)
+    for i in range(3):
+        mine.copy_(x * (i + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i])

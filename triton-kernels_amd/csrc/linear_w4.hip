@@ -9,7 +9,7 @@
 // as a product with ones. A group's sum takes its scale behind the product, in fp32: nothing is rounded but y.
 //
 // us among others of its kind: 1 x 18432 x 3072 8.4, with SiLU 8.8 to 10.3 by the box (floor 5.7), 3 x 9216 x 3072 with SiLU 7.5 to 8.2, 1 x 1000 x 1024 3.1 (a launch), 16 x
-// 9216 x 3072 9.0, 24 x 12288 x 3072 12.4 to 12.9, 128 x 9216 x 3072 29, 512 x 9216 x 3072 47.5 (15 of them for laying the weights out).
+// 9216 x 3072 9.0, 24 x 12288 x 3072 12.4 to 12.9, 128 x 9216 x 3072 29, 512 x 9216 x 3072 41, 1000 x 9216 x 3072 67 (15 of them for laying the weights out).
 #include "common.h"
 #include "../../include/flux_hip_serve.h"
 #include <algorithm>
@@ -21,6 +21,9 @@ namespace flux {
 typedef __bf16 w4_bf16x8 __attribute__((ext_vector_type(8)));
 typedef float w4_f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t w4_u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 w4_f16x2 __attribute__((ext_vector_type(2)));
+typedef float w4_f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 w4_bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kW4Chunk = 128;         // columns of a tile
 constexpr int kW4Tile = 16;           // rows of W (outputs) of a tile
@@ -367,6 +370,165 @@ __global__ __launch_bounds__(64 * NW * KS) void w4_tiles_kernel(W4Params p) {
             }
     }
 }
+// Hundreds of rows of many outputs: 128 rows a workgroup, all of them each wave's, which takes 16 NT outputs, so that a weight is unpacked once for eight matrix
+// instructions, as (q - z) s in bf16. x goes through LDS in four buffers of 128 columns, three of them on their way; weights wait in registers as long. In LDS a row is 256
+// bytes, its 16 bytes c at place c ^ (row mod 16): fragments read one place of 16 rows.
+// A step is 32 columns, 8 NT matrix instructions in a fixed order. Between them the wave unpacks the next step's weights, two in two slots, and reads 16 rows of the next step's x as soon as
+// the last instruction on this step's has them. One wave a SIMD: its slots take some 35 cycles, twice the matrix instruction's 16 (loads of weights 18 % of the time, reads of LDS
+// 13 %, loads of x 7 %). 192 or 256 rows (two outputs' tiles a wave) and weights asked for eight slabs ahead made no difference.
+template <int GPC, bool ZERO, int NT>
+__global__ __launch_bounds__(256, 1) void w4_product_kernel(W4Params p, int row_blocks, int blocks) {
+    constexpr int MT = 8, DEEP = 4, SLAB = 128 * 256, NS = MT * NT;
+    static_assert(NT <= 4, "a step asks for one tile of weights");
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
+    const int per_xcd = gridDim.x / 8, at = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;   // the row blocks of some outputs share an XCD
+    if (at >= blocks) return;
+    const int m0 = at % row_blocks * 128, rows = min(128, p.M - m0);
+    const int tiles = (p.N + kW4Tile - 1) / kW4Tile, tile0 = (at / row_blocks * 4 + wave) * NT;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)lds)) + wave * 1024;
+    const int my_row = wave * 4 + g, my_col = (l16 ^ my_row) * 8;   // what the lane fetches: of rows my_row + 16 i
+    const uint32_t row2 = static_cast<uint32_t>(p.ldx * 2), voff = my_row * row2 + my_col * 2;
+    const uint64_t base = reinterpret_cast<uint64_t>(p.x + m0 * p.ldx);
+    const uint32_t bytes = (rows - 1) * row2 + p.K * 2;   // (rows past the end arrive as zeros)
+    w4_u32x4 rsrc;
+    uint32_t first = 0, more = 0;   // the lane's offset and that of the next load; past the end where its columns are, which would be another row's
+    auto open_x = [&](int c) {
+        const uint64_t from = base + static_cast<uint64_t>(c) * (kW4Chunk * 2);
+        rsrc.x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(from));
+        rsrc.y = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(from >> 32) & 0xffffu);
+        rsrc.z = __builtin_amdgcn_readfirstlane(c < p.chunks ? bytes - c * (kW4Chunk * 2) : 0u);
+        rsrc.w = 0x00020000u;
+        const bool there = c * kW4Chunk + my_col < p.K;
+        first = there ? voff : 0x80000000u;
+        more = there ? 16 * row2 : 0u;
+    };
+    auto load_x = [&](int buffer, int i) { w4_load_lds(rsrc, __builtin_amdgcn_readfirstlane(lds0 + buffer * SLAB + i * 4096), first + i * more); };
+    W4Piece<GPC, ZERO> piece[DEEP][NT];
+    auto load_w = [&](int c, int buffer, int t) {   // (past the end: not used)
+        W4Tile<GPC, ZERO>(p, min(tile0 + t, tiles - 1), lane).template request<false>(piece[buffer][t], min(c, p.chunks - 1));
+    };
+    w4_f32x4 acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[t][m] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < DEEP; ++c) {   // (of the last one what a step asks for)
+#pragma unroll
+        for (int t = 0; t < (c < DEEP - 1 ? NT : 1); ++t) load_w(c, c, t);
+        open_x(c);
+#pragma unroll
+        for (int i = 0; i < (c < DEEP - 1 ? MT : 2); ++i) load_x(c, i);
+    }
+    // Two weights: 1024 + q in fp16, or 1024 + 16 q where that saves a shift; times s (s / 16) less (1024 + z) s ((64 + z) s), exact in fp32, they are rounded once. (Without the
+    // product that is taken off, by 1024 + z in fp16 first, 512 x 9216 x 3072 took 45.9 us for 41.4.) `most`: whether that product was a number.
+    uint32_t magic = 0x64006400u, upper = 0, two = 0;
+    asm volatile("" : "+v"(magic));
+    float most = 0.0f;
+    w4_f32x2 pair = {0.f, 0.f};
+    float scale[2][NT], less[2][NT];
+    auto factors = [&](const W4Piece<GPC, ZERO>& of, int t, int i) {
+        const float s = of.scale(i), z = of.zero(i);
+        scale[0][t] = s;
+        less[0][t] = -(1024.0f + z) * s;
+        scale[1][t] = s * 0.0625f;
+        less[1][t] = -(64.0f + z) * s;
+        most = fmaxf(most, fabsf(less[0][t]));
+    };
+    auto take = [&](uint32_t q, int i) {   // out of a word
+        if (i == 0) upper = q >> 8;
+        two = ((i < 2 ? q : upper) & (i % 2 == 0 ? 0x000f000fu : 0x00f000f0u)) | magic;
+    };
+    auto weigh = [&](int t, int i) {
+        const w4_f16x2 h = __builtin_bit_cast(w4_f16x2, two);
+        pair = w4_f32x2{__builtin_fmaf(static_cast<float>(h.x), scale[i % 2][t], less[i % 2][t]), __builtin_fmaf(static_cast<float>(h.y), scale[i % 2][t], less[i % 2][t])};
+    };
+    auto packed = [&]() { return __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, w4_bf16x2)); };
+    w4_u32x4 w[2][NT];
+    w4_bf16x8 a[MT];
+    const char* const mine = lds + l16 * 256;
+    int place[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) place[j] = ((j * 4 + g) ^ l16) * 16;
+    // the first slab is here when no more than what was asked for behind it is missing
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((DEEP - 2) * MT + 2) : "memory");
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        factors(piece[0][t], t, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            take(piece[0][t].q[0], i);
+            weigh(t, i);
+            w[0][t][i] = packed();
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) a[m] = *reinterpret_cast<const w4_bf16x8*>(mine + m * 4096 + place[0]);
+    for (int c0 = 0; c0 < p.chunks; c0 += DEEP) {
+#pragma unroll
+        for (int b = 0; b < DEEP; ++b) {
+            const int c = c0 + b;
+            if (c >= p.chunks) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int nj = (j + 1) % 4, nb = j == 3 ? (b + 1) % DEEP : b;   // the next step
+                const int to = j == 3 ? b : (b + DEEP - 1) % DEEP, part = nj;   // the buffers of the slab that was read last get a quarter of another one a step
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    const int m = s / NT, t = s % NT;
+                    acc[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m], __builtin_bit_cast(w4_bf16x8, w[j & 1][t]), acc[t][m], 0, 0, 0);
+                    if (j == 3 && s == NT - 1) {
+                        // the next slab is here, as are all but the loads of two behind it, and everyone has read this one
+                        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((DEEP - 2) * MT) : "memory");
+                        open_x(c + DEEP);
+                    }
+                    if (t == NT - 1) a[m] = *reinterpret_cast<const w4_bf16x8*>(mine + nb * SLAB + m * 4096 + place[nj]);
+                    const int u = s / 8, i = s / 2 % 4;
+                    if (s % 2 == 0) {
+                        if (s > 0) w[nj & 1][(s - 1) / 8][(s - 1) / 2 % 4] = packed();
+                        if (i == 0 && nj * GPC % 4 == 0) factors(piece[nb][u], u, nj * GPC / 4);
+                        take(piece[nb][u].q[nj], i);
+                    } else {
+                        weigh(u, i);
+                        if (s == NS - 1) w[nj & 1][u][i] = packed();
+                    }
+                    if (s == NS / 2 && part < NT) load_w(c + (j == 3 ? DEEP : DEEP - 1), to, part);
+                    if (s == NS / 4 || s == 3 * NS / 4) load_x(to, part * 2 + (s > NS / 2));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+    }
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(most < INFINITY)) != 0, 0))
+#pragma unroll
+        for (int t = 0; t < NT; ++t) w4_again<false, GPC, ZERO, MT>(acc[t], p, min(tile0 + t, tiles - 1), m0, rows, 0, 1);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // (loads past the end; everyone is done with x)
+    // through LDS: rows of 32 NT bytes leave 16 at a time
+    constexpr int STRIDE = NT * 32 + 16;
+    char* const stage = lds + wave * (128 * STRIDE);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int n = (tile0 + t) * kW4Tile + l16;
+        const float bias = p.bias != nullptr && n < p.N ? bf2f(p.bias[n]) : 0.0f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<bf16_t*>(stage + (m * 16 + g * 4 + i) * STRIDE + t * 32 + l16 * 2) = w4_result(p, acc[t][m][i], bias);
+    }
+    __builtin_amdgcn_wave_barrier();   // LDS operations of one wave complete in order
+    const bool whole = p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+    for (int i = lane; i < rows * (2 * NT); i += 64) {
+        const int m = i / (2 * NT), v = i - m * (2 * NT), n = tile0 * kW4Tile + v * 8;
+        const Vec16<bf16_t> y = *reinterpret_cast<const Vec16<bf16_t>*>(stage + m * STRIDE + v * 16);
+        bf16_t* const out = p.y + static_cast<int64_t>(m0 + m) * p.ldy + n;
+        if (whole && n + 8 <= p.N) st16(out, y);
+        else
+            for (int e = 0; e < 8; ++e)
+                if (n + e < p.N) out[e] = y.v[e];
+    }
+}
+
 // bytes of LDS: x, one slab or two, or the parts' sums
 static int w4_tiles_lds(const W4Params& p, int held, int parts_kb) {
     const int slabs = (p.chunks + p.slab - 1) / p.slab;
@@ -493,7 +655,25 @@ static void w4_rows_launch(W4Params p, hipStream_t st) {
 #undef CALL
 }
 
-constexpr int kW4MostRows = 128;   // beyond them the weights are laid out first
+constexpr int kW4MostRows = 128;   // of the kernels that multiply whole numbers
+
+// Beyond them: 16 outputs' tiles a wave of the kernel that unpacks weights between its products, 2 or 3, or 0 where they are laid out first. One round of workgroups, one a CU,
+// that leaves less than half of the CUs idle is ahead of a pass that lays thousands of outputs' weights out. us, direct and laid out first: 256 x 9216 x 3072 33.1 and 41.1, 256 x 12288 x
+// 3072 34.3 and 49.7, 512 x 9216 x 3072 41.4 and 49.8 (3 tiles), 256 x 18432 x 8192 96 and 171, 384 x 6144 x 8192 71.3 and 70.5 (144 workgroups). Fewer workgroups: 129 x 6144 x 3072 31.5 and
+// 31.7 (96), 512 x 3072 x 3072 32.3 and 28.6 (96), 129 x 6144 x 8192 71 and 49; fewer outputs: 1000 x 3072 x 3072 35.2 and 34.0 (192), 640 x 3712 x 8192 72 and 60; two rounds: 1000 x 9216 x
+// 3072 80 and 67, 512 x 18432 x 3072 83 and 80.
+static int w4_product_tiles(const flux_linear_w4_args& a) {
+    if (a.w.N < 4608 || a.ldx < a.w.K || a.ldx >= (int64_t{1} << 23)) return 0;   // (32-bit offsets within 128 rows)
+    const int64_t row_blocks = (a.M + 127) / 128, two = row_blocks * ((a.w.N + 127) / 128), three = row_blocks * ((a.w.N + 191) / 192);
+    return two < 144 ? 0 : two <= 256 ? 2 : three <= 256 ? 3 : 0;
+}
+template <int GPC, bool ZERO>
+static void w4_product_launch(const W4Params& p, int nt, hipStream_t st) {
+    const int row_blocks = (p.M + 127) / 128, blocks = row_blocks * ((p.N + 64 * nt - 1) / (64 * nt));
+    const dim3 grid((blocks + 7) / 8 * 8);
+    if (nt == 2) hipLaunchKernelGGL((w4_product_kernel<GPC, ZERO, 2>), grid, dim3(256), 4 * 128 * 256, st, p, row_blocks, blocks);
+    else hipLaunchKernelGGL((w4_product_kernel<GPC, ZERO, 3>), grid, dim3(256), 4 * 128 * 256, st, p, row_blocks, blocks);
+}
 
 static flux_linear_args w4_linear(const flux_linear_w4_args& a, const void* w) {
     flux_linear_args l = {};
@@ -524,7 +704,7 @@ extern "C" int flux_w4_unpack(const flux_w4* w, void* out, void* stream) {
 }
 
 extern "C" int64_t flux_linear_w4_workspace_bytes(const flux_linear_w4_args* a) {
-    if (!a || a->M <= kW4MostRows || w4_check("flux_linear_w4_bf16", a->w) != FLUX_OK || a->w.N == 0 || a->w.K == 0) return 0;
+    if (!a || a->M <= kW4MostRows || w4_check("flux_linear_w4_bf16", a->w) != FLUX_OK || a->w.N == 0 || a->w.K == 0 || w4_product_tiles(*a) != 0) return 0;
     const flux_linear_args l = w4_linear(*a, a->w.q);
     return w4_weights_bytes(a->w) + flux_linear_workspace_bytes(&l);
 }
@@ -546,7 +726,8 @@ extern "C" int flux_linear_w4_bf16(const flux_linear_w4_args* a, void* ws, int64
     if (a->ldy < a->w.N && a->M > 1) return fail(FLUX_E_SHAPE, "%s: rows of y overlap", what);
     if (!aligned16(a->x) || (a->M > 1 && a->ldx % 8 != 0)) return fail(FLUX_E_ALIGN, "%s: x must be 16-byte aligned, its row stride a multiple of 8", what);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a->M > kW4MostRows) {
+    const int nt = a->M > kW4MostRows ? w4_product_tiles(*a) : 0;
+    if (a->M > kW4MostRows && nt == 0) {
         const int64_t weights = w4_weights_bytes(a->w), need = flux_linear_w4_workspace_bytes(a);
         if (!ws || reinterpret_cast<uintptr_t>(ws) % 256 != 0 || ws_bytes < need) return fail(FLUX_E_SHAPE, "%s: needs %lld bytes of 256-byte aligned workspace", what, (long long)need);
         rc = flux_w4_unpack(&a->w, ws, stream);
@@ -557,7 +738,8 @@ extern "C" int flux_linear_w4_bf16(const flux_linear_w4_args* a, void* ws, int64
     W4Params p = {static_cast<const bf16_t*>(a->x), static_cast<const w4_u32x4*>(a->w.q), static_cast<const bf16_t*>(a->w.s), static_cast<const uint8_t*>(a->w.z),
                   static_cast<const bf16_t*>(a->bias), static_cast<bf16_t*>(a->y), a->M > 1 ? a->ldx : 0, a->M > 1 ? a->ldy : 0,
                   static_cast<int>(a->M), static_cast<int>(a->w.N), static_cast<int>(a->w.K), static_cast<int>((a->w.K + kW4Chunk - 1) / kW4Chunk), 0, a->act, a->in_act == FLUX_ACT_SILU};
-#define CALL(GPC) if (p.z) w4_rows_launch<GPC, true>(p, st); else w4_rows_launch<GPC, false>(p, st)
+#define CALL(GPC) if (nt != 0 && p.z) w4_product_launch<GPC, true>(p, nt, st); else if (nt != 0) w4_product_launch<GPC, false>(p, nt, st); \
+                  else if (p.z) w4_rows_launch<GPC, true>(p, st); else w4_rows_launch<GPC, false>(p, st)
     if (a->w.group == 32) { CALL(4); }
     else if (a->w.group == 64) { CALL(2); }
     else { CALL(1); }

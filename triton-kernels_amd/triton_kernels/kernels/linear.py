@@ -372,7 +372,7 @@ def linear_w4(x: Tensor, w: W4, b: Tensor | None = None, *, activation: str = ""
     activation    : "" or "GELU", as in linear
     in_activation : "SiLU" applies x * sigmoid(x) to x on the way in; at most 8 rows
 
-    Sums are fp32 and y is rounded once; up to 128 rows the weights are what the numbers stand for, beyond them they are laid out as bf16 first, each rounded
+    Sums are fp32 and y is rounded once; up to 128 rows the weights are what the numbers stand for, beyond them each is rounded to bf16
     once. Up to 128 rows a group's sum is that of (q + 16) x without that of (zero + 16) x, which keeps what is above 2^-18 of the group's largest |x| times its
     scale. x * sigmoid(x) keeps 16 bits. What is not finite in x goes as in the formula. It is not differentiated: a gradient that reaches it raises NotImplementedError.
     """
