@@ -128,3 +128,31 @@ def test_two_operators_at_once_on_two_streams():
                 got.append(calls())
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for each in got for a, b in zip(each, want))
+
+
+def _args(M, N, K, ldx):
+    from triton_kernels import _native as nv
+    return nv.LinearW4Args(256, None, 256, nv.W4(256, 256, None, N, K, 64), M, ldx, N, 0, 0)
+
+
+def test_workspaces_of_products():
+    """Up to 128 rows, and for hundreds of rows of thousands of outputs, none; else room for the weights in bf16."""
+    from triton_kernels import _native as nv
+    need = lambda *a: nv.lib().flux_linear_w4_workspace_bytes(nv.byref(_args(*a)))  # noqa: E731
+    assert [need(128, 9216, 3072, 3072), need(256, 9216, 3072, 3072), need(512, 9216, 3072, 4096), need(0, 9216, 3072, 3072)] == [0] * 4
+    for M, N, K, ldx in ((129, 4608, 64, 64), (256, 3072, 3072, 3072), (4096, 9216, 3072, 3072), (256, 9216, 64, 2 ** 23)):
+        assert need(M, N, K, ldx) >= N * K * 2
+
+
+@pytest.mark.gpu
+def test_rows_that_lie_far_apart():
+    g = seeded(6)
+    w, rows = tk.quantize_w4(randn(g, 9216, 64), 64).to(DEV), randn(g, 130, 64, dtype=BF).to(DEV)
+    x = torch.empty(129 * 2 ** 23 + 64, dtype=BF, device=DEV).as_strided((130, 64), (2 ** 23, 1))
+    x.copy_(rows)
+    y, near = tk.linear_w4(x, w), tk.linear_w4(rows, w)
+    wf = w.dequantize().double()   # (rounded; both ways sum 64 products of it and round once)
+    want, size = rows.double() @ wf.t(), rows.double().abs() @ wf.abs().t()
+    for got in (y, near):
+        assert bool(((got.double() - want).abs() <= want.abs() * 2.0 ** -8 + size * 2 * 64 * 2.0 ** -24).all())
+    assert torch.equal(tk.linear_w4(x[:128], w), tk.linear_w4(rows[:128], w))
