@@ -156,3 +156,57 @@ def test_rows_that_lie_far_apart():
     for got in (y, near):
         assert bool(((got.double() - want).abs() <= want.abs() * 2.0 ** -8 + size * 2 * 64 * 2.0 ** -24).all())
     assert torch.equal(tk.linear_w4(x[:128], w), tk.linear_w4(rows[:128], w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_modules_in_code_that_is_traced(backend):
+    torch._dynamo.reset()
+    g = seeded(7)
+    lin = torch.nn.Linear(128, 80)
+    lin.weight.data, lin.bias.data = randn(g, 80, 128), randn(g, 80)
+    served = LinearW4.from_linear(lin, 64, True).to(DEV)
+    mod = Modulation(128, double=False)
+    mod.lin.weight.data, mod.lin.bias.data = randn(g, 384, 128), randn(g, 384)
+    mod = mod.bfloat16().quantize(32).to(DEV)
+    x = randn(g, 3, 128, dtype=BF).to(DEV)
+    with torch.no_grad():
+        assert torch.equal(torch.compile(served, backend=backend)(x * 2.0), served(x * 2.0))
+        got, want = torch.compile(mod, backend=backend)(x)[0], mod(x)[0]
+        assert torch.equal(got.scale, want.scale) and torch.equal(got.shift, want.shift) and torch.equal(got.gate, want.gate)
+    torch._dynamo.reset()
+
+
+@pytest.mark.gpu
+def test_lengths_that_change_between_replays():
+    g = seeded(8)
+    q, k, v = (randn(g, 2, h, 700, 64, dtype=BF).to(DEV) for h in (4, 2, 2))
+    lengths = torch.tensor([700, 700], dtype=torch.int32, device=DEV)
+
+    def calls(of):
+        blocks = tk.select_blocks(q, k, 3, always=1, lengths=of)
+        return blocks, tk.block_sparse_attention(q, k, v, blocks, lengths=of)
+
+    calls(lengths)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls(lengths)
+    for pair in ([700, 1], [0, 130], [64, 699], [700, 700]):
+        lengths.copy_(torch.tensor(pair, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = calls(torch.tensor(pair, dtype=torch.int32, device=DEV))
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
+def test_under_autocast_and_inference_mode():
+    g = seeded(9)
+    w, x = tk.quantize_w4(randn(g, 40, 64), 32).to(DEV), randn(g, 3, 64, dtype=BF).to(DEV)
+    q = randn(g, 1, 2, 300, 128, dtype=BF).to(DEV)
+    want = tk.linear_w4(x, w), tk.select_blocks(q, q, 2), tk.block_sparse_attention(q, q, q, tk.select_blocks(q, q, 2))
+    for mode in (torch.inference_mode(), torch.autocast("cuda", dtype=torch.float16), torch.autocast("cuda", dtype=BF)):
+        with mode:
+            got = tk.linear_w4(x, w), tk.select_blocks(q, q, 2), tk.block_sparse_attention(q, q, q, tk.select_blocks(q, q, 2))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
