@@ -107,22 +107,30 @@ class LinearGELU(nn.Linear):
 
 
 class LinearW4(nn.Module):
-    """A projection whose weight is held in 4 bits (linear_w4), for serving: its weight is no parameter. zero_points: whether groups have one."""
+    """A projection whose weight is held in 4 bits (linear_w4), for serving: its weight is no parameter. zero_points: whether groups have one;
+    activation: "" or "GELU", as in linear_w4."""
 
-    def __init__(self, in_features: int, out_features: int, bias: bool = True, group: int = 64, zero_points: bool = False, device=None):
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, group: int = 64, zero_points: bool = False, device=None, activation: str = ""):
         super().__init__()
-        self.in_features, self.out_features, self.group = in_features, out_features, group
+        assert activation in ("", "GELU"), f"an activation of linear_w4, not {activation!r}"
+        self.in_features, self.out_features, self.group, self.activation = in_features, out_features, group, activation
         w = quantize_w4(torch.zeros(out_features, in_features, device=device), group, zero_points)
         self.register_buffer("packed", w.packed)
         self.register_buffer("scale", w.scale)
         self.register_buffer("zero", w.zero)
         self.bias = nn.Parameter(torch.zeros(out_features, dtype=torch.bfloat16, device=device), requires_grad=False) if bias else None
 
+    # The projections whose forward is known here, and what it applies behind the product.
+    _ACTIVATION_OF = {nn.Linear: "", Linear: "", LinearGELU: "GELU"}
+
     @classmethod
     def from_linear(cls, linear: nn.Linear, group: int = 64, zero_points: bool = False) -> "LinearW4":
-        """The projection `linear` with its weight in 4 bits, where that lies."""
-        assert isinstance(linear, nn.Linear), f"a projection with a weight to hold in 4 bits, not {type(linear).__name__}"
-        out = cls(linear.in_features, linear.out_features, linear.bias is not None, group, zero_points, linear.weight.device)
+        """The projection `linear` with its weight in 4 bits, where that lies, and with its activation. What computes anything else (a subclass, a
+        module with hooks or a parametrised weight) is refused: that would be lost."""
+        activation = cls._ACTIVATION_OF.get(type(linear))
+        assert activation is not None, f"an nn.Linear, Linear or LinearGELU, whose weight to hold in 4 bits, not {type(linear).__name__}"
+        assert not ("forward" in linear.__dict__ or linear._forward_hooks or linear._forward_pre_hooks), f"the hooks of a {type(linear).__name__} would be lost in 4 bits: take them off first"
+        out = cls(linear.in_features, linear.out_features, linear.bias is not None, group, zero_points, linear.weight.device, activation)
         w = quantize_w4(linear.weight, group, zero_points)
         out.packed, out.scale, out.zero = w.packed, w.scale, w.zero
         if linear.bias is not None:
@@ -134,7 +142,7 @@ class LinearW4(nn.Module):
         return W4(self.packed, self.scale, self.zero, (self.out_features, self.in_features), self.group)
 
     def forward(self, input: Tensor) -> Tensor:
-        return linear_w4(input, self.weight, self.bias)
+        return linear_w4(input, self.weight, self.bias, activation=self.activation)
 
 
 class SelfAttention(nn.Module):
@@ -170,7 +178,7 @@ class Modulation(nn.Module):
     def forward(self, vec: Tensor) -> tuple[ModulationOut, ModulationOut | None]:
         if isinstance(self.lin, LinearW4):
             if self.takes_fused_silu(vec):
-                out = linear_w4(vec, self.lin.weight, self.lin.bias, in_activation="SiLU")
+                out = linear_w4(vec, self.lin.weight, self.lin.bias, activation=self.lin.activation, in_activation="SiLU")
             else:
                 out = self.lin(_silu(vec))
         elif self.takes_fused_silu(vec):
