@@ -106,3 +106,96 @@ def test_a_modulation_whose_projection_has_an_activation(rows):
         got = torch.cat((out.shift, out.scale, out.gate), -1)[:, 0]
         size = torch.nn.functional.silu(vec).float().abs() @ modulation.lin.weight.dequantize().float().abs().T
     assert bool(((got.float() - plain.float()).abs() <= 1.13 * 2 * HALF * size + 2 * HALF * plain.float().abs()).all())
+
+
+def _single(hidden=256, heads=4):
+    torch.manual_seed(0)
+    return tk.SingleStreamBlock(hidden, heads, mlp_ratio=2.0).to(BF)
+
+
+def _double(hidden=256, heads=4):
+    torch.manual_seed(0)
+    return tk.DoubleStreamBlock(hidden, heads, mlp_ratio=2.0, qkv_bias=True).to(BF)
+
+
+def _set(block, path, module):
+    *at, last = path.split(".")
+    for name in at:
+        block = getattr(block, name)
+    setattr(block, last, module)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("paths", [("linear1",), ("linear2",), ("linear1", "linear2", "modulation.lin")])
+@pytest.mark.parametrize("keep", [None, 4])   # (4: every block, by way of their selection)
+def test_single_block_with_projections_in_4_bits(paths, keep):
+    """Beside the fused block whose weights are what the numbers stand for."""
+    g = seeded(len(paths))
+    block, plain = _single(), _single()
+    _served(g, block, plain, paths)
+    block.sparse_keep = plain.sparse_keep = keep
+    x, vec = randn(g, 2, 200, 256, dtype=BF).to(DEV), randn(g, 2, 256, dtype=BF).to(DEV)
+    pe = tk.rope_table(torch.arange(200, dtype=torch.float32, device=DEV)[None, :, None], [64])
+    with torch.no_grad():
+        got, want = block(x, vec, pe), plain(x, vec, pe)
+    assert (got - want).float().pow(2).mean().sqrt() <= 3 * HALF * want.float().pow(2).mean().sqrt()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("paths", [("img_attn.qkv",), ("txt_attn.qkv",), ("img_attn.proj", "txt_attn.proj"), ("img_mlp.0",), ("txt_mlp.0",), ("img_mlp.2",), ("txt_mlp.2",),
+                                   ("img_mod.lin", "txt_mod.lin", "img_attn.qkv", "txt_attn.qkv", "img_attn.proj", "txt_attn.proj", "img_mlp.0", "img_mlp.2", "txt_mlp.0", "txt_mlp.2")])
+@pytest.mark.parametrize("B", [1, 2])
+def test_double_block_with_projections_in_4_bits(paths, B):
+    g = seeded(len(paths))
+    block, plain = _double(), _double()
+    _served(g, block, plain, paths)
+    img, txt, vec = randn(g, B, 150, 256, dtype=BF).to(DEV), randn(g, B, 40, 256, dtype=BF).to(DEV), randn(g, B, 256, dtype=BF).to(DEV)
+    pe = tk.rope_table(torch.arange(190, dtype=torch.float32, device=DEV)[None, :, None], [64])
+    with torch.no_grad():
+        for got, want in zip(block(img, txt, vec, pe), plain(img, txt, vec, pe)):
+            assert (got - want).float().pow(2).mean().sqrt() <= 3 * HALF * want.float().pow(2).mean().sqrt()
+
+
+def _served(g, block, plain, paths):
+    """The projections at `paths`: in 4 bits with scales that are powers of two in `block`, whose weights bf16 holds as they are, and as such in `plain`."""
+    for path in paths:
+        lin = block.get_submodule(path)
+        n, k = lin.weight.shape
+        q, scale = torch.randint(0, 16, (n, k), generator=g), torch.full((n, k // 64), 2.0 ** -7, dtype=BF)
+        w4 = LinearW4.from_linear(lin, 64)
+        w = tk.pack_w4(q, scale)
+        w4.packed, w4.scale = w.packed, w.scale
+        _set(block, path, w4)
+        plain.get_submodule(path).weight.data = ((q - 8) * 2.0 ** -7).to(BF)
+    block.to(DEV), plain.to(DEV)
+
+
+@pytest.mark.gpu
+def test_a_block_wholly_in_4_bits_in_a_graph():
+    g = seeded(6)
+    block, plain = _double(), _double()
+    _served(g, block, plain, ("img_mod.lin", "txt_mod.lin", "img_attn.qkv", "txt_attn.qkv", "img_attn.proj", "txt_attn.proj", "img_mlp.0", "img_mlp.2", "txt_mlp.0", "txt_mlp.2"))
+    img, txt, vec = randn(g, 1, 150, 256, dtype=BF).to(DEV), randn(g, 1, 40, 256, dtype=BF).to(DEV), randn(g, 1, 256, dtype=BF).to(DEV)
+    pe = tk.rope_table(torch.arange(190, dtype=torch.float32, device=DEV)[None, :, None], [64])
+    with torch.no_grad():
+        block(img, txt, vec, pe)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = block(img, txt, vec, pe)
+        for _ in range(3):
+            img.copy_(randn(g, 1, 150, 256, dtype=BF))
+            vec.copy_(randn(g, 1, 256, dtype=BF))
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(out, block(img, txt, vec, pe)))
+
+
+def test_which_blocks_run_fused():
+    """On the CPU: a block with a projection in 4 bits, beside its modulations, takes its operators one at a time."""
+    for make, mods, rest in ((_single, ("modulation.lin",), ("linear1", "linear2")),
+                             (_double, ("img_mod.lin", "txt_mod.lin"), ("img_attn.qkv", "txt_attn.qkv", "img_attn.proj", "txt_attn.proj", "img_mlp.0", "img_mlp.2", "txt_mlp.0", "txt_mlp.2"))):
+        for path in mods + rest:
+            block = make()
+            assert block._projections_in_4_bits() is False
+            _set(block, path, LinearW4.from_linear(block.get_submodule(path)))
+            assert block._projections_in_4_bits() is (path in rest)

@@ -108,7 +108,7 @@ class LinearGELU(nn.Linear):
 
 class LinearW4(nn.Module):
     """A projection whose weight is held in 4 bits (linear_w4), for serving: its weight is no parameter. zero_points: whether groups have one;
-    activation: "" or "GELU", as in linear_w4."""
+    activation: "" or "GELU", as in linear_w4. Any projection of a block may be one; with any but a modulation's the block takes its operators one at a time."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, group: int = 64, zero_points: bool = False, device=None, activation: str = ""):
         super().__init__()
@@ -215,6 +215,11 @@ def _fusable(*tensors: Tensor) -> bool:
     return all(t.is_cuda and t.dtype == torch.bfloat16 for t in tensors)
 
 
+def _in_4_bits(module: nn.Module, one: str, other: str) -> bool:
+    at = module._modules   # (looked at in front of every pass: as attributes they take ten times as long)
+    return isinstance(at.get(one), LinearW4) or isinstance(at.get(other), LinearW4)
+
+
 class SingleStreamBlock(nn.Module):
     """DiT block with parallel attention and MLP branches (https://arxiv.org/abs/2302.05442)."""
 
@@ -254,7 +259,7 @@ class SingleStreamBlock(nn.Module):
         hook("layer_norm", "begin")
         x_mod = layer_norm_modulation(x, mod.scale, mod.shift)
         hook("layer_norm", "end")
-        if self.fused and _fusable(x, self.linear1.weight, self.linear2.weight, self.norm.query_norm.scale):
+        if self.fused and not self._projections_in_4_bits() and _fusable(x, self.linear1.weight, self.linear2.weight, self.norm.query_norm.scale):
             return self._forward_fused(x, x_mod, mod, pe)
         hid = self.hidden_size
         y1 = self.linear1(x_mod)
@@ -263,6 +268,10 @@ class SingleStreamBlock(nn.Module):
         attn = attention(q, k, v, pe, self.sparse_keep, self.sparse_always)
         both = torch.cat((attn, _gelu_tanh(y1[..., 3 * hid:])), 2)
         return _gated_residual(x, mod.gate, self.linear2(both))
+
+    def _projections_in_4_bits(self) -> bool:
+        """Whether a projection is held in 4 bits: linear_w4 has none of the epilogues that the fused forward is made of."""
+        return _in_4_bits(self, "linear1", "linear2")
 
     def _forward_fused(self, x: Tensor, x_mod: Tensor, mod: ModulationOut, pe: Tensor) -> Tensor:
         B, L, hid = x.shape
@@ -333,7 +342,7 @@ class DoubleStreamBlock(nn.Module):
     def forward(self, img: Tensor, txt: Tensor, vec: Tensor, pe: Tensor) -> tuple[Tensor, Tensor]:
         H = self.num_heads
         Lt = txt.shape[1]
-        fused = self.fused and _fusable(img, txt, self.img_attn.qkv.weight, self.img_attn.norm.query_norm.scale)
+        fused = self.fused and not self._projections_in_4_bits() and _fusable(img, txt, self.img_attn.qkv.weight, self.img_attn.norm.query_norm.scale)
         if fused:
             return self._forward_fused(img, txt, vec, pe)
 
@@ -350,6 +359,12 @@ class DoubleStreamBlock(nn.Module):
         img = self._stream_tail(img, attn[:, Lt:], img_mod1, img_mod2, self.img_attn.proj, self.img_mlp)
         txt = self._stream_tail(txt, attn[:, :Lt], txt_mod1, txt_mod2, self.txt_attn.proj, self.txt_mlp)
         return img, txt
+
+    def _projections_in_4_bits(self) -> bool:
+        """As in SingleStreamBlock."""
+        at = self._modules
+        return (_in_4_bits(at["img_attn"], "qkv", "proj") or _in_4_bits(at["txt_attn"], "qkv", "proj")
+                or _in_4_bits(at["img_mlp"], "0", "2") or _in_4_bits(at["txt_mlp"], "0", "2"))
 
     def _forward_fused(self, img: Tensor, txt: Tensor, vec: Tensor, pe: Tensor) -> tuple[Tensor, Tensor]:
         """The text rows are a small part of the work (a ninth at 4096 + 512 tokens, a fifth at 1024 + 256):
