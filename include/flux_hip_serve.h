@@ -12,7 +12,7 @@
 extern "C" {
 #endif
 
-#define FLUX_SERVE_ABI_VERSION 1
+#define FLUX_SERVE_ABI_VERSION 2
 int flux_serve_abi_version(void);
 
 /* ---------------------------------------------------------------------------------------------
@@ -50,7 +50,8 @@ int flux_w4_unpack(const flux_w4* w, void* out, void* stream);
  * q [B, Hq, Lq, D] and k [B, Hk, Lk, D] bf16 with strides as in flux_src4, Hq a multiple of Hk (query head h reads key head h / (Hq / Hk)), D 64 or 128. For each
  * block of FLUX_QUERY_BLOCK queries (the last may be shorter) the scores of the blocks of FLUX_KEY_BLOCK keys are mean(q) . mean(k), formed in 64 bits;
  * the `keep` largest (or all, where there are no more) are chosen, the lower number among equals, a NaN below everything, the first `always` blocks (up to `keep` of them) in any case.
- * lengths (int32 [B], or null): keys from lengths[b] on are not there; below 0 counts as 0, beyond Lk as Lk.
+ * lengths (int32 [B], or null): keys from lengths[b] on are not there; below 0 counts as 0, beyond Lk as Lk. q_lengths (the same for q and Lq): queries from
+ * q_lengths[b] on are in no mean, and a block of none but them names nothing, -1 throughout. Without it all Lq rows of q are in their blocks' means.
  * blocks receives int32 [B, Hq, ceil(Lq / 128), min(keep, ceil(Lk / 64))]: the chosen numbers in ascending order, -1 behind them.
  * The workspace (flux_select_blocks_workspace_bytes; 256-byte aligned) holds the means and scores.
  * ------------------------------------------------------------------------------------------- */
@@ -60,6 +61,7 @@ typedef struct flux_select_blocks_args {
     const int32_t* lengths; int32_t* blocks;
     int64_t B, Hq, Hk, Lq, Lk, keep, always;
     int32_t D;
+    const int32_t* q_lengths;
 } flux_select_blocks_args;
 int64_t flux_select_blocks_workspace_bytes(const flux_select_blocks_args* args);
 int flux_select_blocks(const flux_select_blocks_args* args, void* workspace, int64_t workspace_bytes, void* stream);

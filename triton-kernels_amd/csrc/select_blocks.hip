@@ -2,6 +2,8 @@
 //
 //   mq[i] = mean of block i's queries, mk[j] = mean of block j's keys, score[i, j] = mq[i] . mk[j]
 //
+// over the queries and keys in front of their sequences' ends.
+//
 // Everything behind the reads of q and k is formed in 64 bits: a row's scores lie close together, and which of two neighbours in their order is chosen must not
 // go with the order of a sum. That is cheap: the sums of the means are an addition a value beside its two bytes, and the products 2 D operations for 64 x 128 x D of
 // the attention itself, on the matrix cores (16x16x4). Bound by reading q and k once.
@@ -14,13 +16,13 @@ namespace flux {
 
 struct SelectParams {
     flux_src4 q, k;
-    const int32_t* lengths; int32_t* blocks;
+    const int32_t* lengths; const int32_t* q_lengths; int32_t* blocks;
     double* mq; double* mk; double* scores;
     int B, Hq, Hk, Lq, Lk, nq, nk, keep, width, always;   // width: entries of a list
     int64_t groups;                                      // of 16 query blocks of a (batch, head)
 };
 
-__device__ __forceinline__ int select_length(const SelectParams& p, int b) { return p.lengths ? min(max(p.lengths[b], 0), p.Lk) : p.Lk; }
+__device__ __forceinline__ int select_length(const int32_t* lengths, int b, int most) { return lengths ? min(max(lengths[b], 0), most) : most; }
 
 // A workgroup takes one block of tokens; a thread 8 columns of every (2048 / D)th row, all requested at once.
 template <int D>
@@ -32,8 +34,8 @@ __global__ __launch_bounds__(256) void block_means_kernel(SelectParams p) {
     const int64_t at = is_q ? blockIdx.x : blockIdx.x - q_blocks;
     const int n = is_q ? p.nq : p.nk, H = is_q ? p.Hq : p.Hk, size = is_q ? FLUX_QUERY_BLOCK : FLUX_KEY_BLOCK;
     const int blk = static_cast<int>(at % n), h = static_cast<int>(at / n % H), b = static_cast<int>(at / n / H);
-    const int rows = min(size, (is_q ? p.Lq : select_length(p, b)) - blk * size);
-    if (rows <= 0) return;   // (a block of keys that is not there)
+    const int rows = min(size, select_length(is_q ? p.q_lengths : p.lengths, b, is_q ? p.Lq : p.Lk) - blk * size);
+    if (rows <= 0) return;   // (a block that is not there)
     const flux_src4 src = is_q ? p.q : p.k;
     const int c = threadIdx.x % CH, rg = threadIdx.x / CH;
     const bf16_t* const base = static_cast<const bf16_t*>(src.ptr) + b * src.sb + h * src.sh + static_cast<int64_t>(blk) * size * src.sl + c * 8;
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(64 * WAVES, MOST > 512 ? 2 : 4) void select_rows_ke
     for (int64_t at = blockIdx.x % 8 * per_xcd + blockIdx.x / 8; at < p.groups; at += gridDim.x) {
         const int64_t bh = at / per_head;
         const int i0 = static_cast<int>(at % per_head) * 16, b = static_cast<int>(bh / p.Hq), h = static_cast<int>(bh % p.Hq);
-        const int have = (select_length(p, b) + FLUX_KEY_BLOCK - 1) / FLUX_KEY_BLOCK;
+        const int have = (select_length(p.lengths, b, p.Lk) + FLUX_KEY_BLOCK - 1) / FLUX_KEY_BLOCK, queries = select_length(p.q_lengths, b, p.Lq);
         const double* const mq = p.mq + (bh * p.nq + min(i0 + l16, p.nq - 1)) * D + g * 2;
         const double* const mk = p.mk + (static_cast<int64_t>(b) * p.Hk + h / (p.Hq / p.Hk)) * p.nk * D + g * 2;
         const int always = min(p.always, min(p.keep, have));
@@ -199,7 +201,9 @@ __global__ __launch_bounds__(64 * WAVES, MOST > 512 ? 2 : 4) void select_rows_ke
         __syncthreads();
         for (int r = wave; r < 16 && i0 + r < p.nq; r += WAVES) {
             SelectRow row = {p.blocks + (bh * p.nq + i0 + r) * p.width, have, p.keep, always, p.width, lane};
-            if (all) {
+            if ((i0 + r) * FLUX_QUERY_BLOCK >= queries) {   // (its mean was not written: a row of the product that goes nowhere)
+                row.rest();
+            } else if (all) {
                 for (int i = 0; i < min(have, p.keep); i += 64) row.take(i, i + lane < min(have, p.keep));
                 row.rest();
             } else if constexpr (MOST == 0) {
@@ -232,7 +236,7 @@ static int read_select_args(const flux_select_blocks_args* a, SelectParams& p, b
     if (nothing) return FLUX_OK;
     if (nk > FLUX_SELECT_MOST_BLOCKS) return fail(FLUX_E_UNSUPPORTED, "%s: %lld blocks of keys, at most %d", what, (long long)nk, FLUX_SELECT_MOST_BLOCKS);
     if (a->B > 0x7fffffff / 64 || a->Hq > 0x7fffffff / 64 / a->B || a->B * a->Hq > 0x7fffffff / 512 / (nq + nk)) return fail(FLUX_E_SHAPE, "%s: problem too large", what);
-    p = {a->q, a->k, a->lengths, a->blocks, nullptr, nullptr, nullptr, (int)a->B, (int)a->Hq, (int)a->Hk, (int)a->Lq, (int)a->Lk, (int)nq, (int)nk, (int)width, (int)width,
+    p = {a->q, a->k, a->lengths, a->q_lengths, a->blocks, nullptr, nullptr, nullptr, (int)a->B, (int)a->Hq, (int)a->Hk, (int)a->Lq, (int)a->Lk, (int)nq, (int)nk, (int)width, (int)width,
          (int)std::min(a->always, nk), a->B * a->Hq * ((nq + 15) / 16)};
     need = mean_bytes(a->B * a->Hq * nq, a->D) + mean_bytes(a->B * a->Hk * nk, a->D);
     if (nk > kSelectNear) need += std::min<int64_t>((p.groups + 7) / 8 * 8, kSelectFarGroups) * 16 * ((nk + 15) / 16 * 16) * 8;

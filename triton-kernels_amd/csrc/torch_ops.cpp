@@ -1117,6 +1117,8 @@ bool recorded(std::initializer_list<const Tensor*> operands) {
 
 // int32 numbers beside `beside`, or none
 bool numbers(const Tensor* t, const Tensor& beside) { return !t || (t->scalar_type() == at::kInt && t->device() == beside.device() && t->is_contiguous()); }
+// The same, one for each batch element of q.
+bool each_batch(const Tensor* t, const Tensor& q) { return numbers(t, q) && (!t || (t->dim() == 1 && t->numel() == q.size(0))); }
 
 // linear_w4(x, packed, scale, zero or None, b or None, N, K, group, activation, in_activation)
 PyObject* py_linear_w4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -1157,24 +1159,25 @@ bool sparse_views(const Tensor& q, const Tensor& k) {
 }
 constexpr int64_t blocks_of(int64_t n, int64_t size) { return (n + size - 1) / size; }
 
-// select_blocks(q, k, keep, always, lengths or None)
+// select_blocks(q, k, keep, always, lengths or None, q_lengths or None)
 PyObject* py_select_blocks(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(nargs == 5, "select_blocks takes 5 arguments");
-    const Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *lengths;
+    TORCH_CHECK(nargs == 6, "select_blocks takes 6 arguments");
+    const Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *lengths, *q_lengths;
     int64_t keep, always;
-    if (!q || !k || !whole_number(args[2], keep) || !whole_number(args[3], always) || !optional_tensor(args[4], lengths) || !quiet() || !sparse_views(*q, *k) || keep <= 0 ||
-        !numbers(lengths, *q) || (lengths && (lengths->dim() != 1 || lengths->numel() != q->size(0))))
+    if (!q || !k || !whole_number(args[2], keep) || !whole_number(args[3], always) || !optional_tensor(args[4], lengths) || !optional_tensor(args[5], q_lengths) || !quiet() ||
+        !sparse_views(*q, *k) || keep <= 0 || !each_batch(lengths, *q) || !each_batch(q_lengths, *q))
         Py_RETURN_NONE;
     Tensor blocks;
     int rc;
     {
-        const Tensor qa = *q, ka = *k, la = lengths ? *lengths : Tensor();
+        const Tensor qa = *q, ka = *k, la = lengths ? *lengths : Tensor(), ends = q_lengths ? *q_lengths : Tensor();
         const WithoutInterpreter free;
         const c10::DeviceGuard guard(qa.device());
         blocks = empty({qa.size(0), qa.size(1), blocks_of(qa.size(2), FLUX_QUERY_BLOCK), std::min(keep, blocks_of(ka.size(2), FLUX_KEY_BLOCK))}, at::kInt, qa);
         const flux_select_blocks_args a = {source(qa), source(ka), la.defined() ? static_cast<const int32_t*>(la.data_ptr()) : nullptr, static_cast<int32_t*>(blocks.data_ptr()),
-                                           qa.size(0), qa.size(1), ka.size(1), qa.size(2), ka.size(2), keep, always, static_cast<int32_t>(qa.size(3))};
+                                           qa.size(0), qa.size(1), ka.size(1), qa.size(2), ka.size(2), keep, always, static_cast<int32_t>(qa.size(3)),
+                                           ends.defined() ? static_cast<const int32_t*>(ends.data_ptr()) : nullptr};
         const int64_t need = flux_select_blocks_workspace_bytes(&a);
         const Tensor ws = need ? empty({need}, at::kByte, qa) : Tensor();
         rc = flux_select_blocks(&a, need ? ws.data_ptr() : nullptr, need, stream_of(qa));
@@ -1192,7 +1195,7 @@ PyObject* py_block_sparse_attention(PyObject*, PyObject* const* args, Py_ssize_t
     const Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *v = tensor_of(args[2]), *blocks = tensor_of(args[3]), *lengths, *out;
     if (!q || !k || !v || !blocks || !optional_tensor(args[5], lengths) || !optional_tensor(args[6], out) || !quiet() || recorded({q, k, v, out}) || !sparse_views(*q, *k) || !sparse_views(*q, *v) ||
         k->sizes() != v->sizes() || !numbers(blocks, *q) || blocks->dim() != 4 || blocks->size(0) != q->size(0) || blocks->size(1) != q->size(1) ||
-        blocks->size(2) != blocks_of(q->size(2), FLUX_QUERY_BLOCK) || !numbers(lengths, *q) || (lengths && (lengths->dim() != 1 || lengths->numel() != q->size(0))) ||
+        blocks->size(2) != blocks_of(q->size(2), FLUX_QUERY_BLOCK) || !each_batch(lengths, *q) ||
         (out && (out->sizes() != q->sizes() || !same_kind(*q, *out) || out->stride(3) != 1)))
         Py_RETURN_NONE;
     double scale = 1.0 / std::sqrt(static_cast<double>(q->size(3)));

@@ -155,6 +155,7 @@ class SelectBlocksArgs(Structure):
     _fields_ = [
         ("q", Src4), ("k", Src4), ("lengths", c_void_p), ("blocks", c_void_p),
         ("B", c_int64), ("Hq", c_int64), ("Hk", c_int64), ("Lq", c_int64), ("Lk", c_int64), ("keep", c_int64), ("always", c_int64), ("D", c_int32),
+        ("q_lengths", c_void_p),
     ]
 
 
@@ -217,7 +218,7 @@ TUNE_SIGNATURES = {
 }
 
 # The same for include/flux_hip_serve.h.
-SERVE_ABI_VERSION = 1
+SERVE_ABI_VERSION = 2
 SERVE_SIGNATURES = {
     "flux_serve_abi_version": (c_int32, []),
     "flux_linear_w4_workspace_bytes": (c_int64, [POINTER(LinearW4Args)]),

@@ -9,7 +9,7 @@ _QUERIES, _KEYS = 128, 64   # of a block
 
 
 def _seen(k: Tensor, lengths: Tensor | None) -> Tensor:
-    """[B, Lk]: the keys that are there."""
+    """[B, L]: the keys (or queries) that are there."""
     end = torch.full((k.shape[0],), k.shape[2], device=k.device) if lengths is None else lengths
     return torch.arange(k.shape[2], device=k.device) < end[:, None]
 
@@ -23,14 +23,14 @@ def _block_means(x: Tensor, size: int, seen: Tensor) -> tuple[Tensor, Tensor]:
     return rows.sum(3) / count.clamp(min=1)[:, None, :, None], count
 
 
-def select_blocks_torch(q: Tensor, k: Tensor, keep: int, always: int = 0, lengths: Tensor | None = None) -> Tensor:
-    mq, _ = _block_means(q, _QUERIES, _seen(q, None))
+def select_blocks_torch(q: Tensor, k: Tensor, keep: int, always: int = 0, lengths: Tensor | None = None, q_lengths: Tensor | None = None) -> Tensor:
+    mq, queries = _block_means(q, _QUERIES, _seen(q, q_lengths))
     mk, count = _block_means(k, _KEYS, _seen(k, lengths))
     score = mq @ mk.repeat_interleave(q.shape[1] // k.shape[1], 1).transpose(2, 3).contiguous()
     score = torch.where(score.isnan(), -math.inf, score)
     score[..., :always] = math.inf
     keep, blocks = min(keep, score.shape[-1]), score.shape[-1]
-    there = (count > 0)[:, None, None].expand_as(score)
+    there = ((queries > 0)[:, None, :, None] & (count > 0)[:, None, None]).expand_as(score)
     # those that are there in front, in the order of their scores
     order = torch.argsort(score, dim=-1, descending=True, stable=True)
     order = order.gather(-1, torch.argsort(there.gather(-1, order).int(), dim=-1, descending=True, stable=True))[..., :keep]

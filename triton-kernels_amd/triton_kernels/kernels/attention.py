@@ -108,21 +108,24 @@ def _sparse_shapes(name: str, q: Tensor, k: Tensor) -> tuple[int, int, int, int,
     return B, Hq, Hk, Lq, Lk, D
 
 
-def select_blocks(q: Tensor, k: Tensor, keep: int, *, always: int = 0, lengths: Tensor | None = None) -> Tensor:
+def select_blocks(q: Tensor, k: Tensor, keep: int, *, always: int = 0, lengths: Tensor | None = None, q_lengths: Tensor | None = None) -> Tensor:
     """The blocks of 64 keys that each block of 128 queries attends to: int32 [B, Hq, ceil(Lq / 128), min(keep, ceil(Lk / 64))].
 
-    q, k    : bf16 [B, Hq, Lq, D] and [B, Hk, Lk, D] views, heads of 64 or 128; Hq is a multiple of Hk, query head h reads key head h // (Hq // Hk).
-              Up to 16384 blocks of keys
-    keep    : how many blocks; all of them where there are no more
-    always  : the first `always` blocks (as many of them as `keep` has room for) are among them in any case: the text in front of an image
-    lengths : whole numbers [B] on the GPU, or None: keys from lengths[b] on are not there
+    q, k      : bf16 [B, Hq, Lq, D] and [B, Hk, Lk, D] views, heads of 64 or 128; Hq is a multiple of Hk, query head h reads key head h // (Hq // Hk).
+                Up to 16384 blocks of keys
+    keep      : how many blocks; all of them where there are no more
+    always    : the first `always` blocks (as many of them as `keep` has room for) are among them in any case: the text in front of an image
+    lengths   : whole numbers [B] on the GPU, or None: keys from lengths[b] on are not there
+    q_lengths : the same for q: rows from q_lengths[b] on are in no mean, and a block of none but them names nothing (-1 throughout). None: all Lq rows
+                are queries. In a padded batch that attends to itself it is `lengths` once more; without it what the padding holds has a share in the
+                list of the block that it shares with the last queries, and a NaN there gives that block the lowest numbers
 
     A block's score is the product of the queries' mean and the mean of its keys, both formed in 64 bits, so that the choice does not go with rounding; the
     lower number goes first among equals, a NaN comes last. The numbers ascend; where a sequence has fewer blocks, -1 stands behind them. Not differentiated.
     """
     if is_dynamo_compiling():
-        return torch.compiler.disable(select_blocks)(q, k, keep, always=always, lengths=lengths)
-    blocks = nv.ops().select_blocks(q, k, keep, always, lengths)
+        return torch.compiler.disable(select_blocks)(q, k, keep, always=always, lengths=lengths, q_lengths=q_lengths)
+    blocks = nv.ops().select_blocks(q, k, keep, always, lengths, q_lengths)
     if blocks is not None:
         return blocks
     B, Hq, Hk, Lq, Lk, D = _sparse_shapes("select_blocks", q, k)
@@ -130,14 +133,14 @@ def select_blocks(q: Tensor, k: Tensor, keep: int, *, always: int = 0, lengths: 
         raise TypeError("select_blocks: the HIP kernel takes bfloat16 q, k")
     keep, always = int(keep), int(always)
     assert keep >= 0 and always >= 0, f"select_blocks: keep and always are counts, not {keep} and {always}"
-    dev = nv.require_gpu(q, k, lengths)
-    lengths = _lengths(lengths, B, dev, Lk)
+    dev = nv.require_gpu(q, k, lengths, q_lengths)
+    lengths, q_lengths = _lengths(lengths, B, dev, Lk), _lengths(q_lengths, B, dev, Lq)
     q, k = _bhld_view(q.detach()), _bhld_view(k.detach())
     keep, always = (min(n, -(-Lk // KEY_BLOCK)) for n in (keep, always))   # (a count may be beyond what the library's arguments hold)
     blocks = torch.empty((B, Hq, -(-Lq // QUERY_BLOCK), keep), dtype=torch.int32, device=dev)
     if blocks.numel() == 0:
         return blocks
-    a = nv.SelectBlocksArgs(nv.src4(q), nv.src4(k), nv.ptr(lengths), blocks.data_ptr(), B, Hq, Hk, Lq, Lk, keep, always, D)
+    a = nv.SelectBlocksArgs(nv.src4(q), nv.src4(k), nv.ptr(lengths), blocks.data_ptr(), B, Hq, Hk, Lq, Lk, keep, always, D, nv.ptr(q_lengths))
     with nv.on_device(dev):
         need = nv.lib().flux_select_blocks_workspace_bytes(nv.byref(a))
         ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
