@@ -7,6 +7,7 @@ import math
 
 import torch
 from torch import Tensor
+from torch.autograd.forward_ad import unpack_dual
 from torch.compiler import is_dynamo_compiling
 
 from triton_kernels import _native as nv
@@ -210,5 +211,7 @@ def block_sparse_attention(q: Tensor, k: Tensor, v: Tensor, blocks: Tensor, sm_s
         return o
     if out is not None:
         assert not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, out))), "block_sparse_attention: a result that goes to `out` is not differentiated"
+        if any(unpack_dual(t).tangent is not None for t in (q, k, v, out)):
+            raise NotImplementedError("block_sparse_attention has no forward-mode derivative")
         return _launch_sparse(q, k, v, blocks, sm_scale, lengths, out)
     return _block_sparse_attention.apply(q, k, v, blocks, sm_scale, lengths, None)
