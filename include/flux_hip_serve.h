@@ -30,8 +30,8 @@ typedef struct flux_w4 {
 
 /* y[m] = act(f(x[m]) W^T + bias): x [M, K] bf16 (row stride ldx), bias [N] bf16 or null, y [M, N] bf16 (row stride ldy); act is FLUX_ACT_NONE or
  * FLUX_ACT_GELU_TANH, in_act FLUX_ACT_NONE or (up to 8 rows) FLUX_ACT_SILU, f(x) = x sigmoid(x). fp32 sums, rounded once; f(x) is held to 2^-16 of its
- * value. Up to 128 rows a group's sum is that of (q + 16) x without that of (z + 16) x, which keeps what is above 2^-18 of the group's largest |x| s. Beyond
- * them each weight is rounded to bf16 once (2^-8 of it), and ldx is at least K: some hundreds of rows of thousands of outputs take them in registers, others lay them
+ * value. Up to 128 rows a group's sum is that of (q + 16) x less that of (z + 16) x, both in fp32: what they lose is some 2^-23 of the group's sum of (32 + q + z) |x| s,
+ * also where q = z leaves nothing of the largest x. Beyond them each weight is rounded to bf16 once (2^-8 of it), and ldx is at least K: some hundreds of rows of thousands of outputs take them in registers, others lay them
  * out in the workspace (flux_linear_w4_workspace_bytes, 0 for all the others; 256-byte aligned, the launch's own until it has run) in front of flux_linear_bf16. */
 typedef struct flux_linear_w4_args {
     const void* x; const void* bias; void* y;

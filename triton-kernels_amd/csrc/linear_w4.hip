@@ -103,7 +103,8 @@ __device__ __forceinline__ void w4_silu(Vec16<bf16_t>& x, Vec16<bf16_t>& lo) {
 }
 
 // acc += s (q - z) x over one chunk, for MT times 16 rows of x, the lane's `row` bytes behind `a`: the sum of (16 + q) x without (16 + z) times the sum of x, which the
-// matrix cores form beside it. `peak` takes the largest of these sums: what goes with it is lost to 2^-23 of it, and where x is not finite it leaves a NaN or an infinity.
+// matrix cores form beside it. Both sums are rounded: some 2^-23 of the sum of (32 + q + z) |x| is lost, however little of it
+// is left. `peak` takes the largest sum of x: where x is not finite it leaves a NaN or an infinity.
 template <int GPC, bool ZERO, int MT>
 __device__ __forceinline__ void w4_chunk(w4_f32x4 (&acc)[MT], const W4Piece<GPC, ZERO>& w, const char* a, const int (&row)[MT], uint32_t sixteens, float& peak) {
     const w4_f32x4 none = {0.f, 0.f, 0.f, 0.f};

@@ -373,8 +373,8 @@ def linear_w4(x: Tensor, w: W4, b: Tensor | None = None, *, activation: str = ""
     in_activation : "SiLU" applies x * sigmoid(x) to x on the way in; at most 8 rows
 
     Sums are fp32 and y is rounded once; up to 128 rows the weights are what the numbers stand for, beyond them each is rounded to bf16
-    once. Up to 128 rows a group's sum is that of (q + 16) x without that of (zero + 16) x, which keeps what is above 2^-18 of the group's largest |x| times its
-    scale. x * sigmoid(x) keeps 16 bits. What is not finite in x goes as in the formula. It is not differentiated: a gradient that reaches it raises NotImplementedError.
+    once. Up to 128 rows a group's sum is that of (q + 16) x less that of (zero + 16) x, both in fp32: what they lose is some 2^-23 of the sum of
+    (32 + q + zero) |x| times the scale over the group, also where q = zero leaves nothing of the largest x. x * sigmoid(x) keeps 16 bits. What is not finite in x goes as in the formula. It is not differentiated: a gradient that reaches it raises NotImplementedError.
     """
     if is_dynamo_compiling():
         return torch.compiler.disable(linear_w4)(x, w, b, activation=activation, in_activation=in_activation)
