@@ -1,0 +1,27 @@
+"""Weights in 4 bits at the edges of what they may be."""
+import pytest
+import torch
+
+import triton_kernels as tk
+from util import DEV, randn, seeded
+
+BF = torch.bfloat16
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.uint16, torch.uint32, torch.uint64])
+def test_numbers_of_every_whole_type(dtype, device):
+    g = seeded(1)
+    q, zero, scale = torch.randint(0, 16, (20, 96), generator=g), torch.randint(0, 16, (20, 3), generator=g), torch.rand(20, 3, generator=g).to(BF)
+    q, zero, scale = q.to(device), zero.to(device), scale.to(device)
+    w = tk.pack_w4(q.to(dtype), scale, zero.to(dtype))
+    want = tk.pack_w4(q, scale, zero)
+    assert torch.equal(w.packed, want.packed) and torch.equal(w.zero, want.zero) and torch.equal(w.scale, want.scale)
+    for bad in ((q + 16).to(dtype), (q * 0 + 127).to(dtype)):
+        with pytest.raises(ValueError):
+            tk.pack_w4(bad, scale)
+        with pytest.raises(ValueError):
+            tk.pack_w4(q, scale, bad[:, :3])
+    if dtype == torch.uint64:
+        with pytest.raises(ValueError):
+            tk.pack_w4(torch.full((20, 96), 2 ** 64 - 1, dtype=dtype).to(device), scale)

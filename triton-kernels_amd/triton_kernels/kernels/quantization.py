@@ -85,6 +85,8 @@ def pack_w4(q: Tensor, scale: Tensor, zero: Tensor | None = None) -> W4:
             continue
         if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
             raise TypeError(f"unsupported dtype {t.dtype} of 4-bit numbers")
+        if t.dtype in (torch.uint16, torch.uint32, torch.uint64):   # (these have no smallest and largest; 2^63 and more are below 0 then)
+            t = t.to(torch.int64)
         if t.numel() and not 0 <= int(t.min()) <= int(t.max()) <= 15:
             raise ValueError("4-bit numbers are 0 .. 15")
     assert zero is None or zero.shape == scale.shape, f"zero is {tuple(scale.shape)} as scale, not {tuple(zero.shape)}"
