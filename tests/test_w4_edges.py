@@ -25,3 +25,21 @@ def test_numbers_of_every_whole_type(dtype, device):
     if dtype == torch.uint64:
         with pytest.raises(ValueError):
             tk.pack_w4(torch.full((20, 96), 2 ** 64 - 1, dtype=dtype).to(device), scale)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_no_outputs(zeros):
+    w = tk.quantize_w4(torch.zeros(0, 96), 32, zeros)
+    assert w.shape == (0, 96) and w.packed.shape == (0, 1, 1024) and w.scale.shape == (0, 1, 16, 4)
+    q, scale, zero = w.unpack()
+    assert q.shape == (0, 96) and scale.shape == (0, 3) and (zero.shape == (0, 3) if zeros else zero is None)
+    again = tk.pack_w4(q, scale, zero)
+    assert again.shape == w.shape and again.packed.shape == w.packed.shape
+
+
+@pytest.mark.gpu
+def test_products_without_outputs():
+    w = tk.quantize_w4(torch.zeros(0, 96, device=DEV), 32)
+    for rows in (0, 1, 40, 200):
+        assert tk.linear_w4(torch.zeros(rows, 96, dtype=BF, device=DEV), w).shape == (rows, 0)
+    assert w.dequantize().shape == (0, 96)

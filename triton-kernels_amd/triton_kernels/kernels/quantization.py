@@ -50,7 +50,7 @@ class W4:
         q = q.permute(0, 3, 1, 4, 2, 5).reshape(rows * _TILE, chunks * _CHUNK)[:n, :k]
 
         def by_group(t):
-            return None if t is None else t.transpose(1, 2).reshape(rows * _TILE, -1)[:n, :k // self.group].contiguous()
+            return None if t is None else t.transpose(1, 2).reshape(rows * _TILE, chunks * (_CHUNK // self.group))[:n, :k // self.group].contiguous()
 
         return q.contiguous(), by_group(self.scale), by_group(self.zero)
 
@@ -95,11 +95,11 @@ def pack_w4(q: Tensor, scale: Tensor, zero: Tensor | None = None) -> W4:
     def padded(t, width, dtype):
         full = torch.zeros(rows * _TILE, width, dtype=dtype, device=t.device)
         full[:n, :t.shape[1]] = t
-        return full.view(rows, _TILE, chunks, -1)
+        return full.view(rows, _TILE, chunks, width // chunks)
 
     e = padded(q, chunks * _CHUNK, torch.uint8).view(rows, _TILE, chunks, 4, 4, 8).permute(0, 2, 4, 1, 3, 5)   # [row tile, chunk, g, row, j, e]
     nibbles = e.unflatten(-1, (4, 2)).transpose(-1, -2).flatten(-2)   # by bit of the word: 0, 2, 4, 6, 1, 3, 5, 7
-    packed = (nibbles[..., ::2] | nibbles[..., 1::2] << 4).reshape(rows, chunks, -1)
+    packed = (nibbles[..., ::2] | nibbles[..., 1::2] << 4).reshape(rows, chunks, _TILE * _CHUNK // 2)
     scales = padded(scale, chunks * per, torch.bfloat16).transpose(1, 2).contiguous()
     zeros = None if zero is None else padded(zero, chunks * per, torch.uint8).transpose(1, 2).contiguous()
     return W4(packed, scales, zeros, (n, k), group)
