@@ -43,3 +43,17 @@ def test_products_without_outputs():
     for rows in (0, 1, 40, 200):
         assert tk.linear_w4(torch.zeros(rows, 96, dtype=BF, device=DEV), w).shape == (rows, 0)
     assert w.dequantize().shape == (0, 96)
+
+
+def test_a_module_on_the_meta_device():
+    """As other modules: made without memory, filled from a state dict."""
+    from triton_kernels.modules import LinearW4
+
+    lin = LinearW4(96, 40, group=32, zero_points=True, device="meta")
+    assert lin.packed.is_meta and lin.weight.shape == (40, 96)
+    from_weight = LinearW4.from_linear(torch.nn.Linear(96, 40), 32, True)
+    lin.load_state_dict(from_weight.state_dict(), assign=True)
+    assert all(torch.equal(a, b) for a, b in zip(lin.weight.unpack(), from_weight.weight.unpack())) and not lin.bias.requires_grad
+    # one that is not filled is a weight of zeros
+    q, scale, zero = LinearW4(96, 40, group=32).weight.unpack()
+    assert zero is None and bool((scale == 0).all()) and q.shape == (40, 96)

@@ -38,6 +38,15 @@ class W4:
             assert t is None or (t.dtype == dtype and t.shape == (*tiles, _TILE, _CHUNK // self.group) and t.is_contiguous()), "scale and zero are laid out by pack_w4"
         assert self.scale is not None, "scale is laid out by pack_w4"
 
+    @classmethod
+    def zeros(cls, n: int, k: int, group: int = 64, zero_points: bool = False, device=None) -> "W4":
+        """A weight of zeros: scales of 0."""
+        assert group in GROUPS and k % group == 0, f"{k} columns are not whole groups of {GROUPS}"
+        tiles = (-(-n // _TILE), -(-k // _CHUNK))
+        numbers = (*tiles, _TILE, _CHUNK // group)
+        return cls(torch.zeros(*tiles, _TILE * _CHUNK // 2, dtype=torch.uint8, device=device), torch.zeros(numbers, dtype=torch.bfloat16, device=device),
+                   torch.zeros(numbers, dtype=torch.uint8, device=device) if zero_points else None, (n, k), group)
+
     def to(self, device) -> "W4":
         return W4(self.packed.to(device), self.scale.to(device), None if self.zero is None else self.zero.to(device), self.shape, self.group)
 

@@ -114,7 +114,7 @@ class LinearW4(nn.Module):
         super().__init__()
         assert activation in ("", "GELU"), f"an activation of linear_w4, not {activation!r}"
         self.in_features, self.out_features, self.group, self.activation = in_features, out_features, group, activation
-        w = quantize_w4(torch.zeros(out_features, in_features, device=device), group, zero_points)
+        w = W4.zeros(out_features, in_features, group, zero_points, device)
         self.register_buffer("packed", w.packed)
         self.register_buffer("scale", w.scale)
         self.register_buffer("zero", w.zero)
