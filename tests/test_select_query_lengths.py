@@ -124,3 +124,42 @@ def test_native_call_and_launcher(monkeypatch):
     for other in (ends.long(), ends.repeat_interleave(2)[::2]):
         assert not took(monkeypatch, tk.select_blocks, q, k, 3, q_lengths=other)
         assert torch.equal(tk.select_blocks(q, k, 3, q_lengths=other), tk.select_blocks(q, k, 3, q_lengths=ends))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_from_code_that_is_traced(backend):
+    torch._dynamo.reset()
+    q, k = (t.to(DEV) for t in inputs(seeded(5), 2, 2, 2, 300, 300, 64))
+    ends = torch.tensor([300, 70], dtype=torch.int32, device=DEV)
+    fn = lambda q: tk.select_blocks(q * 1.0, k, 2, lengths=ends, q_lengths=ends) + 0  # noqa: E731
+    assert torch.equal(torch.compile(fn, backend=backend)(q), fn(q))
+    torch._dynamo.reset()
+
+
+@pytest.mark.gpu
+def test_two_streams_and_two_graphs_of_one_pool():
+    g = seeded(6)
+    q, k = (t.to(DEV) for t in inputs(g, 2, 2, 1, 700, 64 * 40, 64))
+    far = inputs(g, 2, 2, 1, 700, 64 * 1030, 64)[1].to(DEV)   # (scores in the workspace)
+    ends = [torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([700, 130], [257, 0])]
+    calls = [lambda e=e, t=t: tk.select_blocks(q, t, 9, q_lengths=e) for e in ends for t in (k, far)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(4):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append([c() for c in calls])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for each in got for a, b in zip(each, want))
+    pool, graphs, outs = None, [], []
+    for c in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(c())
+        pool = graph.pool()
+        graphs.append(graph)
+    for _ in range(3):
+        for graph, out, expected_ in zip(graphs, outs, want):
+            graph.replay()
+            assert torch.equal(out, expected_)

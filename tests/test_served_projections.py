@@ -199,3 +199,20 @@ def test_which_blocks_run_fused():
             assert block._projections_in_4_bits() is False
             _set(block, path, LinearW4.from_linear(block.get_submodule(path)))
             assert block._projections_in_4_bits() is (path in rest)
+
+
+@pytest.mark.gpu
+def test_blocks_with_projections_in_4_bits_in_code_that_is_traced():
+    torch._dynamo.reset()
+    g = seeded(7)
+    single, double = _single().to(DEV), _double().to(DEV)
+    x, vec = randn(g, 1, 190, 256, dtype=BF).to(DEV), randn(g, 1, 256, dtype=BF).to(DEV)
+    pe = tk.rope_table(torch.arange(190, dtype=torch.float32, device=DEV)[None, :, None], [64])
+    single.linear1, double.img_mlp[0] = LinearW4.from_linear(single.linear1), LinearW4.from_linear(double.img_mlp[0])
+    with torch.no_grad():
+        for keep in (None, 2):
+            single.sparse_keep = double.sparse_keep = keep
+            assert torch.equal(torch.compile(single, backend="eager")(x, vec, pe), single(x, vec, pe))
+            args = x[:, 40:], x[:, :40], vec, pe
+            assert all(torch.equal(a, b) for a, b in zip(torch.compile(double, backend="eager")(*args), double(*args)))
+    torch._dynamo.reset()
