@@ -53,7 +53,8 @@ int flux_w4_unpack(const flux_w4* w, void* out, void* stream);
  * lengths (int32 [B], or null): keys from lengths[b] on are not there; below 0 counts as 0, beyond Lk as Lk. q_lengths (the same for q and Lq): queries from
  * q_lengths[b] on are in no mean, and a block of none but them names nothing, -1 throughout. Without it all Lq rows of q are in their blocks' means.
  * blocks receives int32 [B, Hq, ceil(Lq / 128), min(keep, ceil(Lk / 64))]: the chosen numbers in ascending order, -1 behind them.
- * The workspace (flux_select_blocks_workspace_bytes; 256-byte aligned) holds the means and scores.
+ * The workspace (flux_select_blocks_workspace_bytes; 256-byte aligned) holds the means, 8 D bytes a block and head, and beyond 1024 blocks of keys scores: 64 KB
+ * for each of them, less where there are fewer than 8192 query blocks and heads.
  * ------------------------------------------------------------------------------------------- */
 enum { FLUX_QUERY_BLOCK = 128, FLUX_KEY_BLOCK = 64, FLUX_SELECT_MOST_BLOCKS = 16384 };
 typedef struct flux_select_blocks_args {

@@ -9,7 +9,7 @@
 // as a product with ones. A group's sum takes its scale behind the product, in fp32: nothing is rounded but y.
 //
 // us among others of its kind: 1 x 18432 x 3072 8.4, with SiLU 8.8 to 10.3 by the box (floor 5.7), 3 x 9216 x 3072 with SiLU 7.5 to 8.2, 1 x 1000 x 1024 3.1 (a launch), 16 x
-// 9216 x 3072 9.0, 24 x 12288 x 3072 12.4 to 12.9, 128 x 9216 x 3072 29, 512 x 9216 x 3072 41, 1000 x 9216 x 3072 67 (15 of them for laying the weights out).
+// 9216 x 3072 9.0, 24 x 12288 x 3072 12.4 to 12.9, 128 x 9216 x 3072 29, 512 x 9216 x 3072 39.5, 1000 x 9216 x 3072 67 (15 of them for laying the weights out).
 #include "common.h"
 #include "../../include/flux_hip_serve.h"
 #include <algorithm>
@@ -625,7 +625,7 @@ static void w4_rows_launch(W4Params p, hipStream_t st) {
 #undef CALL
         return;
     }
-    // More: x fills the LDS of a CU at K = 3072, so workgroups run in rounds of 256. What a round takes there, us, by the rows and row tiles of a workgroup; the form
+    // More: x fills the LDS of a CU at K = 3072, so workgroups run in rounds of 256. What a round takes there (measured at that K alone; with less of it several workgroups share a CU), us, by the rows and row tiles of a workgroup; the form
     // whose rounds take least: 16 x 9216 9.3 (16 rows, 4 tiles), 24 x 3072 8.5 (32 rows, 2 tiles), 24 x 12288 13.4 (32, 4), 64 x 12288 21.2 (64, 4; 24.8 with
     // 32, 4), 128 x 12288 29.2 (64, 8; 33.9 with 32, 4), 128 x 3072 12.4 (32, 4).
     struct Form { int rows, tiles; float us; };

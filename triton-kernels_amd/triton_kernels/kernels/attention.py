@@ -113,7 +113,8 @@ def select_blocks(q: Tensor, k: Tensor, keep: int, *, always: int = 0, lengths: 
     """The blocks of 64 keys that each block of 128 queries attends to: int32 [B, Hq, ceil(Lq / 128), min(keep, ceil(Lk / 64))].
 
     q, k      : bf16 [B, Hq, Lq, D] and [B, Hk, Lk, D] views, heads of 64 or 128; Hq is a multiple of Hk, query head h reads key head h // (Hq // Hk).
-                Up to 16384 blocks of keys
+                Up to 16384 blocks of keys. Each call has memory for the means, 8 D bytes a block and head, and beyond 1024 blocks of keys up to
+                64 KB for each of them
     keep      : how many blocks; all of them where there are no more
     always    : the first `always` blocks (as many of them as `keep` has room for) are among them in any case: the text in front of an image
     lengths   : whole numbers [B] on the GPU, or None: keys from lengths[b] on are not there
